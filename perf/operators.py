@@ -124,7 +124,8 @@ def stands_for(element, scale, inner):
 
 
 def encode(element, scale, fmt):
-    """The bytes of a block-scaled tensor: codes [rows, blocks * 16 or 32], scales [rows, blocks]."""
+    """The bytes of a block-scaled tensor: codes [rows, blocks * 16 or 32], scales [rows, blocks padded to a
+    multiple of 4 with zeros]."""
     if fmt == "mx8":
         codes = element.flatten(1).to(torch.float8_e4m3fn).view(torch.uint8)
     else:
@@ -132,7 +133,7 @@ def encode(element, scale, fmt):
         code = torch.searchsorted(levels, element.abs().contiguous()).to(torch.uint8)
         code = (code | (torch.signbit(element).to(torch.uint8) << 3)).flatten(1)
         codes = code[:, 0::2] | (code[:, 1::2] << 4)
-    return codes.contiguous(), (scale + 127).to(torch.uint8).contiguous()
+    return codes.contiguous(), torch.nn.functional.pad((scale + 127).to(torch.uint8), (0, -scale.shape[1] % 4)).contiguous()
 
 
 def decode(codes, scales, fmt, inner):
@@ -143,7 +144,7 @@ def decode(codes, scales, fmt, inner):
         levels = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=codes.device)
         code = torch.stack([codes & 15, codes >> 4], -1).flatten(1)
         element = torch.where(code >= 8, -levels[(code & 7).long()], levels[(code & 7).long()])
-    return stands_for(element.view(codes.shape[0], -1, BLOCK), scales.to(torch.int32) - 127, inner)
+    return stands_for(element.view(codes.shape[0], -1, BLOCK), scales[:, :blocks(inner)].to(torch.int32) - 127, inner)
 
 
 def activate(act, z):
@@ -344,7 +345,7 @@ def held64(state, fmt, inner):
     else:
         magnitude, negative = codes % 128, codes // 128
     value = levels64(fmt)[magnitude.long()] * (1 - 2 * negative.double())
-    return (value * torch.exp2(scales.double() - 127).repeat_interleave(BLOCK, 1))[:, :inner]
+    return (value * torch.exp2(scales[:, :blocks(inner)].double() - 127).repeat_interleave(BLOCK, 1))[:, :inner]
 
 
 def exact(case, seed):
