@@ -1,0 +1,466 @@
+// Block-scaled ("microscaled") tensors: quantisation, restoration, the 4-bit product, and the two backward
+// operations that read 8-bit checkpoints.  The storage form is described in program.hpp.
+#include "kernels.hpp"
+#include "activation.cuh"
+#include "lowp.cuh"
+#include "tensor_core.cuh"
+
+namespace syn {
+namespace kern {
+
+namespace {
+
+constexpr int MX_THREADS = 256;
+constexpr int MX_WARPS = MX_THREADS / 32;
+
+// Storage type of a floating tensor: 0 FLOAT32, 1 BFLOAT16, 2 FLOAT16 (the KIND of lowp.cuh).
+template <int KIND> struct MxElement { using type = uint16_t; };
+template <> struct MxElement<0> { using type = float; };
+template <int KIND> __device__ __forceinline__ float mx_load(const typename MxElement<KIND>::type *p) {
+    if constexpr (KIND == 0) return *p; else return low_decode<KIND>(*p);
+}
+template <int KIND> __device__ __forceinline__ typename MxElement<KIND>::type mx_narrow(float x) {
+    if constexpr (KIND == 0) return x; else return low_encode<KIND>(x);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Element-wise passes.  A thread owns a group of 8 consecutive elements, four lanes own a block of 32: 16 to 32
+// bytes of the wide tensor per thread and access, the block's largest magnitude by two shuffles.  A row has
+// `per_row` groups, counted over the padded scales (a multiple of 16), so a block never straddles two warps.
+// ------------------------------------------------------------------------------------------------
+struct MxRows {
+    int64_t rows, cols;
+    int64_t per_row, total;         // groups of 8 per row and in all
+    int narrow;                     // total < 2^32: 32-bit division
+};
+
+inline MxRows mx_rows(int64_t rows, int64_t cols) {
+    MxRows r;
+    r.rows = rows; r.cols = cols;
+    r.per_row = mx_scale_bytes(cols) * 4; r.total = rows * r.per_row;
+    r.narrow = r.total < (1ll << 32);
+    return r;
+}
+
+struct MxSpot { int64_t row, first; int count; };      // a group: its row, its first column, how many of its 8 columns exist
+
+__device__ __forceinline__ MxSpot mx_spot(const MxRows &r, int64_t g) {
+    MxSpot s;
+    if (g >= r.total) { s.row = 0; s.first = r.cols; s.count = 0; return s; }
+    if (r.rows == 1) s.row = 0;
+    else if (r.narrow) s.row = (uint32_t)g / (uint32_t)r.per_row;
+    else s.row = g / r.per_row;
+    s.first = (g - s.row * r.per_row) * 8;
+    const int64_t left = r.cols - s.first;
+    s.count = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    return s;
+}
+
+// Eight elements from 16-byte aligned memory.
+template <int KIND> __device__ __forceinline__ void mx_load8(const typename MxElement<KIND>::type *p, float (&v)[8]) {
+    if constexpr (KIND == 0) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = low_decode<KIND>((uint16_t)(u[i] & 0xffffu)); v[2 * i + 1] = low_decode<KIND>((uint16_t)(u[i] >> 16)); }
+    }
+}
+template <int KIND> __device__ __forceinline__ void mx_store8(typename MxElement<KIND>::type *p, const float (&v)[8]) {
+    if constexpr (KIND == 0) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] = (uint32_t)low_encode<KIND>(v[2 * i]) | ((uint32_t)low_encode<KIND>(v[2 * i + 1]) << 16);
+        *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+// Rows that do not start on 16 bytes: the warp reads (writes) its 256 elements 32 consecutive ones at a time and
+// hands them over through its part of shared memory; a thread per group would touch every line eight times.
+// `offset`: element offset of this lane's group, `step`: distance of consecutive columns.
+template <int KIND> __device__ __forceinline__ void mx_gather8(const typename MxElement<KIND>::type *p, int64_t offset, int64_t step, int count,
+                                                                float *box, int lane, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int owner = i * 4 + (lane >> 3);
+        const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
+        const int have = __shfl_sync(0xffffffffu, count, owner);
+        box[i * 32 + lane] = (lane & 7) < have ? mx_load<KIND>(p + at + (lane & 7) * step) : 0.0f;
+    }
+    __syncwarp();
+    const float4 a = *reinterpret_cast<const float4 *>(box + lane * 8), b = *reinterpret_cast<const float4 *>(box + lane * 8 + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    __syncwarp();
+}
+template <int KIND> __device__ __forceinline__ void mx_scatter8(typename MxElement<KIND>::type *p, int64_t offset, int count, float *box, int lane, const float (&v)[8]) {
+    *reinterpret_cast<float4 *>(box + lane * 8) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(box + lane * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int owner = i * 4 + (lane >> 3);
+        const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
+        const int have = __shfl_sync(0xffffffffu, count, owner);
+        if ((lane & 7) < have) p[at + (lane & 7)] = mx_narrow<KIND>(box[i * 32 + lane]);
+    }
+    __syncwarp();
+}
+
+// The byte of the least scale 2^(byte - 127) under which `largest` (the bit pattern of a finite magnitude) fits:
+// with largest = 1.f * 2^(E - 127), 6 = 1.5 * 2^2 and 448 = 1.75 * 2^8, that is E - 2 or E - 8, one more when the
+// mantissa exceeds the element type's, and at least 0.  255 for an infinity or a NaN.
+template <int FORMAT> __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t largest) {
+    if (largest >= 0x7f800000u) return 255u;
+    const int e = (int)(largest >> 23);
+    const int b = FORMAT == 4 ? e - 2 + ((largest & 0x7fffffu) > 0x400000u) : e - 8 + ((largest & 0x7fffffu) > 0x600000u);
+    return (uint32_t)(b < 0 ? 0 : b);
+}
+// 2^(byte - 127), NaN for 255.
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+    return byte == 255u ? __uint_as_float(0x7fffffffu) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+__device__ __forceinline__ void low_unpack_half2(uint32_t h, float &a, float &b) {
+    a = low_decode<2>((uint16_t)(h & 0xffffu)); b = low_decode<2>((uint16_t)(h >> 16));
+}
+// Two values, already under their scale, as one byte of E2M1 or two of E4M3; the first in the low part.
+__device__ __forceinline__ uint32_t mx_encode4x2(float a, float b) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t mx_encode8x2(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void mx_decode4x2(uint32_t byte, float &a, float &b) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(byte));
+    low_unpack_half2(h, a, b);
+}
+__device__ __forceinline__ void mx_decode8x2(uint32_t bytes, float &a, float &b) {
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)bytes));
+    low_unpack_half2(h, a, b);
+}
+
+// x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.
+template <int FORMAT, int KIND, bool VEC>
+__global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows r, int64_t row_step, int even,
+                                                                 uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
+    const int lane = threadIdx.x & 31;
+    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK * FORMAT / 8, scale_pitch = r.per_row / 4;
+    // the bound is a multiple of 32, so that whole warps take part in the shuffles
+    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
+        const MxSpot at = mx_spot(r, g);
+        float v[8];
+        int64_t base = at.row * row_step;
+        if (!VEC && !even) {
+            const int64_t r2 = at.row % ix.shape[2], rest = at.row / ix.shape[2];
+            base = r2 * ix.sa[2] + rest % ix.shape[1] * ix.sa[1] + rest / ix.shape[1] * ix.sa[0];
+        }
+        if constexpr (VEC) {
+            if (at.count == 8) mx_load8<KIND>(x + base + at.first, v);
+            else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = i < at.count ? mx_load<KIND>(x + base + at.first + i) : 0.0f;
+            }
+        } else {
+            mx_gather8<KIND>(x, base + at.first * ix.sa[3], ix.sa[3], at.count, boxes[threadIdx.x >> 5], lane, v);
+        }
+        uint32_t largest = 0;       // bit patterns of magnitudes order like the magnitudes, NaN above infinity
+#pragma unroll
+        for (int i = 0; i < 8; i++) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        if (g >= r.total) continue;
+        const int64_t group = at.first >> 3;
+        const bool exists = (at.first & ~(int64_t)(MX_BLOCK - 1)) < r.cols;     // else: padding of the scales
+        const uint32_t byte = exists ? mx_scale_byte<FORMAT>(largest) : 0u;
+        if ((lane & 3) == 0) scales[at.row * scale_pitch + (group >> 2)] = (uint8_t)byte;
+        if (!exists) continue;
+        // the inverse scale 2^(127 - byte) is a normal number for every byte that occurs; a product with it is
+        // exact, or below half the smallest element
+        const float inverse = __uint_as_float((254u - byte) << 23);
+        if (byte == 255u) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 0.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] *= inverse;
+        }
+        uint8_t *dst = codes + at.row * code_pitch + group * FORMAT;
+        if constexpr (FORMAT == 4) {
+            *reinterpret_cast<uint32_t *>(dst) = mx_encode4x2(v[0], v[1]) | mx_encode4x2(v[2], v[3]) << 8 | mx_encode4x2(v[4], v[5]) << 16 | mx_encode4x2(v[6], v[7]) << 24;
+        } else {
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(mx_encode8x2(v[0], v[1]) | mx_encode8x2(v[2], v[3]) << 16, mx_encode8x2(v[4], v[5]) | mx_encode8x2(v[6], v[7]) << 16);
+        }
+    }
+}
+
+// The eight values of a group; the caller has checked that its block exists.
+template <int FORMAT> __device__ __forceinline__ void mx_values8(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t code_pitch,
+                                                                 int64_t scale_pitch, const MxSpot &at, float (&v)[8]) {
+    const int64_t group = at.first >> 3;
+    const float scale = mx_scale_value(scales[at.row * scale_pitch + (group >> 2)]);
+    const uint8_t *src = codes + at.row * code_pitch + group * FORMAT;
+    if constexpr (FORMAT == 4) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
+#pragma unroll
+        for (int i = 0; i < 4; i++) mx_decode4x2(w >> (8 * i) & 0xffu, v[2 * i], v[2 * i + 1]);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(src);
+        mx_decode8x2(w.x & 0xffffu, v[0], v[1]); mx_decode8x2(w.x >> 16, v[2], v[3]);
+        mx_decode8x2(w.y & 0xffffu, v[4], v[5]); mx_decode8x2(w.y >> 16, v[6], v[7]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] *= scale;
+}
+
+template <int FORMAT, int KIND, bool VEC>
+__global__ void __launch_bounds__(MX_THREADS) mx_restore_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxRows r,
+                                                                typename MxElement<KIND>::type *__restrict__ out) {
+    __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
+    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK * FORMAT / 8, scale_pitch = r.per_row / 4;
+    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
+        const MxSpot at = mx_spot(r, g);
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (at.count > 0) mx_values8<FORMAT>(codes, scales, code_pitch, scale_pitch, at, v);
+        const int64_t offset = at.row * r.cols + at.first;
+        if constexpr (VEC) { if (at.count) mx_store8<KIND>(out + offset, v); }      // rows are whole groups here
+        else mx_scatter8<KIND>(out, offset, at.count, boxes[threadIdx.x >> 5], threadIdx.x & 31, v);
+    }
+}
+
+// act'(z) in FLOAT32.  exp(-|z|) keeps every form free of overflow and of cancellation against 1.  Where |z| is
+// above 120 the exponentials are below the smallest number and the slope is 0 or 1 (an infinity, which a scale near
+// the end of its range can make of a finite value, included); NaN stays NaN.
+__device__ __forceinline__ float mx_slope(int act, float z) {
+    if (z != z) return z;
+    if (act == (int)Op::RELU || fabsf(z) > 120.0f) {
+        if (act == (int)Op::TANH || act == (int)Op::SIGMOID) return 0.0f;
+        return z > 0.0f ? 1.0f : 0.0f;
+    }
+    switch ((Op)act) {
+        case Op::TANH: { const float e = expf(-2.0f * fabsf(z)), d = 1.0f + e; return __fdividef(4.0f * e, d * d); }
+        case Op::SIGMOID: { const float e = expf(-fabsf(z)), d = 1.0f + e; return __fdividef(e, d * d); }
+        case Op::SILU: {
+            const float e = expf(-fabsf(z)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
+            const float s = z >= 0.0f ? near : far, t = z >= 0.0f ? far : near;      // sigmoid(z) and 1 - sigmoid(z)
+            return s * fmaf(z, t, 1.0f);
+        }
+        case Op::GELU_TANH: {       // z sigmoid(2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+            const float c = 1.5957691216057308f, zz = z * z;
+            const float u = c * z * fmaf(0.044715f, zz, 1.0f);
+            const float e = expf(-fabsf(u)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
+            const float s = u >= 0.0f ? near : far;
+            return fmaf(z * (near * far), c * fmaf(0.134145f, zz, 1.0f), s);
+        }
+        default:                    // GELU: Phi(z) + z phi(z)
+            return fmaf(0.3989422804014327f * z, expf(-0.5f * z * z), 0.5f * erfcf(-0.7071067811865476f * z));
+    }
+}
+
+// dz = g * act'(z).  A closed ReLU gate gives 0 whatever g holds, like the WHERE of the ordinary gradient rule; a
+// block of NaN gives NaN, so that a step over it is refused rather than taken without its gradient.
+template <int KIND, bool VEC>
+__global__ void __launch_bounds__(MX_THREADS) mx_activation_gradient_kernel(int act, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                                            const typename MxElement<KIND>::type *__restrict__ g_in, MxRows r,
+                                                                            typename MxElement<KIND>::type *__restrict__ out) {
+    __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
+    const int lane = threadIdx.x & 31;
+    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK, scale_pitch = r.per_row / 4;
+    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
+        const MxSpot at = mx_spot(r, g);
+        const int64_t offset = at.row * r.cols + at.first;
+        float z[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, up[8];
+        if constexpr (VEC) { if (at.count) mx_load8<KIND>(g_in + offset, up); }
+        else mx_gather8<KIND>(g_in, offset, 1, at.count, boxes[threadIdx.x >> 5], lane, up);
+        if (at.count > 0) mx_values8<8>(codes, scales, code_pitch, scale_pitch, at, z);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (act == (int)Op::RELU) z[i] = z[i] > 0.0f ? up[i] : z[i] != z[i] ? z[i] : 0.0f;
+            else z[i] = up[i] * mx_slope(act, z[i]);
+        }
+        if constexpr (VEC) { if (at.count) mx_store8<KIND>(out + offset, z); }
+        else mx_scatter8<KIND>(out, offset, at.count, boxes[threadIdx.x >> 5], lane, z);
+    }
+}
+
+int mx_grid(const MxRows &r) {
+    const int64_t blocks = (r.total + MX_THREADS - 1) / MX_THREADS;
+    return (int)(blocks < 148 * 8 ? (blocks < 1 ? 1 : blocks) : 148 * 8);
+}
+
+// ------------------------------------------------------------------------------------------------
+// 4-bit product, one warp per result: lanes take the blocks of the contraction in turn.  Twice an E2M1 value is an
+// integer, so a block's sum of products is exact in an integer.
+// ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int mx_twice4(uint32_t code) {
+    const int magnitude = (int)(0xC8643210u >> (4 * (code & 7u)) & 15u);
+    return code & 8u ? -magnitude : magnitude;
+}
+
+// Activations of a FLOAT32 sum before its one rounding.
+__device__ __forceinline__ float mx_activate(int act, float z) { return activation_value(act, z); }
+
+template <int KIND>
+__global__ void __launch_bounds__(MX_THREADS) mx_linear_simple_kernel(int act, int64_t m, int64_t n, int64_t k, const uint8_t *__restrict__ x, const uint8_t *__restrict__ xs,
+                                                                      const uint8_t *__restrict__ w, const uint8_t *__restrict__ ws,
+                                                                      const typename MxElement<KIND>::type *__restrict__ bias, typename MxElement<KIND>::type *__restrict__ out) {
+    const int lane = threadIdx.x & 31;
+    const int64_t blocks = k / MX_BLOCK, scale_pitch = (blocks + 3) / 4 * 4;
+    for (int64_t i = blockIdx.x * (int64_t)MX_WARPS + (threadIdx.x >> 5); i < m * n; i += (int64_t)gridDim.x * MX_WARPS) {
+        const int64_t row = i / n, col = i - row * n;
+        float sum = 0.0f;
+        for (int64_t b = lane; b < blocks; b += 32) {
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(x + row * (k / 2) + b * 16), *q = reinterpret_cast<const uint32_t *>(w + col * (k / 2) + b * 16);
+            int dot = 0;
+            for (int j = 0; j < 4; j++)
+                for (int e = 0; e < 32; e += 4) dot += mx_twice4(p[j] >> e) * mx_twice4(q[j] >> e);
+            sum += (float)dot * 0.25f * mx_scale_value(xs[row * scale_pitch + b]) * mx_scale_value(ws[col * scale_pitch + b]);
+        }
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) out[i] = mx_narrow<KIND>(mx_activate(act, sum + (bias ? mx_load<KIND>(bias + col) : 0.0f)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Weight gradient from an 8-bit checkpoint, one thread per result.
+// ------------------------------------------------------------------------------------------------
+template <int KIND>
+__global__ void __launch_bounds__(MX_THREADS) mx_weight_gradient_simple_kernel(int64_t rows, int64_t n, int64_t k, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                                               const typename MxElement<KIND>::type *__restrict__ g, float *__restrict__ out) {
+    const int64_t code_pitch = mx_blocks(k) * MX_BLOCK, scale_pitch = mx_scale_bytes(k);
+    for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i < n * k; i += (int64_t)gridDim.x * MX_THREADS) {
+        const int64_t col = i / k, feature = i - col * k;
+        double sum = 0.0;
+        for (int64_t r = 0; r < rows; r++) {
+            float a, b;
+            mx_decode8x2(codes[r * code_pitch + feature], a, b);
+            sum += (double)(a * mx_scale_value(scales[r * scale_pitch + feature / MX_BLOCK])) * (double)mx_load<KIND>(g + r * n + col);
+        }
+        out[i] = (float)sum;
+    }
+}
+
+}  // namespace
+
+#define MX_KINDS(dtype, CALL) ((dtype) == DType::F32 ? CALL(0) : (dtype) == DType::BF16 ? CALL(1) : (dtype) == DType::F16 ? CALL(2) : cudaErrorInvalidValue)
+
+template <int FORMAT, int KIND>
+static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales) {
+    using T = typename MxElement<KIND>::type;
+    const int64_t rows = ix.shape[0] * ix.shape[1] * ix.shape[2], cols = ix.shape[3];
+    if (rows == 0 || cols == 0) return cudaSuccess;
+    // the rows lie at one distance when each leading axis continues the next
+    bool even = true;
+    int64_t row_step = 0, extent = 1;
+    for (int d = 2; d >= 0; d--) {
+        if (ix.shape[d] == 1) continue;
+        if (extent == 1) row_step = ix.sa[d];
+        else even &= ix.sa[d] == row_step * extent;
+        extent *= ix.shape[d];
+    }
+    const bool vec = even && (ix.sa[3] == 1 || cols == 1) && ((uintptr_t)x & 15) == 0 && (rows == 1 || row_step * (int64_t)sizeof(T) % 16 == 0);
+    // dense rows of whole scale words are one long row
+    const bool flat = vec && row_step == cols && cols % (4 * MX_BLOCK) == 0;
+    const MxRows r = flat ? mx_rows(1, rows * cols) : mx_rows(rows, cols);
+    if (vec) mx_quantize_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, 1, codes, scales);
+    else mx_quantize_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, even, codes, scales);
+    return cudaGetLastError();
+}
+
+cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales) {
+#define CALL4(KIND) launch_mx_quantize<4, KIND>(s, x, ix, codes, scales)
+#define CALL8(KIND) launch_mx_quantize<8, KIND>(s, x, ix, codes, scales)
+    return format == 4 ? MX_KINDS(dtype, CALL4) : format == 8 ? MX_KINDS(dtype, CALL8) : cudaErrorInvalidValue;
+#undef CALL4
+#undef CALL8
+}
+
+// Groups of a dense [rows, cols] tensor beside a block-scaled one of the same shape, and whether all of them are
+// whole and aligned.
+template <typename T> static MxRows dense_groups(int64_t rows, int64_t cols, const void *a, const void *b, bool &vec) {
+    vec = cols % 8 == 0 && ((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0;
+    return vec && cols % (4 * MX_BLOCK) == 0 ? mx_rows(1, rows * cols) : mx_rows(rows, cols);
+}
+
+template <int FORMAT, int KIND>
+static cudaError_t launch_mx_restore(cudaStream_t s, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *out) {
+    using T = typename MxElement<KIND>::type;
+    if (rows == 0 || cols == 0) return cudaSuccess;
+    bool vec;
+    const MxRows r = dense_groups<T>(rows, cols, out, out, vec);
+    if (vec) mx_restore_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>(codes, scales, r, (T *)out);
+    else mx_restore_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>(codes, scales, r, (T *)out);
+    return cudaGetLastError();
+}
+
+cudaError_t mx_restore(cudaStream_t s, int format, DType dtype, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *out) {
+#define CALL4(KIND) launch_mx_restore<4, KIND>(s, codes, scales, rows, cols, out)
+#define CALL8(KIND) launch_mx_restore<8, KIND>(s, codes, scales, rows, cols, out)
+    return format == 4 ? MX_KINDS(dtype, CALL4) : format == 8 ? MX_KINDS(dtype, CALL8) : cudaErrorInvalidValue;
+#undef CALL4
+#undef CALL8
+}
+
+template <int KIND>
+static cudaError_t launch_mx_activation_gradient(cudaStream_t s, int act, const uint8_t *codes, const uint8_t *scales, const void *g, int64_t rows, int64_t cols, void *out) {
+    using T = typename MxElement<KIND>::type;
+    if (rows == 0 || cols == 0) return cudaSuccess;
+    bool vec;
+    const MxRows r = dense_groups<T>(rows, cols, g, out, vec);
+    if (vec) mx_activation_gradient_kernel<KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>(act, codes, scales, (const T *)g, r, (T *)out);
+    else mx_activation_gradient_kernel<KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>(act, codes, scales, (const T *)g, r, (T *)out);
+    return cudaGetLastError();
+}
+
+cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const uint8_t *codes, const uint8_t *scales, const void *g,
+                                   int64_t rows, int64_t cols, void *out) {
+#define CALL(KIND) launch_mx_activation_gradient<KIND>(s, act, codes, scales, g, rows, cols, out)
+    return MX_KINDS(dtype, CALL);
+#undef CALL
+}
+
+template <int KIND>
+static cudaError_t launch_mx_linear(cudaStream_t s, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
+                                    const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out) {
+    using T = typename MxElement<KIND>::type;
+    const int64_t blocks = (m * n + MX_WARPS - 1) / MX_WARPS;
+    mx_linear_simple_kernel<KIND><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(act, m, n, k, x, x_scales, w, w_scales, (const T *)bias, (T *)out);
+    return cudaGetLastError();
+}
+
+cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
+                      const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out, int sm_count, int *error_word) {
+    if (m == 0 || n == 0) return cudaSuccess;
+#define CALL(KIND) launch_mx_linear<KIND>(s, act, m, n, k, x, x_scales, w, w_scales, bias, out)
+    return MX_KINDS(dtype, CALL);
+#undef CALL
+}
+
+template <int KIND>
+static cudaError_t launch_mx_weight_gradient(cudaStream_t s, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales, const void *g, float *out) {
+    using T = typename MxElement<KIND>::type;
+    const int64_t blocks = (n * k + MX_THREADS - 1) / MX_THREADS;
+    mx_weight_gradient_simple_kernel<KIND><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(rows, n, k, codes, scales, (const T *)g, out);
+    return cudaGetLastError();
+}
+
+cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
+                               const void *g, float *out, int sm_count, int *error_word) {
+    if (n == 0 || k == 0) return cudaSuccess;
+#define CALL(KIND) launch_mx_weight_gradient<KIND>(s, rows, n, k, codes, scales, g, out)
+    return MX_KINDS(dtype, CALL);
+#undef CALL
+}
+
+}  // namespace kern
+}  // namespace syn

@@ -20,6 +20,11 @@
 //   MSE            a, b -> out scalar
 //   ARG_MAX        a [m,n] -> out [m] INT64
 //   RELU_BACKWARD  a = gate source, b = upstream gradient -> out
+//   MX_QUANTIZE    a [rows m, n] (any view) -> out = codes, out2 = scales (scalar_bits = format)
+//   MX_RESTORE     a, scale_a = codes and scales of [m, n] -> out (scalar_bits = format)
+//   MX_LINEAR      a, scale_a = left [m, k], b, scale_b = weight [n, k], bias = [n] or -1 -> out (act)
+//   MX_WEIGHT_GRADIENT      a, scale_a = checkpoint [m, k], b = upstream gradient [m, n] -> out [n, k]
+//   MX_ACTIVATION_GRADIENT  a, scale_a = checkpoint [m, n], b = upstream gradient [m, n] -> out (act)
 #include "lowering.hpp"
 #include "kernels.hpp"
 
@@ -43,6 +48,8 @@ const char *step_name(StepKind k) {
         case StepKind::UNARY: return "unary"; case StepKind::WHERE: return "where"; case StepKind::ONE_HOT: return "one_hot";
         case StepKind::COPY: return "copy"; case StepKind::ROW_REDUCE: return "row_reduce"; case StepKind::FULL_SUM: return "full_sum";
         case StepKind::COLSUM: return "colsum"; case StepKind::SOFTMAX: return "softmax"; case StepKind::CROSS_ENTROPY: return "cross_entropy"; case StepKind::DENSE_CROSS_ENTROPY: return "dense_cross_entropy"; case StepKind::DENSE_CE_BACKWARD: return "dense_cross_entropy_backward"; case StepKind::SOFTMAX_BACKWARD: return "softmax_backward";
+        case StepKind::MX_QUANTIZE: return "mx_quantize"; case StepKind::MX_RESTORE: return "mx_restore"; case StepKind::MX_LINEAR: return "mx_linear";
+        case StepKind::MX_WEIGHT_GRADIENT: return "mx_weight_gradient"; case StepKind::MX_ACTIVATION_GRADIENT: return "mx_activation_gradient";
         case StepKind::MSE: return "mse"; case StepKind::ARG_MAX: return "arg_max"; case StepKind::RELU_BACKWARD: return "relu_backward";
     }
     return "?";
@@ -799,6 +806,13 @@ Status lower_program(const Program &source, const LoweringOptions &options, Plan
         return -1;
     };
 
+    // codes or scales of a block-scaled tensor: dense, and where TMA and 16-byte loads can read them
+    auto mx_bytes = [&](int v) {
+        if (plan.views[v].dense() && plan.views[v].offset % 16 == 0) return true;
+        message = "codes or scales that are not dense or do not start on a multiple of 16 bytes";
+        return false;
+    };
+
     // engine and operand checks of one GEMM step whose views are assigned
     auto prepare_gemm = [&](Step &st) -> Status {
         {
@@ -1075,6 +1089,45 @@ Status lower_program(const Program &source, const LoweringOptions &options, Plan
                 st.kind = StepKind::ARG_MAX; st.a = in0; st.out = out0; st.m = g.values[in0].shape[0]; st.n = g.values[in0].shape[1];
                 finish_step(st);
                 break;
+            case Op::MX_QUANTIZE:
+                for (int v : n.outputs) assign_output(v);
+                st.kind = StepKind::MX_QUANTIZE; st.a = in0; st.out = out0; st.out2 = n.outputs[1];
+                st.n = g.values[in0].shape.back(); st.m = g.values[in0].elements() / st.n;
+                st.scalar_bits = n.attrs[0];
+                finish_step(st);
+                break;
+            case Op::MX_RESTORE:
+                if (!mx_bytes(in0) || !mx_bytes(n.inputs[1])) return UNSUPPORTED_SHAPE;
+                assign_output(out0);
+                st.kind = StepKind::MX_RESTORE; st.a = in0; st.scale_a = n.inputs[1]; st.out = out0;
+                st.n = ov.shape.back(); st.m = ov.elements() / st.n;
+                st.scalar_bits = n.attrs[0];
+                finish_step(st);
+                break;
+            case Op::MX_LINEAR:
+                for (int i = 0; i < 4; i++) if (!mx_bytes(n.inputs[i])) return UNSUPPORTED_SHAPE;
+                if (n.inputs.size() == 5) { st.bias = n.inputs[4]; if (dense_input(st.bias) < 0) return UNSUPPORTED_SHAPE; }
+                assign_output(out0);
+                st.kind = StepKind::MX_LINEAR; st.a = in0; st.scale_a = n.inputs[1]; st.b = n.inputs[2]; st.scale_b = n.inputs[3]; st.out = out0;
+                st.n = ov.shape.back(); st.m = ov.elements() / st.n; st.k = g.values[in0].shape.back() * 2;
+                st.act = (int)n.attrs[0];
+                finish_step(st);
+                break;
+            case Op::MX_WEIGHT_GRADIENT:
+                if (!mx_bytes(in0) || !mx_bytes(n.inputs[1]) || dense_input(n.inputs[2]) < 0) return UNSUPPORTED_SHAPE;
+                assign_output(out0);
+                st.kind = StepKind::MX_WEIGHT_GRADIENT; st.a = in0; st.scale_a = n.inputs[1]; st.b = n.inputs[2]; st.out = out0;
+                st.n = ov.shape[0]; st.k = ov.shape[1]; st.m = g.values[st.b].elements() / st.n;
+                finish_step(st);
+                break;
+            case Op::MX_ACTIVATION_GRADIENT:
+                if (!mx_bytes(in0) || !mx_bytes(n.inputs[1]) || dense_input(n.inputs[2]) < 0) return UNSUPPORTED_SHAPE;
+                assign_output(out0);
+                st.kind = StepKind::MX_ACTIVATION_GRADIENT; st.a = in0; st.scale_a = n.inputs[1]; st.b = n.inputs[2]; st.out = out0;
+                st.n = ov.shape.back(); st.m = ov.elements() / st.n;
+                st.act = (int)n.attrs[0];
+                finish_step(st);
+                break;
         }
     }
     // publications that are views of something else (a feed, a shared intermediate) are copied out
@@ -1117,6 +1170,9 @@ std::string describe_plan(const Program &g, const Plan &plan) {
         } else if (st.kind == StepKind::CROSS_ENTROPY) {
             os << " rows=" << st.m << " classes=" << st.n << (st.out >= 0 ? " loss" : "") << (st.out2 >= 0 ? " gradient" : "") << (st.out3 >= 0 ? " arg_max" : "");
         }
+        if (st.kind == StepKind::MX_QUANTIZE || st.kind == StepKind::MX_RESTORE) os << " bits=" << st.scalar_bits;
+        if (st.kind == StepKind::MX_LINEAR || st.kind == StepKind::MX_WEIGHT_GRADIENT) os << " k=" << st.k << (st.bias >= 0 ? " bias" : "");
+        if (st.kind >= StepKind::MX_LINEAR && st.act) os << " act=" << op_name((Op)st.act);
         if (st.kind != StepKind::GEMM && st.kind != StepKind::CROSS_ENTROPY && st.m) os << " m=" << st.m << " n=" << st.n;
         os << " nodes=[";
         for (size_t i = 0; i < st.nodes.size(); i++) os << (i ? "," : "") << op_name(g.nodes[st.nodes[i]].op);

@@ -40,7 +40,8 @@ struct View {
 
 enum class StepKind : int {
     GEMM, BINARY, SCALAR, UNARY, WHERE, ONE_HOT, COPY, ROW_REDUCE, FULL_SUM, COLSUM, SOFTMAX,
-    CROSS_ENTROPY, MSE, ARG_MAX, RELU_BACKWARD, DENSE_CROSS_ENTROPY, DENSE_CE_BACKWARD, SOFTMAX_BACKWARD
+    CROSS_ENTROPY, MSE, ARG_MAX, RELU_BACKWARD, DENSE_CROSS_ENTROPY, DENSE_CE_BACKWARD, SOFTMAX_BACKWARD,
+    MX_QUANTIZE, MX_RESTORE, MX_LINEAR, MX_WEIGHT_GRADIENT, MX_ACTIVATION_GRADIENT
 };
 const char *step_name(StepKind k);
 
@@ -53,6 +54,7 @@ struct Step {
     int a = -1, b = -1, c = -1;     // input value ids (meaning per kind, see lowering.cpp)
     int out = -1, out2 = -1, out3 = -1;   // output value ids
     int bias = -1, mask = -1;       // GEMM epilogue operands
+    int scale_a = -1, scale_b = -1; // scale bytes of block-scaled operands a and b
     bool relu = false;
     int act = 0;                    // GEMM epilogue activation other than ReLU: the wire code of TANH, SIGMOID, SILU, GELU_TANH or GELU
     int64_t m = 0, n = 0, k = 0;    // GEMM extents, or rows / cols of row kernels

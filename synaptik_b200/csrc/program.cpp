@@ -24,6 +24,8 @@ const char *op_name(Op op) {
         case Op::CLAMP: return "CLAMP"; case Op::LT: return "LT"; case Op::EQ: return "EQ";
         case Op::SCALAR_SUB: return "SCALAR_SUB"; case Op::GELU: return "GELU"; case Op::ERF: return "ERF";
         case Op::DENSE_CROSS_ENTROPY: return "DENSE_CATEGORICAL_CROSS_ENTROPY_WITH_LOGITS";
+        case Op::MX_QUANTIZE: return "MX_QUANTIZE"; case Op::MX_RESTORE: return "MX_RESTORE"; case Op::MX_LINEAR: return "MX_LINEAR";
+        case Op::MX_WEIGHT_GRADIENT: return "MX_WEIGHT_GRADIENT"; case Op::MX_ACTIVATION_GRADIENT: return "MX_ACTIVATION_GRADIENT";
     }
     return "?";
 }
@@ -74,6 +76,28 @@ bool expands_to(const std::vector<int64_t> &from, const std::vector<int64_t> &to
 }
 
 #define FAIL(status, text) do { std::ostringstream os_; os_ << text; message = os_.str(); return status; } while (0)
+
+// The two byte tensors of a block-scaled tensor of the given shape.
+Status check_mx_pair(const Value &codes, const Value &scales, const std::vector<int64_t> &shape, int64_t format, const char *name, std::string &message) {
+    if (codes.dtype != DType::U8 || scales.dtype != DType::U8) FAIL(UNSUPPORTED_OPERATION, name << ": codes and scales are U8");
+    if (shape.back() < 1) FAIL(UNSUPPORTED_SHAPE, name << ": empty last axis");
+    if (shape.back() >= (1ll << 30)) FAIL(UNSUPPORTED_SHAPE, name << ": last axis of 2^30 or more");
+    std::vector<int64_t> want = shape;
+    want.back() = mx_code_bytes(format, shape.back());
+    if (codes.shape != want) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape of the codes");
+    want.back() = mx_scale_bytes(shape.back());
+    if (scales.shape != want) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape of the scales");
+    // kernels read them with TMA and in 16-byte groups
+    if (codes.offset % 16 || scales.offset % 16) FAIL(UNSUPPORTED_SHAPE, name << ": codes and scales start on a multiple of 16 bytes");
+    return OK;
+}
+
+bool mx_activation(uint64_t code, bool none_allowed) {
+    switch ((Op)code) {
+        case Op::RELU: case Op::TANH: case Op::SIGMOID: case Op::SILU: case Op::GELU_TANH: case Op::GELU: return true;
+        default: return none_allowed && code == 0;
+    }
+}
 
 Status check_node(const Program &g, int index, std::string &message) {
     const Node &n = g.nodes[index];
@@ -133,7 +157,7 @@ Status check_node(const Program &g, int index, std::string &message) {
         case Op::SCALAR_MUL: case Op::SCALAR_MIN: case Op::SCALAR_MAX: case Op::SCALAR_SUB:
             if (!need(1, 1) || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
             if (in(0).dtype != out(0).dtype || in(0).shape != out(0).shape) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape or dtype");
-            if (in(0).dtype == DType::BOOL || (n.op == Op::SCALAR_MUL && in(0).dtype != DType::F32)) FAIL(UNSUPPORTED_OPERATION, name << ": dtype");
+            if (in(0).dtype == DType::BOOL || in(0).dtype == DType::U8 || (n.op == Op::SCALAR_MUL && in(0).dtype != DType::F32)) FAIL(UNSUPPORTED_OPERATION, name << ": dtype");
             return OK;
         case Op::CLAMP:
             if (!need(1, 1) || n.attrs.size() != 2) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
@@ -262,6 +286,56 @@ Status check_node(const Program &g, int index, std::string &message) {
             if (out(0).elements() != in(0).shape[0]) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape");
             return OK;
         }
+        case Op::MX_QUANTIZE: {
+            if (!need(1, 2) || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (n.attrs[0] != 4 && n.attrs[0] != 8) FAIL(UNSUPPORTED_OPERATION, name << ": formats of 4 or 8 bits");
+            if (!dtype_floating(in(0).dtype) || out(0).dtype != DType::U8 || out(1).dtype != DType::U8) FAIL(UNSUPPORTED_OPERATION, name << ": needs a floating input and U8 results");
+            if (in(0).shape.empty() || in(0).shape.size() > 4) FAIL(UNSUPPORTED_SHAPE, name << ": rank outside 1..4");
+            if (Status s = check_mx_pair(out(0), out(1), in(0).shape, n.attr_i(0), name, message)) return s;
+            return OK;
+        }
+        case Op::MX_RESTORE:
+            if (!need(2, 1) || n.attrs.size() != 2) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (n.attrs[0] != 4 && n.attrs[0] != 8) FAIL(UNSUPPORTED_OPERATION, name << ": formats of 4 or 8 bits");
+            if (!dtype_floating(out(0).dtype)) FAIL(UNSUPPORTED_OPERATION, name << ": needs a floating result");
+            if (out(0).shape.empty() || out(0).shape.back() != n.attr_i(1)) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape");
+            return check_mx_pair(in(0), in(1), out(0).shape, n.attr_i(0), name, message);
+        case Op::MX_LINEAR: {
+            if ((n.inputs.size() != 4 && n.inputs.size() != 5) || n.outputs.size() != 1 || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (!dtype_floating(out(0).dtype)) FAIL(UNSUPPORTED_OPERATION, name << ": needs a floating result");
+            if (!mx_activation(n.attrs[0], true)) FAIL(UNSUPPORTED_OPERATION, name << ": unknown activation");
+            if (out(0).shape.size() < 2 || in(2).shape.size() != 2) FAIL(UNSUPPORTED_SHAPE, name << ": rank");
+            const int64_t outer = out(0).shape.back();
+            if (outer < 1) FAIL(UNSUPPORTED_SHAPE, name << ": empty result rows");
+            if (in(0).shape.size() != out(0).shape.size() || in(0).shape.back() < 16 || in(0).shape.back() % 16) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape");
+            // the contraction length in whole blocks; x and W are zero past their last element
+            const int64_t k = in(0).shape.back() * 2;
+            shape = out(0).shape; shape.back() = k;
+            if (Status s = check_mx_pair(in(0), in(1), shape, 4, name, message)) return s;
+            if (Status s = check_mx_pair(in(2), in(3), {outer, k}, 4, name, message)) return s;
+            if (n.inputs.size() == 5 && (in(4).dtype != out(0).dtype || in(4).shape != std::vector<int64_t>{outer})) FAIL(GRAPH_COMPILATION_FAILED, name << ": bias");
+            int64_t rows = out(0).elements() / outer;
+            if (rows >= (1ll << 30) || outer >= (1ll << 30) || k >= (1ll << 30)) FAIL(UNSUPPORTED_SHAPE, name << ": extent of 2^30 or more");
+            return OK;
+        }
+        case Op::MX_WEIGHT_GRADIENT: {
+            if (!need(3, 1) || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (!dtype_floating(in(2).dtype) || out(0).dtype != DType::F32) FAIL(UNSUPPORTED_OPERATION, name << ": needs a floating gradient and a FLOAT32 result");
+            if (out(0).shape.size() != 2 || in(2).shape.size() < 2 || in(2).shape.size() > 4) FAIL(UNSUPPORTED_SHAPE, name << ": rank");
+            shape = in(2).shape; shape.back() = n.attr_i(0);
+            if (out(0).shape[0] != in(2).shape.back() || out(0).shape[1] != n.attr_i(0)) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape");
+            if (out(0).shape[0] < 1) FAIL(UNSUPPORTED_SHAPE, name << ": empty result");
+            if (Status s = check_mx_pair(in(0), in(1), shape, 8, name, message)) return s;
+            int64_t rows = in(2).elements() / out(0).shape[0];
+            if (rows >= (1ll << 30) || out(0).shape[0] >= (1ll << 30) || out(0).shape[1] >= (1ll << 30)) FAIL(UNSUPPORTED_SHAPE, name << ": extent of 2^30 or more");
+            return OK;
+        }
+        case Op::MX_ACTIVATION_GRADIENT:
+            if (!need(3, 1) || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (!dtype_floating(in(2).dtype) || out(0).dtype != in(2).dtype) FAIL(UNSUPPORTED_OPERATION, name << ": gradient and result of one floating type");
+            if (!mx_activation(n.attrs[0], false)) FAIL(UNSUPPORTED_OPERATION, name << ": unknown activation");
+            if (in(2).shape.empty() || out(0).shape != in(2).shape) FAIL(GRAPH_COMPILATION_FAILED, name << ": shape");
+            return check_mx_pair(in(0), in(1), in(2).shape, 8, name, message);
     }
     FAIL(UNSUPPORTED_OPERATION, "unknown operation wire code " << (uint32_t)n.op);
 }
@@ -289,7 +363,7 @@ Status parse_program(const uint8_t *bytes, uint32_t size, Program &g, std::strin
         uint64_t o = off_v + i * 40;
         Value &v = g.values[i];
         uint32_t dt = r.u32(o), rank = r.u32(o + 4), doff = r.u32(o + 8), soff = r.u32(o + 12);
-        if (dt < 1 || dt > 6) FAIL(UNSUPPORTED_OPERATION, "value " << i << ": data type code " << dt);
+        if (dt < 1 || dt > 7) FAIL(UNSUPPORTED_OPERATION, "value " << i << ": data type code " << dt);
         if (rank > 8) FAIL(UNSUPPORTED_SHAPE, "value " << i << ": rank above 8");
         if ((uint64_t)doff + rank > nd) FAIL(GRAPH_COMPILATION_FAILED, "value " << i << ": dimensions out of range");
         v.dtype = (DType)dt;
@@ -318,6 +392,7 @@ Status parse_program(const uint8_t *bytes, uint32_t size, Program &g, std::strin
         v.constant_bits = r.u64(o + 32);
         if (v.role == Role::CONSTANT && v.elements() != 1) FAIL(UNSUPPORTED_SHAPE, "value " << i << ": only splat scalar constants");
         if (v.role == Role::CONSTANT && dtype_low(v.dtype)) FAIL(UNSUPPORTED_OPERATION, "value " << i << ": 16-bit constants");
+        if (v.role == Role::CONSTANT && v.dtype == DType::U8) FAIL(UNSUPPORTED_OPERATION, "value " << i << ": U8 constants");
         if (v.role != Role::FEED && (soff != 0xffffffffu && v.role == Role::CONSTANT)) FAIL(GRAPH_COMPILATION_FAILED, "value " << i << ": constant with strides");
     }
     auto ref = [&](uint64_t index) { return r.u32(off_r + index * 4); };

@@ -42,7 +42,8 @@ enum Status : int32_t {
 // BF16 / F16 are storage types (DataType.BFLOAT16 / FLOAT16 of the reference): raw 16-bit patterns in memory,
 // a FLOAT32 working type inside every node, one narrowing (round to nearest even; BFLOAT16 NaN -> 0x7FC0,
 // BFloat16Bits.java:17-29) of each node's result (CpuScalarReferenceKernel.java:93-115).
-enum class DType : uint32_t { F32 = 1, I32 = 2, I64 = 3, BOOL = 4, BF16 = 5, F16 = 6 };
+// U8: the code and scale bytes of block-scaled tensors (below); only the MX operations and copies take them.
+enum class DType : uint32_t { F32 = 1, I32 = 2, I64 = 3, BOOL = 4, BF16 = 5, F16 = 6, U8 = 7 };
 inline int dtype_bytes(DType t) { return t == DType::F32 || t == DType::I32 ? 4 : t == DType::I64 ? 8 : (t == DType::BF16 || t == DType::F16) ? 2 : 1; }
 inline bool dtype_low(DType t) { return t == DType::BF16 || t == DType::F16; }
 inline bool dtype_floating(DType t) { return t == DType::F32 || dtype_low(t); }
@@ -56,8 +57,29 @@ enum class Op : uint32_t {
     SCALAR_MAX = 9, RELU = 10, EXP = 11, GT = 12, WHERE = 13, EXPAND = 14, EXPAND_DIMS = 15,
     CONTIGUOUS = 16, ONE_HOT = 17, MAX = 18, SUM = 19, SUM_TO_SHAPE = 20, SOFTMAX = 21,
     INDEX_CROSS_ENTROPY = 22, MEAN_SQUARED_ERROR = 23, ARG_MAX = 24, TANH = 25, SIGMOID = 26, SILU = 27, IS_INF = 28, GELU_TANH = 29, CLAMP = 30, LT = 31, EQ = 32,
-    SCALAR_SUB = 33, DENSE_CROSS_ENTROPY = 34, GELU = 35, ERF = 36
+    SCALAR_SUB = 33, DENSE_CROSS_ENTROPY = 34, GELU = 35, ERF = 36,
+    MX_QUANTIZE = 37, MX_RESTORE = 38, MX_LINEAR = 39, MX_WEIGHT_GRADIENT = 40, MX_ACTIVATION_GRADIENT = 41
 };
+
+// Block-scaled ("microscaled") tensors have no counterpart in the reference.  A tensor [.., K] is held as two
+// U8 tensors: per 32 consecutive elements of the last axis one scale byte (E8M0: the value 2^(byte - 127), 255 =
+// NaN), and per element a code of 4 bits (E2M1, two per byte, the even element in the low half) or 8 bits (E4M3).
+//   codes   [.., mx_code_bytes(format, K)]   K rounded up to whole blocks; elements past K are zero
+//   scales  [.., mx_scale_bytes(K)]          K / 32 rounded up to a multiple of four; bytes past the last block zero
+// MX_QUANTIZE chooses the least scale, from 2^-127 up, under which the block's largest magnitude does not exceed
+// the element type's (6 or 448): nothing saturates.  Elements round to nearest even.  A block that holds an
+// infinity or a NaN gets scale 255 and stands for NaN throughout.
+//   MX_QUANTIZE             x (FLOAT32 / BFLOAT16 / FLOAT16) -> codes, scales          attributes: format (4 or 8)
+//   MX_RESTORE              codes, scales -> values                                    attributes: format, K
+//   MX_LINEAR               codes, scales of x [.., M, K] and of W [N, K] (format 4), optional bias [N]
+//                           -> act(x W^T + bias)                                       attributes: activation (0 or its wire code)
+//   MX_WEIGHT_GRADIENT      codes, scales of x [.., R, K] (format 8), g [.., R, N] -> g^T x, [N, K] FLOAT32    attributes: K
+//   MX_ACTIVATION_GRADIENT  codes, scales of z [.., K] (format 8), g [.., K] -> g * act'(z)    attributes: activation
+// All compute in FLOAT32 and round once.
+constexpr int64_t MX_BLOCK = 32;
+constexpr int64_t mx_blocks(int64_t k) { return (k + MX_BLOCK - 1) / MX_BLOCK; }
+constexpr int64_t mx_code_bytes(int64_t format, int64_t k) { return mx_blocks(k) * MX_BLOCK * format / 8; }
+constexpr int64_t mx_scale_bytes(int64_t k) { return (mx_blocks(k) + 3) / 4 * 4; }
 const char *op_name(Op op);
 
 enum class Role : uint32_t { INTERMEDIATE = 0, FEED = 1, CONSTANT = 2 };

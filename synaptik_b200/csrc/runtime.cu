@@ -708,6 +708,28 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 if (dtype_low(plan.views[st.a].dtype)) LAUNCH(kern::argmax_rows_low(s, plan.views[st.a].dtype == DType::BF16 ? 1 : 2, ptr(st.a), (int64_t *)ptr(st.out), st.m, st.n));
                 else LAUNCH(kern::argmax_rows(s, (const float *)ptr(st.a), (int64_t *)ptr(st.out), st.m, st.n));
                 break;
+            case StepKind::MX_QUANTIZE: {
+                const View &a = plan.views[st.a];
+                LAUNCH(kern::mx_quantize(s, (int)st.scalar_bits, a.dtype, ptr(st.a), index4(a.shape, &a.strides, nullptr, nullptr, &a.shape),
+                                         (uint8_t *)ptr(st.out), (uint8_t *)ptr(st.out2)));
+                break;
+            }
+            case StepKind::MX_RESTORE:
+                LAUNCH(kern::mx_restore(s, (int)st.scalar_bits, plan.views[st.out].dtype, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
+                                        st.m, st.n, ptr(st.out)));
+                break;
+            case StepKind::MX_LINEAR:
+                LAUNCH(kern::mx_linear(s, plan.views[st.out].dtype, st.act, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
+                                       (const uint8_t *)ptr(st.b), (const uint8_t *)ptr(st.scale_b), ptr(st.bias), ptr(st.out), ctx->sm_count, ctx->error_dev));
+                break;
+            case StepKind::MX_WEIGHT_GRADIENT:
+                LAUNCH(kern::mx_weight_gradient(s, plan.views[st.b].dtype, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
+                                                ptr(st.b), (float *)ptr(st.out), ctx->sm_count, ctx->error_dev));
+                break;
+            case StepKind::MX_ACTIVATION_GRADIENT:
+                LAUNCH(kern::mx_activation_gradient(s, st.act, plan.views[st.b].dtype, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
+                                                    ptr(st.b), st.m, st.n, ptr(st.out)));
+                break;
             case StepKind::RELU_BACKWARD: {
                 int64_t total = 1; for (auto d : plan.views[st.out].shape) total *= d;
                 LAUNCH(kern::relu_backward(s, (const float *)ptr(st.a), (const float *)ptr(st.b), (float *)ptr(st.out), total));

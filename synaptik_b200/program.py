@@ -17,8 +17,8 @@ import struct
 from dataclasses import dataclass, field
 from typing import List, Sequence
 
-F32, I32, I64, BOOL, BF16, F16 = 1, 2, 3, 4, 5, 6
-DTYPE_BYTES = {F32: 4, I32: 4, I64: 8, BOOL: 1, BF16: 2, F16: 2}
+F32, I32, I64, BOOL, BF16, F16, U8 = 1, 2, 3, 4, 5, 6, 7
+DTYPE_BYTES = {F32: 4, I32: 4, I64: 8, BOOL: 1, BF16: 2, F16: 2, U8: 1}
 # BFLOAT16 / FLOAT16 are storage types (DataType.BFLOAT16 / FLOAT16): values travel as raw 16-bit patterns,
 # every node widens its operands to FLOAT32, computes there and narrows its result once.  They are accepted
 # by the views, MATMUL, ADD / SUB / MUL / DIV, the activations, CONTIGUOUS and ARG_MAX: the inference path.
@@ -65,7 +65,23 @@ OPS = {
     "CONTIGUOUS": 16, "ONE_HOT": 17, "MAX": 18, "SUM": 19, "SUM_TO_SHAPE": 20, "SOFTMAX": 21,
     "INDEX_CROSS_ENTROPY": 22, "MEAN_SQUARED_ERROR": 23, "ARG_MAX": 24, "TANH": 25, "SIGMOID": 26, "SILU": 27, "IS_INF": 28, "GELU_TANH": 29, "CLAMP": 30, "LT": 31, "EQ": 32,
     "SCALAR_SUB": 33, "DENSE_CROSS_ENTROPY": 34, "GELU": 35, "ERF": 36,
+    "MX_QUANTIZE": 37, "MX_RESTORE": 38, "MX_LINEAR": 39, "MX_WEIGHT_GRADIENT": 40, "MX_ACTIVATION_GRADIENT": 41,
 }
+
+# Block-scaled ("microscaled") storage: 32 consecutive elements of the last axis share one power-of-two scale
+# (a byte: 2^(byte - 127), 255 = NaN); an element is a code of 4 bits ("mx4", E2M1) or 8 bits ("mx8", E4M3).
+MX_BLOCK = 32
+MX_FORMATS = {"mx4": 4, "mx8": 8}
+
+
+def mx_code_bytes(fmt: str, features: int) -> int:
+    """Bytes of codes per row: whole blocks, elements past the last feature zero."""
+    return -(-features // MX_BLOCK) * MX_BLOCK * MX_FORMATS[fmt] // 8
+
+
+def mx_scale_bytes(features: int) -> int:
+    """Bytes of scales per row: one per block, padded with zeros to a multiple of four."""
+    return -(-features // (4 * MX_BLOCK)) * 4
 ROLE_INTERMEDIATE, ROLE_FEED, ROLE_CONSTANT = 0, 1, 2
 MASK64 = (1 << 64) - 1
 
@@ -98,6 +114,15 @@ class Value:
     @property
     def nbytes(self) -> int:
         return self.elements * DTYPE_BYTES[self.dtype]
+
+
+@dataclass
+class MxValue:
+    """A block-scaled tensor [.., features]: its two U8 values, to feed, publish or pass on together."""
+    format: str
+    shape: tuple
+    codes: Value
+    scales: Value
 
 
 @dataclass
@@ -299,6 +324,48 @@ class GraphBuilder:
         else:
             del shape[axis]
         return self._node("ARG_MAX", [x], I64, shape, [axis, int(keep_dimensions)])
+
+    # ---- block-scaled tensors (no counterpart in the reference) -----------------------------
+    def mx_feed(self, fmt: str, shape: Sequence[int]) -> MxValue:
+        """Two feeds, codes then scales, of a block-scaled tensor of the given shape."""
+        shape = tuple(int(d) for d in shape)
+        return MxValue(fmt, shape, self.feed(U8, shape[:-1] + (mx_code_bytes(fmt, shape[-1]),)), self.feed(U8, shape[:-1] + (mx_scale_bytes(shape[-1]),)))
+
+    def mx_quantize(self, x: Value, fmt: str) -> MxValue:
+        """MX_QUANTIZE: x in 4 or 8 bits per element.  Each block of 32 takes the least power-of-two scale under
+        which nothing saturates and rounds to nearest even; a block with an infinity or a NaN stands for NaN."""
+        codes = self._value(U8, tuple(x.shape[:-1]) + (mx_code_bytes(fmt, x.shape[-1]),))
+        scales = self._value(U8, tuple(x.shape[:-1]) + (mx_scale_bytes(x.shape[-1]),))
+        self.nodes.append(_Node(OPS["MX_QUANTIZE"], [x.index], [codes.index, scales.index], [MX_FORMATS[fmt]]))
+        return MxValue(fmt, tuple(x.shape), codes, scales)
+
+    def mx_restore(self, x: MxValue, dtype: int = F32) -> Value:
+        """MX_RESTORE: the values a block-scaled tensor stands for."""
+        return self._node("MX_RESTORE", [x.codes, x.scales], dtype, x.shape, [MX_FORMATS[x.format], x.shape[-1]])
+
+    def mx_linear(self, x: MxValue, weight: MxValue, bias: Value | None = None, activation: str | None = None, dtype: int = F32) -> Value:
+        """MX_LINEAR: act(x . W^T + b) of 4-bit operands x [.., in] and W [out, in]; sums and activation in
+        FLOAT32, one rounding to `dtype`, which is also the bias's type."""
+        if x.format != "mx4" or weight.format != "mx4":
+            raise ValueError("MX_LINEAR multiplies 4-bit operands")
+        if len(weight.shape) != 2 or x.shape[-1] != weight.shape[-1]:
+            raise ValueError("MX_LINEAR contraction extents differ")
+        inputs = [x.codes, x.scales, weight.codes, weight.scales] + ([bias] if bias is not None else [])
+        return self._node("MX_LINEAR", inputs, dtype, x.shape[:-1] + (weight.shape[0],), [OPS[activation.upper()] if activation else 0])
+
+    def mx_weight_gradient(self, checkpoint: MxValue, upstream: Value) -> Value:
+        """MX_WEIGHT_GRADIENT: dW = upstream^T . x [out, in] from the 8-bit checkpoint of x [.., in] and the
+        gradient [.., out] of x . W^T; FLOAT32 sums."""
+        if checkpoint.format != "mx8" or checkpoint.shape[:-1] != tuple(upstream.shape[:-1]):
+            raise ValueError("MX_WEIGHT_GRADIENT needs an 8-bit checkpoint of the upstream gradient's leading dimensions")
+        return self._node("MX_WEIGHT_GRADIENT", [checkpoint.codes, checkpoint.scales, upstream], F32, (upstream.shape[-1], checkpoint.shape[-1]), [checkpoint.shape[-1]])
+
+    def mx_activation_gradient(self, kind: str, checkpoint: MxValue, upstream: Value) -> Value:
+        """MX_ACTIVATION_GRADIENT: upstream * act'(z) from the 8-bit checkpoint of the pre-activation z (for "relu"
+        the activation's own checkpoint serves as well: it is positive exactly where the held z is)."""
+        if checkpoint.format != "mx8" or checkpoint.shape != tuple(upstream.shape):
+            raise ValueError("MX_ACTIVATION_GRADIENT needs an 8-bit checkpoint of the upstream gradient's shape")
+        return self._node("MX_ACTIVATION_GRADIENT", [checkpoint.codes, checkpoint.scales, upstream], upstream.dtype, upstream.shape, [OPS[kind.upper()]])
 
     # ---- composite expressions, as the reference builds them -----------------------------
     def linear(self, x: Value, weight: Value, bias: Value | None):
