@@ -188,11 +188,19 @@ def context():
     return _context
 
 
-class Shared:
-    """Memory of a framework buffer as a torch tensor."""
+class Memory:
+    """A framework buffer as memory that torch can see.  Every tensor over it keeps it alive; the last one frees it."""
 
-    def __init__(self, buffer):
-        self.__cuda_array_interface__ = {"data": (buffer.device_pointer(), False), "shape": (buffer.nbytes,), "typestr": "|u1", "version": 3}
+    def __init__(self, nbytes):
+        self.buffer = context().buffer(nbytes)
+        self.__cuda_array_interface__ = {"data": (self.buffer.device_pointer(), False), "shape": (nbytes,), "typestr": "|u1", "version": 3}
+
+    def tensor(self, shape, dtype):
+        return torch.as_tensor(self, device="cuda").view(dtype).view(shape)
+
+    def __del__(self):
+        if hasattr(self, "buffer"):
+            self.buffer.close()
 
 
 class Plan:
@@ -200,33 +208,21 @@ class Plan:
 
     def __init__(self, builder, inputs, outputs):
         from synaptik_b200 import native
-        self.buffers, self.inputs, self.outputs = [], [], []
-        for tensor in inputs:
-            buffer, view = self.buffer(tensor.shape, tensor.dtype)
-            view.copy_(tensor)
-            self.inputs.append(buffer)
-        self.results = []
-        for shape, dtype in outputs:
-            buffer, view = self.buffer(shape, dtype)
-            self.outputs.append(buffer)
-            self.results.append(view)
+        fed = [Memory(tensor.nbytes) for tensor in inputs]
+        for memory, tensor in zip(fed, inputs):
+            memory.tensor(tensor.shape, tensor.dtype).copy_(tensor)
+        made = [Memory(math.prod(shape) * dtype.itemsize) for shape, dtype in outputs]
+        self.results = [memory.tensor(*out) for memory, out in zip(made, outputs)]
+        self.fed, self.inputs, self.outputs = fed, [m.buffer for m in fed], [m.buffer for m in made]
         self.executable = native.Executable(context(), builder.build())
-
-    def buffer(self, shape, dtype):
-        buffer = context().buffer(math.prod(shape) * dtype.itemsize)
-        self.buffers.append(buffer)
-        return buffer, torch.as_tensor(Shared(buffer), device="cuda").view(dtype).view(shape)
 
     def __call__(self):
         self.executable.enqueue(self.inputs, self.outputs)
         return self.results
 
     def __del__(self):
-        self.results = None
         if hasattr(self, "executable"):
             self.executable.close()
-        for buffer in self.buffers:
-            buffer.close()
 
 
 def prepare(case, seed):
