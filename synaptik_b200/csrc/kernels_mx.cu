@@ -298,36 +298,256 @@ int mx_grid(const MxRows &r) {
     return (int)(blocks < 148 * 8 ? (blocks < 1 ? 1 : blocks) : 148 * 8);
 }
 
-// ------------------------------------------------------------------------------------------------
-// 4-bit product, one warp per result: lanes take the blocks of the contraction in turn.  Twice an E2M1 value is an
-// integer, so a block's sum of products is exact in an integer.
-// ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ int mx_twice4(uint32_t code) {
-    const int magnitude = (int)(0xC8643210u >> (4 * (code & 7u)) & 15u);
-    return code & 8u ? -magnitude : magnitude;
+// Activations of a FLOAT32 sum before its one rounding, from exp(-|z|) like the slopes above; below -120 SILU and
+// both GELUs are below the smallest number (-0, also for -infinity).
+__device__ __forceinline__ float mx_activate(int act, float z) {
+    switch ((Op)act) {
+        case Op::RELU: return relu_value(z);
+        case Op::TANH: return tanhf(z);
+        case Op::SIGMOID: { const float e = expf(-fabsf(z)), near = __fdividef(1.0f, 1.0f + e); return z >= 0.0f ? near : e * near; }
+        case Op::SILU: case Op::GELU_TANH: {
+            if (z < -120.0f) return -0.0f;
+            if (z > 120.0f) return z;
+            const float u = act == (int)Op::SILU ? z : 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f);
+            const float e = expf(-fabsf(u)), near = __fdividef(1.0f, 1.0f + e);
+            return z * (u >= 0.0f ? near : e * near);
+        }
+        case Op::GELU: return z < -120.0f ? -0.0f : 0.5f * z * erfcf(-0.7071067811865476f * z);
+        default: return z;
+    }
+}
+__device__ __noinline__ float4 mx_activate4(int act, float4 z) {
+    return make_float4(mx_activate(act, z.x), mx_activate(act, z.y), mx_activate(act, z.z), mx_activate(act, z.w));
 }
 
-// Activations of a FLOAT32 sum before its one rounding.
-__device__ __forceinline__ float mx_activate(int act, float z) { return activation_value(act, z); }
+// ------------------------------------------------------------------------------------------------
+// 4-bit products on the tensor cores: tcgen05.mma kind::mxf4 multiplies E2M1 codes under one E8M0 scale per 32
+// contraction steps, exactly, and adds in FP32 in tensor memory.  Codes go from the tensors to shared memory by TMA
+// (a k-block is 256 elements = one 128-byte swizzle row); their scales have to lie in tensor memory in the
+// order [lane = row mod 32][column = row / 32], four contraction blocks per 32-bit word.  Two warps fetch the words
+// with 4-byte asynchronous copies into that order (512-byte atoms of 128 rows x 4 blocks), zero past the matrix, and
+// the issuing thread sends them on with tcgen05.cp in front of the MMAs that use them.
+// ------------------------------------------------------------------------------------------------
+constexpr int MX_BK = 256;                      // contraction steps per k-block
+constexpr int MX_ATOM = 512;                    // scales of 128 rows x 128 contraction steps
 
-template <int KIND>
-__global__ void __launch_bounds__(MX_THREADS) mx_linear_simple_kernel(int act, int64_t m, int64_t n, int64_t k, const uint8_t *__restrict__ x, const uint8_t *__restrict__ xs,
-                                                                      const uint8_t *__restrict__ w, const uint8_t *__restrict__ ws,
-                                                                      const typename MxElement<KIND>::type *__restrict__ bias, typename MxElement<KIND>::type *__restrict__ out) {
-    const int lane = threadIdx.x & 31;
-    const int64_t blocks = k / MX_BLOCK, scale_pitch = (blocks + 3) / 4 * 4;
-    for (int64_t i = blockIdx.x * (int64_t)MX_WARPS + (threadIdx.x >> 5); i < m * n; i += (int64_t)gridDim.x * MX_WARPS) {
-        const int64_t row = i / n, col = i - row * n;
-        float sum = 0.0f;
-        for (int64_t b = lane; b < blocks; b += 32) {
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(x + row * (k / 2) + b * 16), *q = reinterpret_cast<const uint32_t *>(w + col * (k / 2) + b * 16);
-            int dot = 0;
-            for (int j = 0; j < 4; j++)
-                for (int e = 0; e < 32; e += 4) dot += mx_twice4(p[j] >> e) * mx_twice4(q[j] >> e);
-            sum += (float)dot * 0.25f * mx_scale_value(xs[row * scale_pitch + b]) * mx_scale_value(ws[col * scale_pitch + b]);
+// Instruction descriptor of kind::mxf4: E2M1 x E2M1 (format 1), UE8M0 scales (bit 23), K-major, M rows, N columns;
+// sf: which two of the four scale bytes per word the 64 contraction steps use (0 or 2).
+__device__ __forceinline__ uint32_t mx_idesc(int rows, int cols, int sf) {
+    return ((uint32_t)sf << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) | ((uint32_t)(rows >> 4) << 24) | ((uint32_t)sf << 29);
+}
+__device__ __forceinline__ uint64_t mx_operand_desc(uint32_t smem_addr) {       // K-major, 128-byte swizzle
+    return (1ull << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61) | (uint64_t)((smem_addr & 0x3ffffu) >> 4);
+}
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr) {         // 32 rows of 16 bytes, 8-row groups 128 bytes apart
+    return ((uint64_t)(128u >> 4) << 32) | (1ull << 46) | (uint64_t)((smem_addr & 0x3ffffu) >> 4);
+}
+template <int PAIR> __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
+}
+template <int PAIR> __device__ __forceinline__ void mx_copy_atom(uint32_t taddr, uint32_t smem_addr) {
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
+}
+// Four bytes global -> shared, the part past `bytes` (0 to 4) zero.
+__device__ __forceinline__ void mx_copy_word(uint32_t dst, const uint8_t *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// The scale words of `count` rows from row0 for the k-block that starts at contraction block b0, `threads` threads in
+// turn.  dst: atoms [contraction half][row / 128].
+__device__ __forceinline__ void mx_copy_scales(uint32_t dst, int atoms, const uint8_t *scales, int64_t pitch, int rows, int blocks, int row0, int count, int b0, int thread, int threads) {
+    for (int i = thread; i < 2 * count; i += threads) {
+        const int half = i & 1, r = i >> 1, b = b0 + half * 4;
+        const int left = blocks - b;
+        const int bytes = row0 + r < rows ? (left >= 4 ? 4 : left > 0 ? left : 0) : 0;
+        const uint8_t *src = bytes ? scales + (int64_t)(row0 + r) * pitch + b : scales;
+        mx_copy_word(dst + (uint32_t)((half * atoms + (r >> 7)) * MX_ATOM + (r & 31) * 16 + ((r >> 5) & 3) * 4), src, bytes);
+    }
+}
+
+// Waits, for at most a tenth of a second and whatever the abort flag says, for copies whose barrier nothing else arrives on.
+__device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
+    const uint64_t start = global_timer();
+    while (!mbar_try_wait(bar, parity) && global_timer() - start < 100000000ull) { }
+}
+
+struct MxLinear {
+    int m, n, blocks, k_blocks;         // blocks: contraction blocks of 32; k_blocks: of 256
+    int64_t scale_pitch;
+    const uint8_t *xs, *ws;
+    const void *bias; void *out;
+    int act;
+    int tiles_m, tiles_n, group_n;
+    int staged;                         // rows of `out` can be written by TMA
+    int *error_word;
+};
+
+// ---- few rows: weights on the M side ----------------------------------------------------------------
+// One block multiplies 128 rows of W by BN rows of x over a slice of the contraction; the up to eight blocks of a
+// cluster share a tile and add their partial sums, in ascending order, through each other's shared memory.  With
+// W as the M operand a tile wastes no MMA rows on absent rows of x, and the result leaves with 32 consecutive
+// columns per warp without a transposition.
+template <int BN> struct MxFewConfig {
+    static constexpr int kStages = BN <= 64 ? 6 : 5;
+    static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
+    static constexpr int kScaleBytes = 4 * MX_ATOM;             // two halves of W's atom, two of x's
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kScaleCols = 16;                       // tensor-memory columns of one stage's scales
+    static constexpr int kTmemCols = BN + kStages * kScaleCols <= 128 ? 128 : 256;
+    static constexpr int kSmemBytes = kStages * (kStageBytes + kScaleBytes) + 1024 + 256;
+    static_assert(BN * 128 * 4 <= kStages * kStageBytes, "partial sums reuse the operand stages");
+};
+
+template <int BN, int KIND>
+__global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxLinear prm, int slices) {
+    using Cfg = MxFewConfig<BN>;
+    using T = typename MxElement<KIND>::type;
+    constexpr int S = Cfg::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * (Cfg::kStageBytes + Cfg::kScaleBytes));
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem), scale_base = smem_base + S * Cfg::kStageBytes;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
+    auto scale_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };
+    const uint32_t done_bar = bar_base + 8u * (3 * S);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), 2); }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    // a cluster of `slices` blocks per tile; neighbouring clusters share the rows of x
+    const int slice = (int)(blockIdx.x % slices), tile = (int)(blockIdx.x / slices);
+    const int n0 = tile % prm.tiles_n * 128, m0 = tile / prm.tiles_n * BN;
+    const int kb0 = (int)((int64_t)prm.k_blocks * slice / slices), kb1 = (int)((int64_t)prm.k_blocks * (slice + 1) / slices);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0; uint32_t phase = 0;
+            int armed = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
+                mbar_expect_tx(full_bar(stage), Cfg::kStageBytes);
+                tma_load_2d(sa, &map_w, full_bar(stage), kb * (MX_BK / 2), n0);
+                tma_load_2d(sa + Cfg::kABytes, &map_x, full_bar(stage), kb * (MX_BK / 2), m0);
+                armed++;
+                if (++stage == S) { stage = 0; phase ^= 1u; }
+            }
+            // giving up: the copies in flight land before the block leaves
+            if (!ok || *abort_flag) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
         }
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) out[i] = mx_narrow<KIND>(mx_activate(act, sum + (bias ? mx_load<KIND>(bias + col) : 0.0f)));
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0; uint32_t phase = 0;
+            const uint32_t id0 = mx_idesc(128, BN, 0), id2 = mx_idesc(128, BN, 2);
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!mbar_wait(full_bar(stage), phase, abort_flag) || !mbar_wait(scale_bar(stage), phase, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes, ps = scale_base + stage * Cfg::kScaleBytes;
+                const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx_copy_atom<0>(ts + i * 4, ps + i * MX_ATOM);
+#pragma unroll
+                for (int k4 = 0; k4 < 4; k4++)
+                    mx_mma<0>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 4,
+                              (kb != kb0 || k4 != 0) ? 1u : 0u);
+                umma_commit(empty_bar(stage));
+                if (++stage == S) { stage = 0; phase ^= 1u; }
+            }
+            if (ok) umma_commit(done_bar);
+        }
+    } else if (warp < 4) {
+        // scales: copies of up to three stages in flight per thread
+        const int thread = threadIdx.x - 64;
+        int stage = 0; uint32_t phase = 0;
+        bool ok = true;
+        auto arrive = [&](int kb) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(scale_bar((kb - kb0) % S));
+        };
+        for (int kb = kb0; kb < kb1; kb++) {
+            ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag));
+            if (!ok) break;
+            const uint32_t ps = scale_base + stage * Cfg::kScaleBytes;
+            mx_copy_scales(ps, 1, prm.ws, prm.scale_pitch, prm.n, prm.blocks, n0, 128, kb * 8, thread, 64);
+            mx_copy_scales(ps + 2 * MX_ATOM, 1, prm.xs, prm.scale_pitch, prm.m, prm.blocks, m0, BN < 128 ? BN : 128, kb * 8, thread, 64);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (kb - kb0 >= 2) { asm volatile("cp.async.wait_group 2;" ::: "memory"); arrive(kb - 2); }
+            if (++stage == S) { stage = 0; phase ^= 1u; }
+        }
+        if (ok && kb1 - kb0 >= 2) { asm volatile("cp.async.wait_group 1;" ::: "memory"); arrive(kb1 - 2); }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (ok && kb1 > kb0) arrive(kb1 - 1);
+    }
+    __syncwarp();
+    bool ok = true;
+    float *partial = reinterpret_cast<float *>(smem);       // [BN][128]
+    if (warp >= 4) {
+        ok = kb1 == kb0 || mbar_wait(done_bar, 0u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        const int row = (warp & 3) * 32 + lane;             // of W's tile
+#pragma unroll
+        for (int c = 0; c < BN / 16; c++) {
+            float t[16];
+            if (ok && kb1 > kb0) tmem_load16(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(c * 16), t);
+            else for (int i = 0; i < 16; i++) t[i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) partial[(c * 16 + i) * 128 + row] = t[i];
+        }
+    }
+    tc_fence_before();
+    if (slices > 1) cluster_sync_all(); else __syncthreads();
+    // every block finishes its share of the tile's rows of x; two rows at a time, 128 threads each
+    const int per = (BN + slices - 1) / slices;
+    const int col = n0 + (int)(threadIdx.x & 127);
+    const int first = slice * per, last = first + per < BN ? first + per : BN;
+    const uint32_t mine = smem_u32(partial) + (threadIdx.x & 127) * 4;
+    const float b = prm.bias && col < prm.n ? mx_load<KIND>((const T *)prm.bias + col) : 0.0f;
+    for (int r = first + (int)(threadIdx.x >> 7); r < last; r += 2) {
+        if (m0 + r >= prm.m) break;
+        float sum;
+        if (slices == 1) sum = partial[r * 128 + (threadIdx.x & 127)];
+        else {
+            sum = 0.0f;
+            for (int q = 0; q < slices; q++) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(mine + (uint32_t)r * 512u, (uint32_t)q)) : "memory");
+                sum = q ? __fadd_rn(sum, v) : v;
+            }
+        }
+        if (col < prm.n) ((T *)prm.out)[(int64_t)(m0 + r) * prm.n + col] = mx_narrow<KIND>(mx_activate(prm.act, prm.bias ? __fadd_rn(sum, b) : sum));
+    }
+    if (slices > 1) cluster_sync_all(); else __syncthreads();      // no block leaves while another reads its sums
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(prm.error_word, ERR_WAIT_TIMEOUT);
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::kTmemCols) : "memory");
     }
 }
 
@@ -429,19 +649,62 @@ cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const u
 #undef CALL
 }
 
+// Tensor map over the codes of a 4-bit operand [rows, k]: boxes of 256 elements x box_rows, 128-byte swizzle.
+static bool make_code_map(CUtensorMap *map, const uint8_t *codes, int64_t rows, int64_t k, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
+    cuuint32_t box[2] = {MX_BK / 2, (cuuint32_t)box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, int KIND>
+static cudaError_t launch_mx_few(cudaStream_t s, const uint8_t *x, const uint8_t *w, const MxLinear &prm, int slices) {
+    using Cfg = MxFewConfig<BN>;
+    CUtensorMap map_w, map_x;
+    const int64_t k = (int64_t)prm.blocks * MX_BLOCK;
+    if (!make_code_map(&map_w, w, prm.n, k, 128) || !make_code_map(&map_x, x, prm.m, k, BN)) return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(mx_linear_few_kernel<BN, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((int64_t)slices * prm.tiles_n * prm.tiles_m));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)slices, 1, 1};
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mx_linear_few_kernel<BN, KIND>, map_w, map_x, prm, slices);
+}
+
 template <int KIND>
-static cudaError_t launch_mx_linear(cudaStream_t s, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
-                                    const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out) {
-    using T = typename MxElement<KIND>::type;
-    const int64_t blocks = (m * n + MX_WARPS - 1) / MX_WARPS;
-    mx_linear_simple_kernel<KIND><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(act, m, n, k, x, x_scales, w, w_scales, (const T *)bias, (T *)out);
-    return cudaGetLastError();
+static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint8_t *w, MxLinear prm, int sm_count) {
+    const int bn = prm.m <= 16 ? 16 : prm.m <= 32 ? 32 : prm.m <= 64 ? 64 : 128;
+    prm.tiles_n = (prm.n + 127) / 128; prm.tiles_m = (prm.m + bn - 1) / bn;
+    const int64_t tiles = (int64_t)prm.tiles_n * prm.tiles_m;
+    if (tiles >= (1ll << 28)) return cudaErrorInvalidValue;
+    int slices = 1;
+    while (slices < 8 && tiles * slices * 2 <= sm_count && prm.k_blocks >= slices * 2) slices *= 2;
+    switch (bn) {
+        case 16: return launch_mx_few<16, KIND>(s, x, w, prm, slices);
+        case 32: return launch_mx_few<32, KIND>(s, x, w, prm, slices);
+        case 64: return launch_mx_few<64, KIND>(s, x, w, prm, slices);
+        default: return launch_mx_few<128, KIND>(s, x, w, prm, slices);
+    }
 }
 
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
                       const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out, int sm_count, int *error_word) {
     if (m == 0 || n == 0) return cudaSuccess;
-#define CALL(KIND) launch_mx_linear<KIND>(s, act, m, n, k, x, x_scales, w, w_scales, bias, out)
+    MxLinear prm = {};
+    prm.m = (int)m; prm.n = (int)n; prm.blocks = (int)(k / MX_BLOCK); prm.k_blocks = (int)((k + MX_BK - 1) / MX_BK);
+    prm.scale_pitch = mx_scale_bytes(k); prm.xs = x_scales; prm.ws = w_scales;
+    prm.bias = bias; prm.out = out; prm.act = act; prm.error_word = error_word;
+#define CALL(KIND) launch_mx_linear<KIND>(s, x, w, prm, sm_count)
     return MX_KINDS(dtype, CALL);
 #undef CALL
 }
