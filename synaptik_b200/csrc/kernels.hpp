@@ -206,15 +206,21 @@ cudaError_t argmax_rows_low(cudaStream_t s, int kind, const void *x, int64_t *ou
 // ---- block-scaled ("microscaled") tensors (kernels_mx.cu; the storage form is described in program.hpp) ----
 // Codes and scales start on multiples of 16 bytes; rows of codes are whole 16-byte groups, rows of scales whole
 // words.  `format` 4 or 8 bits.
-// ix: the iteration space of x, last axis in shape[3], strides in sa; codes and scales dense.
-cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales);
+// ix: the iteration space of x, last axis in shape[3], strides in sa; codes and scales dense.  tiles (optional):
+// the scales once more in the order the two-SM product reads, mx_tile_bytes(rows, k) bytes that were zero at first.
+cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles = nullptr);
 cudaError_t mx_restore(cudaStream_t s, int format, DType dtype, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *out);
 // out = g * act'(z), z held in 8 bits; g and out dense [rows, cols] of one type.
 cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const uint8_t *codes, const uint8_t *scales, const void *g,
                                    int64_t rows, int64_t cols, void *out);
-// out[m, n] = act(x[m, k] . w[n, k]^T + bias[n]), both operands in 4 bits, k a multiple of 32.
+// out[m, n] = act(x[m, k] . w[n, k]^T + bias[n]), both operands in 4 bits, k a multiple of 32.  Where mx_linear_tiled
+// says so the product runs on two-SM tiles and needs the scales of both operands in tiles (else x_tiles = w_tiles = null).
+bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count);
+int64_t mx_tile_bytes(int64_t rows, int64_t k);
+cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles);
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
-                      const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out, int sm_count, int *error_word);
+                      const uint8_t *w, const uint8_t *w_scales, const uint8_t *x_tiles, const uint8_t *w_tiles, const void *bias, void *out,
+                      int sm_count, int *error_word);
 // out[n, k] = sum over rows of g[row, n] * x[row, k], x held in 8 bits, out FLOAT32.
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
                                const void *g, float *out, int sm_count, int *error_word);

@@ -218,21 +218,6 @@ struct SliceParams {                         // two-SM kernel: split of the cont
     int *unit_counter;                       // dynamic assignment: the next unit number, zero before the launch
 };
 
-// Tile order of the two-SM kernel.  The 74 pairs work on 74 consecutive tiles at a time.  In plain
-// row-major order those cover every tile column and few row bands, so all of Q (134 MB of planes for a
-// 4096 x 4096 weight) cycles through L2 once per few row bands and is read from DRAM again and again
-// (measured: 16.7 GB per 65536 x 4096 x 4096 product whose operands are 2.3 GB).  Grouped order: the
-// tile columns are cut into groups of group_n, and each group is swept down all row bands before the
-// next group starts, so the tiles in flight share fewer distinct Q columns and more P row bands.
-__device__ __forceinline__ void tile_origin(int tile, int tiles_m, int tiles_n, int group_n, int &mi, int &ni) {
-    const int per_group = tiles_m * group_n;
-    const int g = tile / per_group, within = tile - g * per_group;
-    const int first = g * group_n;
-    const int width = tiles_n - first < group_n ? tiles_n - first : group_n;     // the last group may be narrower
-    mi = within / width;
-    ni = first + (within - mi * width);
-}
-
 
 // The activations other than ReLU evaluate an elementary function in binary64 (activation.cuh).  Kept out
 // of line and out of the kernels that never need them: inlined into the 32 call sites of an epilogue
@@ -1247,12 +1232,6 @@ __device__ __forceinline__ void low_emit4(const LowParams &prm, int row, int col
 // conversions into 128-byte-swizzled boxes of 32 rows x 64 columns in shared memory and one lane hands each
 // box to a TMA store, which also clips rows and columns past the matrix.  Same arithmetic, node by node, as
 // low_emit4: narrow the sum; add the bias in FLOAT32 and narrow; activation and narrow.
-template <int KIND> __device__ __forceinline__ uint32_t low_pack2(float lo, float hi) {
-    uint32_t r;
-    if constexpr (KIND == 1) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 template <int KIND> __device__ __forceinline__ void low_unpack2(uint32_t r, float &lo, float &hi) {
     if constexpr (KIND == 1) { lo = __uint_as_float(r << 16); hi = __uint_as_float(r & 0xffff0000u); }
     else { lo = __half2float(__ushort_as_half((uint16_t)(r & 0xffffu))); hi = __half2float(__ushort_as_half((uint16_t)(r >> 16))); }
@@ -1263,12 +1242,6 @@ template <int KIND> __device__ __forceinline__ uint32_t low_relu2(uint32_t r) {
     if constexpr (KIND == 1) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(r), "r"(0u));
     else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(r), "r"(0u));
     return d;
-}
-// The packed instructions give every NaN as 0x7FFF; the storage types' NaN is 0x7FC0 / 0x7E00 (low_encode).
-template <int KIND> __device__ __forceinline__ uint32_t low_canonical_nan2(uint32_t r) {
-    constexpr uint32_t inf2 = KIND == 1 ? 0x7F807F80u : 0x7C007C00u, nan2 = KIND == 1 ? 0x7FC07FC0u : 0x7E007E00u;
-    const uint32_t mask = __vcmpgtu2(r & 0x7FFF7FFFu, inf2);
-    return mask ? ((r & ~mask) | (nan2 & mask)) : r;
 }
 
 // The bias of a warp's columns lives in its lanes' registers, four columns per lane (lane l: columns

@@ -5,6 +5,8 @@
 #include "lowp.cuh"
 #include "tensor_core.cuh"
 
+#include <cstdlib>
+
 namespace syn {
 namespace kern {
 
@@ -149,10 +151,33 @@ __device__ __forceinline__ void mx_decode8x2(uint32_t bytes, float &a, float &b)
     low_unpack_half2(h, a, b);
 }
 
+// Scales of a 4-bit operand in the order tensor memory takes them: atoms of 512 bytes hold 128 rows x 4 blocks, row r
+// of an atom at 16 (r mod 32) + 4 (r / 32); atoms of one band of rows in a row, an even number of them (a k-block of
+// the product takes two).
+constexpr int MX_ATOM = 512;
+__host__ __device__ constexpr int64_t mx_tile_atoms(int64_t k) { return (k + 255) / 256 * 2; }
+__device__ __forceinline__ int64_t mx_tile_offset(int64_t row, int64_t block, int64_t atoms) {
+    return ((row >> 7) * atoms + (block >> 2)) * MX_ATOM + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+// The same from scales that exist already: a thread moves one word of four rows.  Bytes past the last block are not
+// taken over: against codes of zero a scale of NaN would still make NaN.
+__global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_t *__restrict__ scales, int64_t rows, int64_t blocks, uint8_t *__restrict__ tiles) {
+    const int64_t words = (blocks + 3) / 4, atoms = mx_tile_atoms(blocks * MX_BLOCK), total = (rows + 127) / 128 * 32 * words;
+    for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * MX_THREADS) {
+        const int64_t line = i / words, word = i - line * words, band = line >> 5, r = band * 128 + (line & 31);
+        const int left = blocks - word * 4 < 4 ? (int)(blocks - word * 4) : 4;
+        const uint32_t keep = left == 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+        uint32_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) v[q] = r + 32 * q < rows ? *reinterpret_cast<const uint32_t *>(scales + (r + 32 * q) * words * 4 + word * 4) & keep : 0u;
+        *reinterpret_cast<uint4 *>(tiles + (band * atoms + word) * MX_ATOM + (line & 31) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
 // x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.
 template <int FORMAT, int KIND, bool VEC>
 __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows r, int64_t row_step, int even,
-                                                                 uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+                                                                 uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles) {
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
     const int lane = threadIdx.x & 31;
     const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK * FORMAT / 8, scale_pitch = r.per_row / 4;
@@ -183,7 +208,10 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
         const int64_t group = at.first >> 3;
         const bool exists = (at.first & ~(int64_t)(MX_BLOCK - 1)) < r.cols;     // else: padding of the scales
         const uint32_t byte = exists ? mx_scale_byte<FORMAT>(largest) : 0u;
-        if ((lane & 3) == 0) scales[at.row * scale_pitch + (group >> 2)] = (uint8_t)byte;
+        if ((lane & 3) == 0) {
+            scales[at.row * scale_pitch + (group >> 2)] = (uint8_t)byte;
+            if (tiles) tiles[mx_tile_offset(at.row, group >> 2, mx_tile_atoms(r.cols))] = (uint8_t)byte;
+        }
         if (!exists) continue;
         // the inverse scale 2^(127 - byte) is a normal number for every byte that occurs; a product with it is
         // exact, or below half the smallest element
@@ -324,12 +352,10 @@ __device__ __noinline__ float4 mx_activate4(int act, float4 z) {
 // 4-bit products on the tensor cores: tcgen05.mma kind::mxf4 multiplies E2M1 codes under one E8M0 scale per 32
 // contraction steps, exactly, and adds in FP32 in tensor memory.  Codes go from the tensors to shared memory by TMA
 // (a k-block is 256 elements = one 128-byte swizzle row); their scales have to lie in tensor memory in the
-// order [lane = row mod 32][column = row / 32], four contraction blocks per 32-bit word.  Two warps fetch the words
-// with 4-byte asynchronous copies into that order (512-byte atoms of 128 rows x 4 blocks), zero past the matrix, and
-// the issuing thread sends them on with tcgen05.cp in front of the MMAs that use them.
+// order [lane = row mod 32][column = row / 32], four contraction blocks per 32-bit word: the issuing thread sends
+// them there with tcgen05.cp in front of the MMAs that use them.
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_BK = 256;                      // contraction steps per k-block
-constexpr int MX_ATOM = 512;                    // scales of 128 rows x 128 contraction steps
 
 // Instruction descriptor of kind::mxf4: E2M1 x E2M1 (format 1), UE8M0 scales (bit 23), K-major, M rows, N columns;
 // sf: which two of the four scale bytes per word the 64 contraction steps use (0 or 2).
@@ -551,6 +577,250 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
     }
 }
 
+// ---- many rows: two-SM tiles of 256 x 256 -----------------------------------------------------------
+// A cluster of two blocks per tile (cta_group::2, M = 256): each loads its 128 rows of x, half of the tile's 256
+// rows of W, and the scales of its rows of x and of all of W's (tensor memory of both blocks needs those), in tiles
+// that TMA can fetch: gathering them word by word from rows took three quarters of the time.  A
+// one-SM block would move (128 + 256) x 128 bytes of codes into shared memory and the tensor core read them out again
+// within 512 clocks of MMA, more than shared memory delivers; the pair moves a third less.  Accumulators take 256
+// columns of tensor memory and the scales of the stages in flight most of the rest, so there is one accumulator: the
+// epilogue warps first copy it to registers, hand it back, and finish the tile under the next one's main loop.
+struct MxPairConfig {
+    static constexpr int BN = 256;
+    static constexpr int kStages = 5;
+    static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kScaleBytes = 6 * MX_ATOM;             // two atoms of x's rows, two of each half of W's
+    static constexpr int kScaleCols = 24;
+    static constexpr int kTmemCols = 512;
+    static constexpr int kStagingBytes = 8 * 4096;
+    static constexpr int kSmemBytes = kStages * (kStageBytes + kScaleBytes) + kStagingBytes + 1024 + 256;
+};
+constexpr int MX_PAIR_THREADS = 384;    // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue
+
+// One warp's 32 rows x 128 columns: bias, activation, one rounding, then boxes of 32 rows x 128 bytes through
+// shared memory (16-byte chunk j of row r at chunk j ^ (r & 7), the 128-byte swizzle) and out by TMA, which clips the
+// edges; rows of `out` that TMA cannot address are copied from the box 32 columns at a time.
+template <int KIND, bool GENERAL>
+__device__ __forceinline__ void mx_emit(const MxLinear &prm, const CUtensorMap *map_out, uint32_t stage, int row0, int col0, float (&sum)[128], float4 bias_lane, int lane) {
+    using T = typename MxElement<KIND>::type;
+    constexpr int WIDTH = KIND == 0 ? 32 : 64;          // columns per box
+    constexpr int PER = WIDTH / 8;                      // columns per 16-byte chunk
+#pragma unroll
+    for (int b = 0; b < 128 / WIDTH; b++) {
+        const int c0 = col0 + b * WIDTH;
+        if (c0 >= prm.n || row0 >= prm.m) break;        // warp-uniform
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the previous box has been read
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            uint32_t words[4];
+#pragma unroll
+            for (int q = 0; q < PER / 4; q++) {
+                float *v = &sum[b * WIDTH + j * PER + q * 4];
+                const int src = (b * WIDTH + j * PER) / 4 + q;
+                float z[4] = {v[0], v[1], v[2], v[3]};
+                if (prm.bias) {
+                    z[0] = __fadd_rn(z[0], __shfl_sync(0xffffffffu, bias_lane.x, src));
+                    z[1] = __fadd_rn(z[1], __shfl_sync(0xffffffffu, bias_lane.y, src));
+                    z[2] = __fadd_rn(z[2], __shfl_sync(0xffffffffu, bias_lane.z, src));
+                    z[3] = __fadd_rn(z[3], __shfl_sync(0xffffffffu, bias_lane.w, src));
+                }
+                if constexpr (GENERAL) {
+                    const float4 a = mx_activate4(prm.act, make_float4(z[0], z[1], z[2], z[3]));
+                    z[0] = a.x; z[1] = a.y; z[2] = a.z; z[3] = a.w;
+                } else if (prm.act) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[e] = relu_value(z[e]);
+                }
+                if constexpr (KIND == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) words[e] = __float_as_uint(z[e]);
+                } else {
+                    words[2 * q] = low_canonical_nan2<KIND>(low_pack2<KIND>(z[0], z[1]));
+                    words[2 * q + 1] = low_canonical_nan2<KIND>(low_pack2<KIND>(z[2], z[3]));
+                }
+            }
+            const uint32_t dst = stage + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) << 4));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(words[0]), "r"(words[1]), "r"(words[2]), "r"(words[3]) : "memory");
+        }
+        if (prm.staged) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(map_out, stage, c0, row0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        } else {
+            __syncwarp();
+            const int rows = prm.m - row0 < 32 ? prm.m - row0 : 32;
+            for (int r = 0; r < rows; r++) {
+                T *out = (T *)prm.out + (int64_t)(row0 + r) * prm.n + c0;
+                uint32_t w;
+                if constexpr (KIND == 0) {
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(stage + (uint32_t)(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)));
+                    if (c0 + lane < prm.n) out[lane] = __uint_as_float(w);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int c = h * 32 + lane;
+                        uint16_t e;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e) : "r"(stage + (uint32_t)(r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2)));
+                        if (c0 + c < prm.n) out[c] = e;
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+}
+
+template <int KIND, bool GENERAL>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) mx_linear_pair_kernel(
+        const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
+        const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws, MxLinear prm) {
+    using Cfg = MxPairConfig;
+    using T = typename MxElement<KIND>::type;
+    constexpr int S = Cfg::kStages, BN = Cfg::BN;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * (Cfg::kStageBytes + Cfg::kScaleBytes) + Cfg::kStagingBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 2);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem);
+    const uint32_t staging_base = smem_base + S * Cfg::kStageBytes, scale_base = staging_base + Cfg::kStagingBytes;
+    // full and accumulator-empty barriers are those of the even block; empty and accumulator-full are each block's own
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
+    const uint32_t acc_full_bar = bar_base + 8u * (2 * S), acc_empty_bar = bar_base + 8u * (2 * S + 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        mbar_init(acc_full_bar, 1); mbar_init(acc_empty_bar, 512);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)Cfg::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = prm.tiles_m * prm.tiles_n, kb_count = prm.k_blocks;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            if (lane == 0) {
+                int stage = 0; uint32_t phase = 0;
+                int armed = 0;
+                bool ok = true;
+                for (int tile = pair; tile < total_tiles && ok; tile += pairs) {
+                    int mi, ni;
+                    tile_origin(tile, prm.tiles_m, prm.tiles_n, prm.group_n, mi, ni);
+                    const int m0 = mi * 256 + (int)rank * 128, n0 = ni * BN + (int)rank * 128;
+                    for (int kb = 0; kb < kb_count; kb++) {
+                        if (!mbar_wait_cluster(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                        const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
+                        const uint32_t leader_full = map_to_rank(full_bar(stage), 0);
+                        const uint32_t ss = scale_base + stage * Cfg::kScaleBytes;
+                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * (Cfg::kStageBytes + Cfg::kScaleBytes));
+                        tma_load_2d_pair(sa, &map_x, leader_full, kb * (MX_BK / 2), m0);
+                        tma_load_2d_pair(sa + Cfg::kABytes, &map_w, leader_full, kb * (MX_BK / 2), n0);
+                        // two atoms, 256 words: always a multiple of 16 bytes
+                        tma_load_2d_pair(ss, &map_xs, leader_full, kb * 256, mi * 2 + (int)rank);
+                        tma_load_2d_pair(ss + 2 * MX_ATOM, &map_ws, leader_full, kb * 256, ni * 2);
+                        armed = armed < (1 << 30) ? armed + 1 : armed;
+                        if (++stage == S) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                // giving up: the even block waits for both blocks' copies in flight; the odd one cannot leave before it
+                if ((!ok || *abort_flag) && rank == 0) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
+            }
+        } else if (warp == 1) {
+            if (rank == 0 && lane == 0) {
+                const uint32_t id0 = mx_idesc(256, BN, 0), id2 = mx_idesc(256, BN, 2);
+                int stage = 0; uint32_t phase = 0, done = 0;
+                bool ok = true;
+                for (int tile = pair; tile < total_tiles && ok; tile += pairs, done++) {
+                    if (!mbar_wait_cluster(acc_empty_bar, (done & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    for (int kb = 0; kb < kb_count; kb++) {
+                        if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes, ps = scale_base + stage * Cfg::kScaleBytes;
+                        const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            mx_copy_atom<1>(ts + i * 4, ps + i * MX_ATOM);
+                            mx_copy_atom<1>(ts + 8 + i * 8, ps + (2 + i) * MX_ATOM);
+                            mx_copy_atom<1>(ts + 12 + i * 8, ps + (4 + i) * MX_ATOM);
+                        }
+#pragma unroll
+                        for (int k4 = 0; k4 < 4; k4++)
+                            mx_mma<1>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 8,
+                                      (kb != 0 || k4 != 0) ? 1u : 0u);
+                        umma_commit_pair(empty_bar(stage));
+                        umma_commit_pair(map_to_rank(empty_bar(stage), 1));
+                        if (++stage == S) { stage = 0; phase ^= 1u; }
+                    }
+                    if (ok) { umma_commit_pair(acc_full_bar); umma_commit_pair(map_to_rank(acc_full_bar, 1)); }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        uint32_t done = 0;
+        for (int tile = pair; tile < total_tiles; tile += pairs, done++) {
+            int mi, ni;
+            tile_origin(tile, prm.tiles_m, prm.tiles_n, prm.group_n, mi, ni);
+            const int row0 = mi * 256 + (int)rank * 128 + quarter * 32, col0 = ni * BN + half * 128;
+            float4 bias_lane = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (prm.bias) {
+                const T *b = (const T *)prm.bias;
+                const int c = col0 + lane * 4;
+                if (c < prm.n) bias_lane.x = mx_load<KIND>(b + c);
+                if (c + 1 < prm.n) bias_lane.y = mx_load<KIND>(b + c + 1);
+                if (c + 2 < prm.n) bias_lane.z = mx_load<KIND>(b + c + 2);
+                if (c + 3 < prm.n) bias_lane.w = mx_load<KIND>(b + c + 3);
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait_cluster(acc_full_bar, done & 1u, abort_flag))) break;
+            tc_fence_after();
+            float sum[128];
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                float t[16];
+                tmem_load16(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128 + c * 16), t);
+#pragma unroll
+                for (int i = 0; i < 16; i++) sum[c * 16 + i] = t[i];
+            }
+            tc_fence_before();
+            mbar_arrive_cluster(map_to_rank(acc_empty_bar, 0));
+            mx_emit<KIND, GENERAL>(prm, &map_out, staging_base + (uint32_t)((warp - 4) * 4096), row0, col0, sum, bias_lane, lane);
+        }
+        staged_drain(lane);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    __syncwarp();
+    cluster_sync_all();     // neither block frees tensor memory or leaves while the partner may still signal it
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(prm.error_word, ERR_WAIT_TIMEOUT);
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)Cfg::kTmemCols) : "memory");
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // Weight gradient from an 8-bit checkpoint, one thread per result.
 // ------------------------------------------------------------------------------------------------
@@ -575,7 +845,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_weight_gradient_simple_kernel(i
 #define MX_KINDS(dtype, CALL) ((dtype) == DType::F32 ? CALL(0) : (dtype) == DType::BF16 ? CALL(1) : (dtype) == DType::F16 ? CALL(2) : cudaErrorInvalidValue)
 
 template <int FORMAT, int KIND>
-static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales) {
+static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles) {
     using T = typename MxElement<KIND>::type;
     const int64_t rows = ix.shape[0] * ix.shape[1] * ix.shape[2], cols = ix.shape[3];
     if (rows == 0 || cols == 0) return cudaSuccess;
@@ -590,16 +860,16 @@ static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index
     }
     const bool vec = even && (ix.sa[3] == 1 || cols == 1) && ((uintptr_t)x & 15) == 0 && (rows == 1 || row_step * (int64_t)sizeof(T) % 16 == 0);
     // dense rows of whole scale words are one long row
-    const bool flat = vec && row_step == cols && cols % (4 * MX_BLOCK) == 0;
+    const bool flat = vec && !tiles && row_step == cols && cols % (4 * MX_BLOCK) == 0;
     const MxRows r = flat ? mx_rows(1, rows * cols) : mx_rows(rows, cols);
-    if (vec) mx_quantize_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, 1, codes, scales);
-    else mx_quantize_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, even, codes, scales);
+    if (vec) mx_quantize_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, 1, codes, scales, tiles);
+    else mx_quantize_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, even, codes, scales, tiles);
     return cudaGetLastError();
 }
 
-cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales) {
-#define CALL4(KIND) launch_mx_quantize<4, KIND>(s, x, ix, codes, scales)
-#define CALL8(KIND) launch_mx_quantize<8, KIND>(s, x, ix, codes, scales)
+cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles) {
+#define CALL4(KIND) launch_mx_quantize<4, KIND>(s, x, ix, codes, scales, tiles)
+#define CALL8(KIND) launch_mx_quantize<8, KIND>(s, x, ix, codes, scales, tiles)
     return format == 4 ? MX_KINDS(dtype, CALL4) : format == 8 ? MX_KINDS(dtype, CALL8) : cudaErrorInvalidValue;
 #undef CALL4
 #undef CALL8
@@ -661,6 +931,18 @@ static bool make_code_map(CUtensorMap *map, const uint8_t *codes, int64_t rows, 
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tensor map over tiled scales: rows are the bands of 128 rows; boxes of two atoms x `bands`.
+static bool make_tile_map(CUtensorMap *map, const uint8_t *tiles, int64_t rows, int64_t k, int bands) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)(mx_tile_atoms(k) * MX_ATOM / 4), (cuuint64_t)((rows + 127) / 128)};
+    cuuint64_t strides[1] = {(cuuint64_t)(mx_tile_atoms(k) * MX_ATOM)};
+    cuuint32_t box[2] = {256, (cuuint32_t)bands};
+    cuuint32_t elem[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t *>(tiles), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BN, int KIND>
 static cudaError_t launch_mx_few(cudaStream_t s, const uint8_t *x, const uint8_t *w, const MxLinear &prm, int slices) {
     using Cfg = MxFewConfig<BN>;
@@ -681,8 +963,65 @@ static cudaError_t launch_mx_few(cudaStream_t s, const uint8_t *x, const uint8_t
     return cudaLaunchKernelEx(&cfg, mx_linear_few_kernel<BN, KIND>, map_w, map_x, prm, slices);
 }
 
+template <int KIND, bool GENERAL>
+static cudaError_t launch_mx_pair(cudaStream_t s, const uint8_t *x, const uint8_t *w, const uint8_t *x_tiles, const uint8_t *w_tiles, MxLinear prm, int sm_count) {
+    using Cfg = MxPairConfig;
+    using T = typename MxElement<KIND>::type;
+    CUtensorMap map_x, map_w, map_out, map_xs, map_ws;
+    const int64_t k = (int64_t)prm.blocks * MX_BLOCK;
+    EncodeTiledFn fn = encode_fn();
+    if (!fn || !make_code_map(&map_x, x, prm.m, k, 128) || !make_code_map(&map_w, w, prm.n, k, 128)
+        || !make_tile_map(&map_xs, x_tiles, prm.m, k, 1) || !make_tile_map(&map_ws, w_tiles, prm.n, k, 2)) return cudaErrorInvalidValue;
+    prm.staged = 0;
+    map_out = map_x;            // unused unless staged
+    if ((int64_t)prm.n * sizeof(T) % 16 == 0 && ((uintptr_t)prm.out & 15) == 0) {
+        cuuint64_t dims[2] = {(cuuint64_t)prm.n, (cuuint64_t)prm.m};
+        cuuint64_t strides[1] = {(cuuint64_t)prm.n * sizeof(T)};
+        cuuint32_t box[2] = {128 / sizeof(T), 32};
+        cuuint32_t elem[2] = {1, 1};
+        prm.staged = fn(&map_out, KIND == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, prm.out, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    prm.tiles_m = (prm.m + 255) / 256; prm.tiles_n = (prm.n + 255) / 256;
+    if ((int64_t)prm.tiles_m * prm.tiles_n >= (1ll << 30)) return cudaErrorInvalidValue;
+    const int groups = (prm.tiles_n + 7) / 8;
+    prm.group_n = (prm.tiles_n + groups - 1) / groups;
+    const int tiles = prm.tiles_m * prm.tiles_n, pairs = sm_count / 2;
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaFuncGetAttributes(&attr, mx_linear_pair_kernel<KIND, GENERAL>);
+    if (e != cudaSuccess) return e;
+    // the register split draws on what the block was launched with
+    if (attr.numRegs * MX_PAIR_THREADS < 128 * 72 + 256 * 216) return cudaErrorLaunchOutOfResources;
+    e = cudaFuncSetAttribute(mx_linear_pair_kernel<KIND, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    mx_linear_pair_kernel<KIND, GENERAL><<<2 * (tiles < pairs ? tiles : pairs), MX_PAIR_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_w, map_out, map_xs, map_ws, prm);
+    return cudaGetLastError();
+}
+
+// SYNAPTIK_CUDA_MX_PAIR=0 / 1 forces the one-SM / two-SM form of the 4-bit product (for comparisons).
+static int forced_mx_pair() {
+    static const int v = [] { const char *e = getenv("SYNAPTIK_CUDA_MX_PAIR"); return e && (e[0] == '0' || e[0] == '1') ? e[0] - '0' : -1; }();
+    return v;
+}
+
+bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count) {
+    if (sm_count < 2) return false;
+    if (forced_mx_pair() >= 0) return forced_mx_pair() == 1;
+    return m > 256;
+}
+int64_t mx_tile_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * mx_tile_atoms(k) * MX_ATOM; }
+cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles) {
+    if (rows == 0) return cudaSuccess;
+    const int64_t blocks = ((rows + 127) / 128 * 32 * ((mx_blocks(k) + 3) / 4) + MX_THREADS - 1) / MX_THREADS;
+    mx_tile_scales_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(scales, rows, mx_blocks(k), tiles);
+    return cudaGetLastError();
+}
+
 template <int KIND>
-static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint8_t *w, MxLinear prm, int sm_count) {
+static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint8_t *w, const uint8_t *x_tiles, const uint8_t *w_tiles, MxLinear prm, int sm_count) {
+    if (x_tiles && w_tiles)
+        return prm.act && prm.act != (int)Op::RELU ? launch_mx_pair<KIND, true>(s, x, w, x_tiles, w_tiles, prm, sm_count)
+                                                   : launch_mx_pair<KIND, false>(s, x, w, x_tiles, w_tiles, prm, sm_count);
     const int bn = prm.m <= 16 ? 16 : prm.m <= 32 ? 32 : prm.m <= 64 ? 64 : 128;
     prm.tiles_n = (prm.n + 127) / 128; prm.tiles_m = (prm.m + bn - 1) / bn;
     const int64_t tiles = (int64_t)prm.tiles_n * prm.tiles_m;
@@ -698,13 +1037,14 @@ static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint
 }
 
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
-                      const uint8_t *w, const uint8_t *w_scales, const void *bias, void *out, int sm_count, int *error_word) {
+                      const uint8_t *w, const uint8_t *w_scales, const uint8_t *x_tiles, const uint8_t *w_tiles, const void *bias, void *out,
+                      int sm_count, int *error_word) {
     if (m == 0 || n == 0) return cudaSuccess;
     MxLinear prm = {};
     prm.m = (int)m; prm.n = (int)n; prm.blocks = (int)(k / MX_BLOCK); prm.k_blocks = (int)((k + MX_BK - 1) / MX_BK);
     prm.scale_pitch = mx_scale_bytes(k); prm.xs = x_scales; prm.ws = w_scales;
     prm.bias = bias; prm.out = out; prm.act = act; prm.error_word = error_word;
-#define CALL(KIND) launch_mx_linear<KIND>(s, x, w, prm, sm_count)
+#define CALL(KIND) launch_mx_linear<KIND>(s, x, w, x_tiles, w_tiles, prm, sm_count)
     return MX_KINDS(dtype, CALL);
 #undef CALL
 }

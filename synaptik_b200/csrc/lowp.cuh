@@ -27,6 +27,19 @@ template <int KIND> __device__ __forceinline__ uint16_t low_encode(float x) {
     }
 }
 template <int KIND> __device__ __forceinline__ float low_round(float x) { return low_decode<KIND>(low_encode<KIND>(x)); }
+// Two values narrowed at once, the first in the low half.
+template <int KIND> __device__ __forceinline__ uint32_t low_pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (KIND == 1) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// The packed instructions give every NaN as 0x7FFF; the storage types' NaN is 0x7FC0 / 0x7E00 (low_encode).
+template <int KIND> __device__ __forceinline__ uint32_t low_canonical_nan2(uint32_t r) {
+    constexpr uint32_t inf2 = KIND == 1 ? 0x7F807F80u : 0x7C007C00u, nan2 = KIND == 1 ? 0x7FC07FC0u : 0x7E007E00u;
+    const uint32_t mask = __vcmpgtu2(r & 0x7FFF7FFFu, inf2);
+    return mask ? ((r & ~mask) | (nan2 & mask)) : r;
+}
 
 // FLOAT32 working result of an activation on an exactly decoded low input, before the one narrowing.
 // SIGMOID, SILU and both GELUs are FLOAT32 composites, every product, sum and quotient a binary32 rounding,

@@ -130,6 +130,10 @@ PlaneKey plane_key(const View &v, int orientation) {
                     v.shape[c], v.shape[c] == 1 ? 0 : v.strides[c]};
 }
 
+// Scales of a 4-bit operand of two-SM products, in tiles; filled by the MX_QUANTIZE that makes them, else by a pass of
+// its own, once per run.
+struct MxTiles { uint8_t *ptr = nullptr; int last_run = -1; };
+
 struct StepExec {
     kern::TensorCoreGemm *tc = nullptr;
     int planes_a = -1, planes_b = -1;       // indices into Executable::planes of the MATMUL's two operands
@@ -155,6 +159,7 @@ struct Executable {
     void *constants = nullptr;              // 8 bytes per constant slot
     std::vector<Planes> planes;
     std::map<PlaneKey, int> plane_index;
+    std::map<int, MxTiles> mx_tiles;        // by the program value of the scales
     float *gemm_workspace = nullptr;        // partial products of GEMMs whose contraction is split into slices
     int64_t gemm_workspace_floats = 0;
     int *unit_counters = nullptr;           // one per plan step, zeroed at the start of every run (dynamic tile assignment)
@@ -434,6 +439,15 @@ int32_t prepare_executable(Executable *x) {
             se.tc = kern::tc_gemm_prepare(se.tc_p, se.tc_q, se.tc_m, se.tc_n, st.k, ctx->sm_count, mode, &status);
             if (se.tc) workspace_floats = std::max(workspace_floats, kern::tc_gemm_workspace_floats(se.tc));
             if (!se.tc) return status;
+        } else if (st.kind == StepKind::MX_LINEAR && st.m > 0 && kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) {
+            for (int operand = 0; operand < 2; operand++) {
+                const int64_t bytes = kern::mx_tile_bytes(operand ? st.n : st.m, st.k);
+                MxTiles &tiles = x->mx_tiles[operand ? st.scale_b : st.scale_a];
+                if (tiles.ptr) continue;
+                void *p; if (!alloc((uint64_t)bytes, &p)) return ALLOCATION_FAILED;
+                if (cudaMemsetAsync(p, 0, (uint64_t)bytes, ctx->stream) != cudaSuccess) return EXECUTION_FAILED;
+                tiles.ptr = (uint8_t *)p;
+            }
         } else if (st.kind == StepKind::GEMM && st.engine == GemmEngine::NARROW_REDUCE) {
             void *p; if (!alloc((uint64_t)kern::narrow_reduce_partial_floats(st.m, st.n, st.k) * 4, &p)) return ALLOCATION_FAILED;
             se.narrow_partials = (float *)p;
@@ -710,18 +724,33 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 break;
             case StepKind::MX_QUANTIZE: {
                 const View &a = plan.views[st.a];
+                auto tiles = x->mx_tiles.find(st.out2);
                 LAUNCH(kern::mx_quantize(s, (int)st.scalar_bits, a.dtype, ptr(st.a), index4(a.shape, &a.strides, nullptr, nullptr, &a.shape),
-                                         (uint8_t *)ptr(st.out), (uint8_t *)ptr(st.out2)));
+                                         (uint8_t *)ptr(st.out), (uint8_t *)ptr(st.out2), tiles != x->mx_tiles.end() ? tiles->second.ptr : nullptr));
+                if (tiles != x->mx_tiles.end()) tiles->second.last_run = x->run_counter;
                 break;
             }
             case StepKind::MX_RESTORE:
                 LAUNCH(kern::mx_restore(s, (int)st.scalar_bits, plan.views[st.out].dtype, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
                                         st.m, st.n, ptr(st.out)));
                 break;
-            case StepKind::MX_LINEAR:
+            case StepKind::MX_LINEAR: {
+                const uint8_t *tiles[2] = {nullptr, nullptr};
+                for (int operand = 0; operand < 2; operand++) {
+                    const int value = operand ? st.scale_b : st.scale_a;
+                    auto it = x->mx_tiles.find(value);
+                    if (it == x->mx_tiles.end() || !kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) continue;
+                    if (it->second.last_run != x->run_counter) {
+                        LAUNCH(kern::mx_tile_scales(s, (const uint8_t *)ptr(value), operand ? st.n : st.m, st.k, it->second.ptr));
+                        it->second.last_run = x->run_counter;
+                    }
+                    tiles[operand] = it->second.ptr;
+                }
                 LAUNCH(kern::mx_linear(s, plan.views[st.out].dtype, st.act, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
-                                       (const uint8_t *)ptr(st.b), (const uint8_t *)ptr(st.scale_b), ptr(st.bias), ptr(st.out), ctx->sm_count, ctx->error_dev));
+                                       (const uint8_t *)ptr(st.b), (const uint8_t *)ptr(st.scale_b), tiles[0], tiles[1], ptr(st.bias), ptr(st.out),
+                                       ctx->sm_count, ctx->error_dev));
                 break;
+            }
             case StepKind::MX_WEIGHT_GRADIENT:
                 LAUNCH(kern::mx_weight_gradient(s, plan.views[st.b].dtype, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
                                                 ptr(st.b), (float *)ptr(st.out), ctx->sm_count, ctx->error_dev));

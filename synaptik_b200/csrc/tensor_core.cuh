@@ -150,6 +150,21 @@ __device__ __forceinline__ void staged_drain(int lane) {
     __syncwarp();
 }
 
+// Tile order of the two-SM kernels.  The 74 pairs work on 74 consecutive tiles at a time.  In plain
+// row-major order those cover every tile column and few row bands, so all of Q (134 MB of planes for a
+// 4096 x 4096 weight) cycles through L2 once per few row bands and is read from DRAM again and again
+// (measured: 16.7 GB per 65536 x 4096 x 4096 product whose operands are 2.3 GB).  Grouped order: the
+// tile columns are cut into groups of group_n, and each group is swept down all row bands before the
+// next group starts, so the tiles in flight share fewer distinct Q columns and more P row bands.
+__device__ __forceinline__ void tile_origin(int tile, int tiles_m, int tiles_n, int group_n, int &mi, int &ni) {
+    const int per_group = tiles_m * group_n;
+    const int g = tile / per_group, within = tile - g * per_group;
+    const int first = g * group_n;
+    const int width = tiles_n - first < group_n ? tiles_n - first : group_n;     // the last group may be narrower
+    mi = within / width;
+    ni = first + (within - mi * width);
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
