@@ -402,6 +402,13 @@ __device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && global_timer() - start < 100000000ull) { }
 }
 
+// One lane waits for the warp.
+__device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int lane) {
+    if (lane == 0) mbar_wait_cluster(bar, parity, abort_flag);
+    __syncwarp();
+    return *abort_flag == 0;
+}
+
 struct MxLinear {
     int m, n, blocks, k_blocks;         // blocks: contraction blocks of 32; k_blocks: of 256
     int64_t scale_pitch;
@@ -822,21 +829,333 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Weight gradient from an 8-bit checkpoint, one thread per result.
+// Weight gradient from an 8-bit checkpoint: D[n, k] = sum over rows of g[row, n] x[row, k] on the tensor cores
+// (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k.
+//   An E4M3 element under a power-of-two scale is a BFLOAT16 number as it stands (below 2^-133 it rounds), so the
+// checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly: 8 + 8 + 8 significand bits for
+// FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
+// takes three products at the BFLOAT16 rate where a split into TF32 numbers would take three at half of it.
+//   Both operands are contracted along their rows, that is, they are MN-major tiles (64 columns of one row = one
+// 128-byte swizzle row).  Eight worker warps per block fetch the rows, convert and write them in that form, so no
+// converted copy of either matrix exists in memory.  Tensor memory adds with truncation, so it only holds partial sums
+// of MX_CHUNK stages, which the workers, who have the time, add into FP32 registers: two accumulators in turn.
+//   Work is cut into units of one tile and one slice of the rows where that fills the block pairs better; slices go to
+// a workspace and are added in ascending order by a second kernel.
 // ------------------------------------------------------------------------------------------------
-template <int KIND>
-__global__ void __launch_bounds__(MX_THREADS) mx_weight_gradient_simple_kernel(int64_t rows, int64_t n, int64_t k, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                                                                               const typename MxElement<KIND>::type *__restrict__ g, float *__restrict__ out) {
-    const int64_t code_pitch = mx_blocks(k) * MX_BLOCK, scale_pitch = mx_scale_bytes(k);
-    for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i < n * k; i += (int64_t)gridDim.x * MX_THREADS) {
-        const int64_t col = i / k, feature = i - col * k;
-        double sum = 0.0;
-        for (int64_t r = 0; r < rows; r++) {
-            float a, b;
-            mx_decode8x2(codes[r * code_pitch + feature], a, b);
-            sum += (double)(a * mx_scale_value(scales[r * scale_pitch + feature / MX_BLOCK])) * (double)mx_load<KIND>(g + r * n + col);
+constexpr int MX_ROWS = 64;             // rows per stage
+constexpr int MX_GRAD_THREADS = 384;    // warp 0 MMA, warps 4-11 workers
+constexpr int MX_GRAD_REGS_LOW = 40, MX_GRAD_REGS_WORKER = 232;
+
+template <int KIND> struct MxGradConfig {
+    static constexpr int kPieces = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
+    static constexpr int kTileBytes = MX_ROWS * 128 * 2;                // one operand piece of 128 columns
+    static constexpr int kStageBytes = (kPieces + 1) * kTileBytes;
+    static constexpr int kStages = KIND == 0 ? 3 : KIND == 1 ? 6 : 4;
+    static constexpr int kChunk = KIND == 0 ? 4 : 8;                    // stages per partial sum in tensor memory
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+};
+
+struct MxGrad {
+    int64_t rows; int n, k;
+    const uint8_t *codes, *scales; const void *g;
+    int64_t code_pitch, scale_pitch;
+    int tiles_n, tiles_k, slices;
+    int stages, stages_per_slice;       // of MX_ROWS rows
+    float *out; int64_t slice_floats;   // [slices][n][k]
+    int *error_word;
+};
+
+// Two floats as the next piece: the upper 16 bits of each (truncation keeps the remainder exact), which are taken off.
+__device__ __forceinline__ uint32_t mx_piece(float &a, float &b) {
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    const uint32_t word = __byte_perm(ua, ub, 0x7632);
+    // an infinity has no remainder (infinity - infinity would be NaN); a NaN leaves a NaN
+    a = fabsf(a) == __uint_as_float(0x7f800000u) ? 0.0f : __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
+    b = fabsf(b) == __uint_as_float(0x7f800000u) ? 0.0f : __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
+    return word;
+}
+__device__ __forceinline__ void mx_store_chunk(uint32_t tile, int row, int chunk, const uint32_t (&w)[4]) {
+    const uint32_t dst = tile + (uint32_t)((chunk >> 3) * (MX_ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
+// What a worker thread holds of a stage: four groups of eight columns of g and one block of the checkpoint, all of one row.
+template <int KIND> struct MxStageRegs { uint4 g[4][KIND == 0 ? 2 : 1]; uint4 x[2]; uint32_t scale; };
+
+template <int KIND, bool VEC>
+__device__ __forceinline__ void mx_fetch_stage(const MxGrad &prm, int64_t row, int n0, int k0, int lane, MxStageRegs<KIND> &v) {
+    using T = typename MxElement<KIND>::type;
+    const bool here = row < prm.rows;
+    const T *g = (const T *)prm.g + row * prm.n;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int c = n0 + (j * 4 + (lane >> 3)) * 8;
+#pragma unroll
+        for (int h = 0; h < (KIND == 0 ? 2 : 1); h++) v.g[j][h] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (VEC) {            // rows are whole groups of eight columns
+            if (here && c < prm.n) {
+#pragma unroll
+                for (int h = 0; h < (KIND == 0 ? 2 : 1); h++) v.g[j][h] = __ldg(reinterpret_cast<const uint4 *>(g + c) + h);
+            }
+        } else if (here) {
+            if constexpr (KIND == 0) {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) t[e] = c + e < prm.n ? __ldg(g + c + e) : 0.0f;
+                v.g[j][0] = make_uint4(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3]));
+                v.g[j][KIND == 0 ? 1 : 0] = make_uint4(__float_as_uint(t[4]), __float_as_uint(t[5]), __float_as_uint(t[6]), __float_as_uint(t[7]));
+            } else {
+                uint32_t t[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) t[e] = c + e < prm.n ? (uint32_t)__ldg(g + c + e) : 0u;
+                v.g[j][0] = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+            }
         }
-        out[i] = (float)sum;
+    }
+    const int c = k0 + (lane >> 3) * MX_BLOCK;
+    v.x[0] = v.x[1] = make_uint4(0u, 0u, 0u, 0u);
+    v.scale = 0u;
+    if (here && c < prm.k) {
+        const uint4 *x = reinterpret_cast<const uint4 *>(prm.codes + row * prm.code_pitch + c);
+        v.x[0] = __ldg(x); v.x[1] = __ldg(x + 1);
+        v.scale = __ldg(prm.scales + row * prm.scale_pitch + (c >> 5));
+    }
+}
+
+// Converts and writes a stage: pieces of g, smallest last in memory, then the checkpoint.
+template <int KIND>
+__device__ __forceinline__ void mx_put_stage(uint32_t stage, int row, int lane, const MxStageRegs<KIND> &v) {
+    using Cfg = MxGradConfig<KIND>;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int chunk = j * 4 + (lane >> 3);
+        if constexpr (KIND == 1) {
+            const uint32_t w[4] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w};
+            mx_store_chunk(stage, row, chunk, w);
+        } else {
+            float f[8];
+            if constexpr (KIND == 0) {
+                const uint32_t u[8] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w, v.g[j][1].x, v.g[j][1].y, v.g[j][1].z, v.g[j][1].w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = __uint_as_float(u[e]);
+            } else {
+                const uint32_t u[4] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) low_unpack_half2(u[e], f[2 * e], f[2 * e + 1]);
+            }
+#pragma unroll
+            for (int piece = 0; piece < Cfg::kPieces; piece++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = mx_piece(f[2 * e], f[2 * e + 1]);
+                mx_store_chunk(stage + piece * Cfg::kTileBytes, row, chunk, w);
+            }
+        }
+    }
+    const uint32_t tile = stage + Cfg::kPieces * Cfg::kTileBytes;
+    const float scale = mx_scale_value(v.scale);
+    const uint32_t x[8] = {v.x[0].x, v.x[0].y, v.x[0].z, v.x[0].w, v.x[1].x, v.x[1].y, v.x[1].z, v.x[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float a, b;
+            mx_decode8x2(x[i * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
+            w[e] = low_pack2<1>(a * scale, b * scale);
+        }
+        mx_store_chunk(tile, row, (lane >> 3) * 4 + i, w);
+    }
+}
+
+template <int KIND, bool VEC>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) mx_weight_gradient_kernel(MxGrad prm) {
+    using Cfg = MxGradConfig<KIND>;
+    constexpr int S = Cfg::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem);
+    // full and accumulator-empty barriers are those of the even block (one arrival per worker warp of both blocks);
+    // empty and accumulator-full are each block's own
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
+    auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * S + a); };
+    auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 16); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 16); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int units = prm.tiles_n * prm.tiles_k * prm.slices;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    // stages of a unit; every slice has at least one
+    auto first_stage = [&](int unit) { return unit % prm.slices * prm.stages_per_slice; };
+    auto stage_count = [&](int unit) { const int left = prm.stages - first_stage(unit); return left < prm.stages_per_slice ? left : prm.stages_per_slice; };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_LOW));
+        if (warp == 0 && rank == 0 && lane == 0) {
+            // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+            // groups of 64 columns 8 KB apart (leading offset), groups of 8 rows 1 KB (stride offset), 128-byte swizzle
+            const uint64_t fixed = ((uint64_t)((MX_ROWS * 128u) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+            auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
+            int stage = 0; uint32_t phase = 0, chunk = 0;
+            bool ok = true;
+            for (int unit = pair; unit < units && ok; unit += pairs) {
+                const int count = stage_count(unit);
+                for (int i0 = 0; i0 < count && ok; i0 += Cfg::kChunk, chunk++) {
+                    const int buf = chunk & 1;
+                    if (!mbar_wait_cluster(acc_empty_bar(buf), ((chunk >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + (uint32_t)(buf * 256);
+                    const int i1 = i0 + Cfg::kChunk < count ? i0 + Cfg::kChunk : count;
+                    for (int i = i0; i < i1; i++) {
+                        if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kPieces * Cfg::kTileBytes;
+#pragma unroll
+                        for (int piece = Cfg::kPieces - 1; piece >= 0; piece--)         // small terms first
+#pragma unroll
+                            for (int r16 = 0; r16 < MX_ROWS / 16; r16++)
+                                umma_f16_pair(d, desc(pa + piece * Cfg::kTileBytes + r16 * 2048), desc(pb + r16 * 2048), idesc,
+                                              (i != i0 || piece != Cfg::kPieces - 1 || r16 != 0) ? 1u : 0u);
+                        umma_commit_pair(empty_bar(stage));
+                        umma_commit_pair(map_to_rank(empty_bar(stage), 1));
+                        if (++stage == S) { stage = 0; phase ^= 1u; }
+                    }
+                    if (ok) { umma_commit_pair(acc_full_bar(buf)); umma_commit_pair(map_to_rank(acc_full_bar(buf), 1)); }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_WORKER));
+        const int worker = warp - 4, row_in_stage = worker * 8 + (lane & 7);
+        const int quarter = warp & 3, half = worker >> 2;
+        float sum[128];
+        int stage = 0; uint32_t phase = 0, chunk = 0;
+        bool ok = true;
+        // the chunk that still waits in tensor memory: its unit (-1 none), whether it is the unit's first and last
+        int open_unit = -1; bool open_first = false, open_last = false;
+        auto tile_of = [&](int unit, int &n0, int &k0) {
+            const int tile = unit / prm.slices;
+            n0 = tile % prm.tiles_n * 256 + (int)rank * 128; k0 = tile / prm.tiles_n * 256;
+        };
+        auto promote = [&](uint32_t c) {
+            const int buf = c & 1;
+            ok = mx_warp_wait(acc_full_bar(buf), (c >> 1) & 1u, abort_flag, lane);
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                float t[16];
+                tmem_load16(taddr + (uint32_t)(q * 16), t);
+#pragma unroll
+                for (int e = 0; e < 16; e++) sum[q * 16 + e] = open_first ? t[e] : __fadd_rn(sum[q * 16 + e], t[e]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(acc_empty_bar(buf), 0));
+            if (!open_last) return;
+            int n0, k0;
+            tile_of(open_unit, n0, k0);
+            const int n = n0 + quarter * 32 + lane, c0 = k0 + half * 128;
+            if (n >= prm.n) return;
+            float *out = prm.out + open_unit % prm.slices * prm.slice_floats + (int64_t)n * prm.k + c0;
+            const bool vec = (prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0;
+#pragma unroll
+            for (int q = 0; q < 32; q++) {
+                if (vec) { if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]); }
+                else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) if (c0 + q * 4 + e < prm.k) out[q * 4 + e] = sum[q * 4 + e];
+                }
+            }
+        };
+        MxStageRegs<KIND> regs;
+        if (pair < units) {
+            int n0, k0;
+            tile_of(pair, n0, k0);
+            mx_fetch_stage<KIND, VEC>(prm, (int64_t)first_stage(pair) * MX_ROWS + row_in_stage, n0, k0 + (int)rank * 128, lane, regs);
+        }
+        for (int unit = pair; unit < units && ok; unit += pairs) {
+            int n0, k0;
+            tile_of(unit, n0, k0);
+            const int count = stage_count(unit);
+            for (int i = 0; i < count; i++) {
+                ok = mx_warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, lane);
+                if (!ok) break;
+                mx_put_stage<KIND>(smem_base + stage * Cfg::kStageBytes, row_in_stage, lane, regs);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(full_bar(stage), 0));
+                if (++stage == S) { stage = 0; phase ^= 1u; }
+                // the next stage's rows, of this unit or the next one
+                if (i + 1 < count) mx_fetch_stage<KIND, VEC>(prm, (int64_t)(first_stage(unit) + i + 1) * MX_ROWS + row_in_stage, n0, k0 + (int)rank * 128, lane, regs);
+                else if (unit + pairs < units) {
+                    int n1, k1;
+                    tile_of(unit + pairs, n1, k1);
+                    mx_fetch_stage<KIND, VEC>(prm, (int64_t)first_stage(unit + pairs) * MX_ROWS + row_in_stage, n1, k1 + (int)rank * 128, lane, regs);
+                }
+                if ((i + 1) % Cfg::kChunk == 0 || i + 1 == count) {
+                    // a chunk has been handed over: the one before it is done, or nearly
+                    if (open_unit >= 0) { promote(chunk - 1); if (!ok) break; }
+                    open_unit = unit; open_first = i < Cfg::kChunk; open_last = i + 1 == count;
+                    chunk++;
+                }
+            }
+        }
+        if (ok && open_unit >= 0) promote(chunk - 1);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    __syncwarp();
+    cluster_sync_all();     // neither block frees tensor memory or leaves while the partner may still signal it
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(prm.error_word, ERR_WAIT_TIMEOUT);
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
+}
+
+// out = the slices' sums in ascending order.
+__global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(const float *__restrict__ ws, int slices, int64_t count, float *__restrict__ out) {
+    for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i * 4 < count; i += (int64_t)gridDim.x * MX_THREADS) {
+        const int64_t at = i * 4;
+        if (at + 3 < count && (count & 3) == 0 && ((uintptr_t)out & 15) == 0) {
+            float4 a = __ldg(reinterpret_cast<const float4 *>(ws + at));
+            for (int q = 1; q < slices; q++) {
+                const float4 b = __ldg(reinterpret_cast<const float4 *>(ws + q * count + at));
+                a.x = __fadd_rn(a.x, b.x); a.y = __fadd_rn(a.y, b.y); a.z = __fadd_rn(a.z, b.z); a.w = __fadd_rn(a.w, b.w);
+            }
+            *reinterpret_cast<float4 *>(out + at) = a;
+        } else {
+            for (int e = 0; e < 4 && at + e < count; e++) {
+                float a = ws[at + e];
+                for (int q = 1; q < slices; q++) a = __fadd_rn(a, ws[q * count + at + e]);
+                out[at + e] = a;
+            }
+        }
     }
 }
 
@@ -1049,20 +1368,67 @@ cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n
 #undef CALL
 }
 
-template <int KIND>
-static cudaError_t launch_mx_weight_gradient(cudaStream_t s, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales, const void *g, float *out) {
-    using T = typename MxElement<KIND>::type;
-    const int64_t blocks = (n * k + MX_THREADS - 1) / MX_THREADS;
-    mx_weight_gradient_simple_kernel<KIND><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(rows, n, k, codes, scales, (const T *)g, out);
+// Slices of the rows: the choice with the least time in stages, counting a slice's own cost (filling the pipeline, and
+// the second pass over its share of the result) as two stages of 64 rows.
+static int mx_gradient_slices(int64_t rows, int64_t n, int64_t k, int sm_count) {
+    const int64_t tiles = ((n + 255) / 256) * ((k + 255) / 256), pairs = sm_count / 2 > 0 ? sm_count / 2 : 1, stages = (rows + MX_ROWS - 1) / MX_ROWS;
+    int best = 1;
+    double best_cost = 1e300;
+    for (int64_t s = 1; s <= 64 && s <= stages; s++) {
+        const int64_t per = (stages + s - 1) / s;
+        if ((stages + per - 1) / per != s) continue;            // some slice would be empty
+        const double cost = (double)((tiles * s + pairs - 1) / pairs) * ((double)per + 2.0) + (s > 1 ? 4.0 + 0.25 * (double)(tiles * s) / (double)pairs : 0.0);
+        if (cost < best_cost) { best_cost = cost; best = (int)s; }
+    }
+    return best;
+}
+
+int64_t mx_weight_gradient_workspace(int64_t rows, int64_t n, int64_t k, int sm_count) {
+    const int slices = mx_gradient_slices(rows, n, k, sm_count);
+    return slices > 1 ? (int64_t)slices * n * k : 0;
+}
+
+template <int KIND, bool VEC>
+static cudaError_t launch_mx_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
+    using Cfg = MxGradConfig<KIND>;
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaFuncGetAttributes(&attr, mx_weight_gradient_kernel<KIND, VEC>);
+    if (e != cudaSuccess) return e;
+    // the register split draws on what the block was launched with
+    if (attr.numRegs * 3 < MX_GRAD_REGS_LOW + 2 * MX_GRAD_REGS_WORKER) return cudaErrorLaunchOutOfResources;
+    e = cudaFuncSetAttribute(mx_weight_gradient_kernel<KIND, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const int units = prm.tiles_n * prm.tiles_k * prm.slices, pairs = sm_count / 2;
+    mx_weight_gradient_kernel<KIND, VEC><<<2 * (units < pairs ? units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(prm);
     return cudaGetLastError();
 }
 
+template <int KIND>
+static cudaError_t launch_mx_weight_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
+    using T = typename MxElement<KIND>::type;
+    return (int64_t)prm.n % 8 == 0 && ((uintptr_t)prm.g & 15) == 0 ? launch_mx_gradient<KIND, true>(s, prm, sm_count) : launch_mx_gradient<KIND, false>(s, prm, sm_count);
+}
+
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
-                               const void *g, float *out, int sm_count, int *error_word) {
+                               const void *g, float *out, float *workspace, int sm_count, int *error_word) {
     if (n == 0 || k == 0) return cudaSuccess;
-#define CALL(KIND) launch_mx_weight_gradient<KIND>(s, rows, n, k, codes, scales, g, out)
-    return MX_KINDS(dtype, CALL);
+    if (rows == 0) return cudaMemsetAsync(out, 0, (size_t)n * k * 4, s);
+    if (sm_count < 2) return cudaErrorInvalidValue;
+    MxGrad prm = {};
+    prm.rows = rows; prm.n = (int)n; prm.k = (int)k; prm.codes = codes; prm.scales = scales; prm.g = g;
+    prm.code_pitch = mx_code_bytes(8, k); prm.scale_pitch = mx_scale_bytes(k);
+    prm.tiles_n = (int)((n + 255) / 256); prm.tiles_k = (int)((k + 255) / 256);
+    prm.slices = mx_gradient_slices(rows, n, k, sm_count);
+    prm.stages = (int)((rows + MX_ROWS - 1) / MX_ROWS); prm.stages_per_slice = (prm.stages + prm.slices - 1) / prm.slices;
+    prm.out = prm.slices > 1 ? workspace : out; prm.slice_floats = n * k; prm.error_word = error_word;
+    if ((int64_t)prm.tiles_n * prm.tiles_k * prm.slices >= (1ll << 30) || !prm.out) return cudaErrorInvalidValue;
+#define CALL(KIND) launch_mx_weight_gradient<KIND>(s, prm, sm_count)
+    const cudaError_t e = MX_KINDS(dtype, CALL);
 #undef CALL
+    if (e != cudaSuccess || prm.slices == 1) return e;
+    const int64_t blocks = (n * k / 4 + MX_THREADS) / MX_THREADS;
+    mx_add_slices_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(workspace, prm.slices, n * k, out);
+    return cudaGetLastError();
 }
 
 }  // namespace kern
