@@ -396,6 +396,12 @@ __device__ __forceinline__ void mx_copy_scales(uint32_t dst, int atoms, const ui
     }
 }
 
+// Arrival on a barrier of the cluster's block `rank`.  Default (block) scope: what the arrival announces lies in this
+// block's own shared or tensor memory and has been made visible to the tensor core by a proxy or tcgen05 fence; a
+// release at cluster scope waits for every access of the thread, which cost more than a stage's work.
+__device__ __forceinline__ void mx_arrive_rank(uint32_t bar, uint32_t rank) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, rank)) : "memory");
+}
 // Waits, for at most a tenth of a second and whatever the abort flag says, for copies whose barrier nothing else arrives on.
 __device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
     const uint64_t start = global_timer();
@@ -810,7 +816,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                 for (int i = 0; i < 16; i++) sum[c * 16 + i] = t[i];
             }
             tc_fence_before();
-            mbar_arrive_cluster(map_to_rank(acc_empty_bar, 0));
+            mx_arrive_rank(acc_empty_bar, 0);
             mx_emit<KIND, GENERAL>(prm, &map_out, staging_base + (uint32_t)((warp - 4) * 4096), row0, col0, sum, bias_lane, lane);
         }
         staged_drain(lane);
@@ -836,23 +842,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
 // takes three products at the BFLOAT16 rate where a split into TF32 numbers would take three at half of it.
 //   Both operands are contracted along their rows, that is, they are MN-major tiles (64 columns of one row = one
-// 128-byte swizzle row).  Eight worker warps per block fetch the rows, convert and write them in that form, so no
-// converted copy of either matrix exists in memory.  Tensor memory adds with truncation, so it only holds partial sums
+// 128-byte swizzle row).  TMA brings the rows as they are into a ring of raw slots, eight worker warps per block convert
+// them into operand tiles of that form, so no converted copy of either matrix exists in memory; BFLOAT16 gradients need
+// no conversion and go into the operand tiles at once.  (Rows of g that TMA cannot address, widths that are no multiple
+// of 16 bytes, the workers read themselves, one stage ahead.)  Tensor memory adds with truncation, so it only holds partial sums
 // of MX_CHUNK stages, which the workers, who have the time, add into FP32 registers: two accumulators in turn.
 //   Work is cut into units of one tile and one slice of the rows where that fills the block pairs better; slices go to
 // a workspace and are added in ascending order by a second kernel.
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 64;             // rows per stage
-constexpr int MX_GRAD_THREADS = 384;    // warp 0 MMA, warps 4-11 workers
-constexpr int MX_GRAD_REGS_LOW = 40, MX_GRAD_REGS_WORKER = 232;
+constexpr int MX_GRAD_THREADS = 384;    // warp 0 MMA, warp 2 raw slots, warp 3 gradients that need no conversion, warps 4-11 workers
+constexpr int MX_GRAD_REGS_LOW = 56, MX_GRAD_REGS_WORKER = 224;
 
 template <int KIND> struct MxGradConfig {
     static constexpr int kPieces = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
     static constexpr int kTileBytes = MX_ROWS * 128 * 2;                // one operand piece of 128 columns
     static constexpr int kStageBytes = (kPieces + 1) * kTileBytes;
-    static constexpr int kStages = KIND == 0 ? 3 : KIND == 1 ? 6 : 4;
+    static constexpr int kStages = KIND == 0 ? 2 : KIND == 1 ? 5 : 3;
+    static constexpr int kRawG = KIND == 0 ? MX_ROWS * 128 * 4 : KIND == 1 ? 0 : MX_ROWS * 128 * 2;
+    static constexpr int kRawBytes = kRawG + MX_ROWS * 128;             // rows of g, codes of the checkpoint
+    static constexpr int kRawSlots = KIND == 0 ? 2 : KIND == 1 ? 6 : 3;
     static constexpr int kChunk = KIND == 0 ? 4 : 8;                    // stages per partial sum in tensor memory
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kRawSlots * (kRawBytes + MX_ROWS * 4) + 1024 + 512;
 };
 
 struct MxGrad {
@@ -879,116 +890,72 @@ __device__ __forceinline__ void mx_store_chunk(uint32_t tile, int row, int chunk
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
 
-// What a worker thread holds of a stage: four groups of eight columns of g and one block of the checkpoint, all of one row.
-template <int KIND> struct MxStageRegs { uint4 g[4][KIND == 0 ? 2 : 1]; uint4 x[2]; uint32_t scale; };
-
-template <int KIND, bool VEC>
-__device__ __forceinline__ void mx_fetch_stage(const MxGrad &prm, int64_t row, int n0, int k0, int lane, MxStageRegs<KIND> &v) {
-    using T = typename MxElement<KIND>::type;
-    const bool here = row < prm.rows;
-    const T *g = (const T *)prm.g + row * prm.n;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int c = n0 + (j * 4 + (lane >> 3)) * 8;
-#pragma unroll
-        for (int h = 0; h < (KIND == 0 ? 2 : 1); h++) v.g[j][h] = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (VEC) {            // rows are whole groups of eight columns
-            if (here && c < prm.n) {
-#pragma unroll
-                for (int h = 0; h < (KIND == 0 ? 2 : 1); h++) v.g[j][h] = __ldg(reinterpret_cast<const uint4 *>(g + c) + h);
-            }
-        } else if (here) {
-            if constexpr (KIND == 0) {
-                float t[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) t[e] = c + e < prm.n ? __ldg(g + c + e) : 0.0f;
-                v.g[j][0] = make_uint4(__float_as_uint(t[0]), __float_as_uint(t[1]), __float_as_uint(t[2]), __float_as_uint(t[3]));
-                v.g[j][KIND == 0 ? 1 : 0] = make_uint4(__float_as_uint(t[4]), __float_as_uint(t[5]), __float_as_uint(t[6]), __float_as_uint(t[7]));
-            } else {
-                uint32_t t[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) t[e] = c + e < prm.n ? (uint32_t)__ldg(g + c + e) : 0u;
-                v.g[j][0] = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
-            }
-        }
-    }
-    const int c = k0 + (lane >> 3) * MX_BLOCK;
-    v.x[0] = v.x[1] = make_uint4(0u, 0u, 0u, 0u);
-    v.scale = 0u;
-    if (here && c < prm.k) {
-        const uint4 *x = reinterpret_cast<const uint4 *>(prm.codes + row * prm.code_pitch + c);
-        v.x[0] = __ldg(x); v.x[1] = __ldg(x + 1);
-        v.scale = __ldg(prm.scales + row * prm.scale_pitch + (c >> 5));
-    }
-}
-
-// Converts and writes a stage: pieces of g, smallest last in memory, then the checkpoint.
+// Eight columns of one row of g that TMA cannot address.
 template <int KIND>
-__device__ __forceinline__ void mx_put_stage(uint32_t stage, int row, int lane, const MxStageRegs<KIND> &v) {
-    using Cfg = MxGradConfig<KIND>;
+__device__ __forceinline__ void mx_fetch8(const typename MxElement<KIND>::type *row, int c, int n, bool here, uint32_t (&v)[KIND == 0 ? 8 : 4]) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int chunk = j * 4 + (lane >> 3);
-        if constexpr (KIND == 1) {
-            const uint32_t w[4] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w};
-            mx_store_chunk(stage, row, chunk, w);
-        } else {
-            float f[8];
-            if constexpr (KIND == 0) {
-                const uint32_t u[8] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w, v.g[j][1].x, v.g[j][1].y, v.g[j][1].z, v.g[j][1].w};
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = __uint_as_float(u[e]);
-            } else {
-                const uint32_t u[4] = {v.g[j][0].x, v.g[j][0].y, v.g[j][0].z, v.g[j][0].w};
-#pragma unroll
-                for (int e = 0; e < 4; e++) low_unpack_half2(u[e], f[2 * e], f[2 * e + 1]);
-            }
-#pragma unroll
-            for (int piece = 0; piece < Cfg::kPieces; piece++) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = mx_piece(f[2 * e], f[2 * e + 1]);
-                mx_store_chunk(stage + piece * Cfg::kTileBytes, row, chunk, w);
-            }
-        }
-    }
-    const uint32_t tile = stage + Cfg::kPieces * Cfg::kTileBytes;
-    const float scale = mx_scale_value(v.scale);
-    const uint32_t x[8] = {v.x[0].x, v.x[0].y, v.x[0].z, v.x[0].w, v.x[1].x, v.x[1].y, v.x[1].z, v.x[1].w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            float a, b;
-            mx_decode8x2(x[i * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
-            w[e] = low_pack2<1>(a * scale, b * scale);
-        }
-        mx_store_chunk(tile, row, (lane >> 3) * 4 + i, w);
+    for (int e = 0; e < (KIND == 0 ? 8 : 4); e++) {
+        if constexpr (KIND == 0) v[e] = here && c + e < n ? __float_as_uint(__ldg(row + c + e)) : 0u;
+        else v[e] = (here && c + 2 * e < n ? (uint32_t)__ldg(row + c + 2 * e) : 0u) | (here && c + 2 * e + 1 < n ? (uint32_t)__ldg(row + c + 2 * e + 1) << 16 : 0u);
     }
 }
 
-template <int KIND, bool VEC>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) mx_weight_gradient_kernel(MxGrad prm) {
+// Eight columns of one row of g as operand pieces, the leading one first in memory.
+template <int KIND>
+__device__ __forceinline__ void mx_put_pieces(uint32_t stage, int row, int chunk, const uint32_t (&u)[KIND == 0 ? 8 : 4]) {
     using Cfg = MxGradConfig<KIND>;
-    constexpr int S = Cfg::kStages;
+    if constexpr (KIND == 1) mx_store_chunk(stage, row, chunk, u);
+    else {
+        float f[8];
+        if constexpr (KIND == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = __uint_as_float(u[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) low_unpack_half2(u[e], f[2 * e], f[2 * e + 1]);
+        }
+#pragma unroll
+        for (int piece = 0; piece < Cfg::kPieces; piece++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = mx_piece(f[2 * e], f[2 * e + 1]);
+            mx_store_chunk(stage + piece * Cfg::kTileBytes, row, chunk, w);
+        }
+    }
+}
+__device__ __forceinline__ void mx_read16(uint32_t addr, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+
+template <int KIND, bool TMA>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) mx_weight_gradient_kernel(
+        const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, MxGrad prm) {
+    using Cfg = MxGradConfig<KIND>;
+    using T = typename MxElement<KIND>::type;
+    constexpr int S = Cfg::kStages, R = Cfg::kRawSlots;
+    constexpr bool DIRECT = TMA && KIND == 1;           // g goes into the operand tiles as it is
+    constexpr bool RAW_G = TMA && KIND != 1;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes + R * (Cfg::kRawBytes + MX_ROWS * 4));
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 2 * R + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem);
+    const uint32_t raw_base = smem_base + S * Cfg::kStageBytes, scale_base = raw_base + R * Cfg::kRawBytes;
     // full and accumulator-empty barriers are those of the even block (one arrival per worker warp of both blocks);
-    // empty and accumulator-full are each block's own
+    // empty, accumulator-full and the two of the raw slots are each block's own
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
-    auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * S + a); };
-    auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
+    auto raw_full_bar = [&](int i) { return bar_base + 8u * (2 * S + i); };
+    auto raw_empty_bar = [&](int i) { return bar_base + 8u * (2 * S + R + i); };
+    auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 * R + a); };
+    auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 * R + 2 + a); };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 16); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), DIRECT ? 17 : 16); mbar_init(empty_bar(s), 1); }
+        for (int i = 0; i < R; i++) { mbar_init(raw_full_bar(i), 33); mbar_init(raw_empty_bar(i), 8); }     // TMA and 32 lanes of scales
         for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 16); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1008,122 +975,228 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     // stages of a unit; every slice has at least one
     auto first_stage = [&](int unit) { return unit % prm.slices * prm.stages_per_slice; };
     auto stage_count = [&](int unit) { const int left = prm.stages - first_stage(unit); return left < prm.stages_per_slice ? left : prm.stages_per_slice; };
+    auto tile_of = [&](int unit, int &n0, int &k0) {        // of the pair's tile
+        const int tile = unit / prm.slices;
+        n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * 256;
+    };
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_LOW));
-        if (warp == 0 && rank == 0 && lane == 0) {
-            // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
-            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-            // groups of 64 columns 8 KB apart (leading offset), groups of 8 rows 1 KB (stride offset), 128-byte swizzle
-            const uint64_t fixed = ((uint64_t)((MX_ROWS * 128u) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
-            auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
-            int stage = 0; uint32_t phase = 0, chunk = 0;
+        if (warp == 0) {
+            if (rank == 0 && lane == 0) {
+                // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+                // groups of 64 columns 8 KB apart (leading offset), groups of 8 rows 1 KB (stride offset), 128-byte swizzle
+                const uint64_t fixed = ((uint64_t)((MX_ROWS * 128u) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+                auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
+                int stage = 0; uint32_t phase = 0, chunk = 0;
+                bool ok = true;
+                for (int unit = pair; unit < units && ok; unit += pairs) {
+                    const int count = stage_count(unit);
+                    for (int i0 = 0; i0 < count && ok; i0 += Cfg::kChunk, chunk++) {
+                        const int buf = chunk & 1;
+                        if (!mbar_wait_cluster(acc_empty_bar(buf), ((chunk >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t d = tmem_base + (uint32_t)(buf * 256);
+                        const int i1 = i0 + Cfg::kChunk < count ? i0 + Cfg::kChunk : count;
+                        for (int i = i0; i < i1; i++) {
+                            if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                            tc_fence_after();
+                            const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kPieces * Cfg::kTileBytes;
+#pragma unroll
+                            for (int piece = Cfg::kPieces - 1; piece >= 0; piece--)         // small terms first
+#pragma unroll
+                                for (int r16 = 0; r16 < MX_ROWS / 16; r16++)
+                                    umma_f16_pair(d, desc(pa + piece * Cfg::kTileBytes + r16 * 2048), desc(pb + r16 * 2048), idesc,
+                                                  (i != i0 || piece != Cfg::kPieces - 1 || r16 != 0) ? 1u : 0u);
+                            umma_commit_pair(empty_bar(stage));
+                            umma_commit_pair(map_to_rank(empty_bar(stage), 1));
+                            if (++stage == S) { stage = 0; phase ^= 1u; }
+                        }
+                        if (ok) { umma_commit_pair(acc_full_bar(buf)); umma_commit_pair(map_to_rank(acc_full_bar(buf), 1)); }
+                    }
+                }
+            }
+        } else if (warp == 2) {
+            // raw slots: one lane's TMA for the rows, every lane two words of scales
+            int slot = 0; uint32_t phase = 0;
+            int armed = 0;
             bool ok = true;
             for (int unit = pair; unit < units && ok; unit += pairs) {
+                int n0, k0;
+                tile_of(unit, n0, k0);
+                n0 += (int)rank * 128; k0 += (int)rank * 128;
                 const int count = stage_count(unit);
-                for (int i0 = 0; i0 < count && ok; i0 += Cfg::kChunk, chunk++) {
-                    const int buf = chunk & 1;
-                    if (!mbar_wait_cluster(acc_empty_bar(buf), ((chunk >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t d = tmem_base + (uint32_t)(buf * 256);
-                    const int i1 = i0 + Cfg::kChunk < count ? i0 + Cfg::kChunk : count;
-                    for (int i = i0; i < i1; i++) {
-                        if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
-                        tc_fence_after();
-                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kPieces * Cfg::kTileBytes;
+                for (int i = 0; i < count; i++) {
+                    ok = mx_warp_wait(raw_empty_bar(slot), phase ^ 1u, abort_flag, lane);
+                    if (!ok) break;
+                    const int r0 = (first_stage(unit) + i) * MX_ROWS;
+                    const uint32_t raw = raw_base + slot * Cfg::kRawBytes;
+                    if (lane == 0) {
+                        mbar_expect_tx(raw_full_bar(slot), (RAW_G ? Cfg::kRawG : 0) + MX_ROWS * 128);
+                        // boxes of 128 bytes x 64 rows; coordinates along a row are multiples of 128 bytes, what lies past the
+                        // matrix reads as zeros
+                        if constexpr (RAW_G) {
+                            constexpr int WIDTH = 128 / sizeof(T);
 #pragma unroll
-                        for (int piece = Cfg::kPieces - 1; piece >= 0; piece--)         // small terms first
+                            for (int b = 0; b < 128 / WIDTH; b++) tma_load_2d(raw + b * (MX_ROWS * 128), &map_g, raw_full_bar(slot), n0 + b * WIDTH, r0);
+                        }
+                        tma_load_2d(raw + Cfg::kRawG, &map_x, raw_full_bar(slot), k0, r0);
+                    }
 #pragma unroll
-                            for (int r16 = 0; r16 < MX_ROWS / 16; r16++)
-                                umma_f16_pair(d, desc(pa + piece * Cfg::kTileBytes + r16 * 2048), desc(pb + r16 * 2048), idesc,
-                                              (i != i0 || piece != Cfg::kPieces - 1 || r16 != 0) ? 1u : 0u);
-                        umma_commit_pair(empty_bar(stage));
-                        umma_commit_pair(map_to_rank(empty_bar(stage), 1));
+                    for (int h = 0; h < 2; h++) {
+                        const int64_t row = r0 + h * 32 + lane;
+                        const bool here = row < prm.rows && k0 < prm.k;
+                        mx_copy_word(scale_base + (uint32_t)(slot * MX_ROWS + h * 32 + lane) * 4u, here ? prm.scales + row * prm.scale_pitch + (k0 >> 5) : prm.scales, here ? 4 : 0);
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full_bar(slot)) : "memory");
+                    armed = armed < (1 << 30) ? armed + 1 : armed;
+                    if (++slot == R) { slot = 0; phase ^= 1u; }
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (lane == 0 && (!ok || *abort_flag)) for (int i = armed > R ? armed - R : 0; i < armed; i++) mx_wait_landed(raw_full_bar(i % R), (uint32_t)(i / R) & 1u);
+        } else if (warp == 3) {
+            if (DIRECT && lane == 0) {
+                int stage = 0; uint32_t phase = 0;
+                int armed = 0;
+                bool ok = true;
+                for (int unit = pair; unit < units && ok; unit += pairs) {
+                    int n0, k0;
+                    tile_of(unit, n0, k0);
+                    n0 += (int)rank * 128;
+                    const int count = stage_count(unit);
+                    for (int i = 0; i < count; i++) {
+                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                        const uint32_t leader_full = map_to_rank(full_bar(stage), 0), pa = smem_base + stage * Cfg::kStageBytes;
+                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kTileBytes);
+                        const int r0 = (first_stage(unit) + i) * MX_ROWS;
+                        tma_load_2d_pair(pa, &map_g, leader_full, n0, r0);
+                        tma_load_2d_pair(pa + MX_ROWS * 128, &map_g, leader_full, n0 + 64, r0);
+                        armed = armed < (1 << 30) ? armed + 1 : armed;
                         if (++stage == S) { stage = 0; phase ^= 1u; }
                     }
-                    if (ok) { umma_commit_pair(acc_full_bar(buf)); umma_commit_pair(map_to_rank(acc_full_bar(buf), 1)); }
                 }
+                // giving up: these barriers also wait for the workers, so this may take its whole tenth of a second
+                if ((!ok || *abort_flag) && rank == 0) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_WORKER));
-        const int worker = warp - 4, row_in_stage = worker * 8 + (lane & 7);
+        const int worker = warp - 4, row_in_stage = worker * 8 + (lane & 7), group = lane >> 3;
         const int quarter = warp & 3, half = worker >> 2;
         float sum[128];
-        int stage = 0; uint32_t phase = 0, chunk = 0;
+        uint32_t ahead[4][KIND == 0 ? 8 : 4];               // of g, without TMA
+        int stage = 0, slot = 0; uint32_t phase = 0, slot_phase = 0;
+        auto fetch_ahead = [&](int unit, int i) {
+            if constexpr (!TMA) {
+                int n0, k0;
+                tile_of(unit, n0, k0);
+                const int64_t row = (int64_t)(first_stage(unit) + i) * MX_ROWS + row_in_stage;
+                const bool here = row < prm.rows;
+                const T *p = (const T *)prm.g + (here ? row : 0) * prm.n;
+#pragma unroll
+                for (int j = 0; j < 4; j++) mx_fetch8<KIND>(p, n0 + (int)rank * 128 + (j * 4 + group) * 8, prm.n, here, ahead[j]);
+            }
+        };
         bool ok = true;
-        // the chunk that still waits in tensor memory: its unit (-1 none), whether it is the unit's first and last
-        int open_unit = -1; bool open_first = false, open_last = false;
-        auto tile_of = [&](int unit, int &n0, int &k0) {
-            const int tile = unit / prm.slices;
-            n0 = tile % prm.tiles_n * 256 + (int)rank * 128; k0 = tile / prm.tiles_n * 256;
-        };
-        auto promote = [&](uint32_t c) {
-            const int buf = c & 1;
-            ok = mx_warp_wait(acc_full_bar(buf), (c >> 1) & 1u, abort_flag, lane);
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
+        int unit = pair, i0 = 0, count = unit < units ? stage_count(unit) : 0;
+        int open_unit = -1; bool open_first = false, open_last = false;        // the chunk that still lies in tensor memory
+        if (unit < units) fetch_ahead(unit, 0);
+        // A chunk is handed over stage by stage; then the one before it, which the MMAs have finished meanwhile, is added up.
+        for (uint32_t chunk = 0; ok; chunk++) {
+            const bool more = unit < units;
+            const int this_unit = unit;
+            bool first = false, last = false;
+            if (more) {
+                const int i1 = i0 + Cfg::kChunk < count ? i0 + Cfg::kChunk : count;
+                first = i0 == 0; last = i1 == count;
+                for (int i = i0; i < i1; i++) {
+                    if (!mx_warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, lane) || !mx_warp_wait(raw_full_bar(slot), slot_phase, abort_flag, lane)) { ok = false; break; }
+                    const uint32_t dst = smem_base + stage * Cfg::kStageBytes, raw = raw_base + slot * Cfg::kRawBytes + row_in_stage * 128;
+                    const uint32_t twist = (uint32_t)(row_in_stage & 7);
+                    if constexpr (!DIRECT) {
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-                float t[16];
-                tmem_load16(taddr + (uint32_t)(q * 16), t);
+                        for (int j = 0; j < 4; j++) {
+                            if constexpr (RAW_G) {
+                                uint32_t u[KIND == 0 ? 8 : 4];
+                                const int c = j * 4 + group;        // chunk of eight columns: 16 or 32 bytes of the row
+                                if constexpr (KIND == 0) {
+                                    const uint32_t box = raw + (uint32_t)((c >> 2) * (MX_ROWS * 128)), q = (uint32_t)(c & 3) * 2u;
+                                    mx_read16(box + ((q ^ twist) << 4), u[0], u[1], u[2], u[3]);
+                                    mx_read16(box + (((q + 1u) ^ twist) << 4), u[KIND == 0 ? 4 : 0], u[KIND == 0 ? 5 : 1], u[KIND == 0 ? 6 : 2], u[KIND == 0 ? 7 : 3]);
+                                } else mx_read16(raw + (uint32_t)((c >> 3) * (MX_ROWS * 128)) + (((uint32_t)(c & 7) ^ twist) << 4), u[0], u[1], u[2], u[3]);
+                                mx_put_pieces<KIND>(dst, row_in_stage, c, u);
+                            } else mx_put_pieces<KIND>(dst, row_in_stage, j * 4 + group, ahead[j]);
+                        }
+                    }
+                    uint32_t byte;
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_base + (uint32_t)((slot * MX_ROWS + row_in_stage) * 4 + group)));
+                    const float scale = mx_scale_value(byte);
 #pragma unroll
-                for (int e = 0; e < 16; e++) sum[q * 16 + e] = open_first ? t[e] : __fadd_rn(sum[q * 16 + e], t[e]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(acc_empty_bar(buf), 0));
-            if (!open_last) return;
-            int n0, k0;
-            tile_of(open_unit, n0, k0);
-            const int n = n0 + quarter * 32 + lane, c0 = k0 + half * 128;
-            if (n >= prm.n) return;
-            float *out = prm.out + open_unit % prm.slices * prm.slice_floats + (int64_t)n * prm.k + c0;
-            const bool vec = (prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0;
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t x[4];
+                        mx_read16(raw + Cfg::kRawG + ((((uint32_t)group * 2u + h) ^ twist) << 4), x[0], x[1], x[2], x[3]);
 #pragma unroll
-            for (int q = 0; q < 32; q++) {
-                if (vec) { if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]); }
-                else {
+                        for (int q = 0; q < 2; q++) {
+                            uint32_t w[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) if (c0 + q * 4 + e < prm.k) out[q * 4 + e] = sum[q * 4 + e];
+                            for (int e = 0; e < 4; e++) {
+                                float a, b;
+                                mx_decode8x2(x[q * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
+                                w[e] = low_pack2<1>(a * scale, b * scale);
+                            }
+                            mx_store_chunk(dst + Cfg::kPieces * Cfg::kTileBytes, row_in_stage, group * 4 + h * 2 + q, w);
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) { mx_arrive_rank(full_bar(stage), 0); mbar_arrive(raw_empty_bar(slot)); }
+                    if (++stage == S) { stage = 0; phase ^= 1u; }
+                    if (++slot == R) { slot = 0; slot_phase ^= 1u; }
+                    if (i + 1 < count) fetch_ahead(unit, i + 1);
+                    else if (unit + pairs < units) fetch_ahead(unit + pairs, 0);
                 }
-            }
-        };
-        MxStageRegs<KIND> regs;
-        if (pair < units) {
-            int n0, k0;
-            tile_of(pair, n0, k0);
-            mx_fetch_stage<KIND, VEC>(prm, (int64_t)first_stage(pair) * MX_ROWS + row_in_stage, n0, k0 + (int)rank * 128, lane, regs);
-        }
-        for (int unit = pair; unit < units && ok; unit += pairs) {
-            int n0, k0;
-            tile_of(unit, n0, k0);
-            const int count = stage_count(unit);
-            for (int i = 0; i < count; i++) {
-                ok = mx_warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, lane);
                 if (!ok) break;
-                mx_put_stage<KIND>(smem_base + stage * Cfg::kStageBytes, row_in_stage, lane, regs);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_rank(full_bar(stage), 0));
-                if (++stage == S) { stage = 0; phase ^= 1u; }
-                // the next stage's rows, of this unit or the next one
-                if (i + 1 < count) mx_fetch_stage<KIND, VEC>(prm, (int64_t)(first_stage(unit) + i + 1) * MX_ROWS + row_in_stage, n0, k0 + (int)rank * 128, lane, regs);
-                else if (unit + pairs < units) {
-                    int n1, k1;
-                    tile_of(unit + pairs, n1, k1);
-                    mx_fetch_stage<KIND, VEC>(prm, (int64_t)first_stage(unit + pairs) * MX_ROWS + row_in_stage, n1, k1 + (int)rank * 128, lane, regs);
+                i0 = i1;
+                if (i0 == count) { unit += pairs; i0 = 0; count = unit < units ? stage_count(unit) : 0; }
+            }
+            if (open_unit >= 0) {
+                const uint32_t c = chunk - 1;
+                const int buf = c & 1;
+                ok = mx_warp_wait(acc_full_bar(buf), (c >> 1) & 1u, abort_flag, lane);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    float t[16];
+                    tmem_load16(taddr + (uint32_t)(q * 16), t);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sum[q * 16 + e] = open_first ? t[e] : __fadd_rn(sum[q * 16 + e], t[e]);
                 }
-                if ((i + 1) % Cfg::kChunk == 0 || i + 1 == count) {
-                    // a chunk has been handed over: the one before it is done, or nearly
-                    if (open_unit >= 0) { promote(chunk - 1); if (!ok) break; }
-                    open_unit = unit; open_first = i < Cfg::kChunk; open_last = i + 1 == count;
-                    chunk++;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mx_arrive_rank(acc_empty_bar(buf), 0);
+                if (open_last) {
+                    int n0, k0;
+                    tile_of(open_unit, n0, k0);
+                    const int n = n0 + (int)rank * 128 + quarter * 32 + lane, c0 = k0 + half * 128;
+                    float *out = prm.out + open_unit % prm.slices * prm.slice_floats + (int64_t)n * prm.k + c0;
+                    if (n < prm.n) {
+                        if ((prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0) {
+#pragma unroll
+                            for (int q = 0; q < 32; q++) if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 128; q++) if (c0 + q < prm.k) out[q] = sum[q];
+                        }
+                    }
                 }
             }
+            if (!more) break;
+            open_unit = this_unit; open_first = first; open_last = last;
         }
-        if (ok && open_unit >= 0) promote(chunk - 1);
     }
 
     tc_fence_before();
@@ -1388,25 +1461,42 @@ int64_t mx_weight_gradient_workspace(int64_t rows, int64_t n, int64_t k, int sm_
     return slices > 1 ? (int64_t)slices * n * k : 0;
 }
 
-template <int KIND, bool VEC>
+// Tensor map over [rows, cols] of elements of `bytes` bytes: boxes of 128 bytes x 64 rows, 128-byte swizzle.
+static bool make_row_map(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t pitch, CUtensorMapDataType type, int bytes) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(pitch * bytes)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), (cuuint32_t)MX_ROWS};
+    cuuint32_t elem[2] = {1, 1};
+    return fn(map, type, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KIND, bool TMA>
 static cudaError_t launch_mx_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
     using Cfg = MxGradConfig<KIND>;
+    using T = typename MxElement<KIND>::type;
+    CUtensorMap map_x, map_g;
+    if (!make_row_map(&map_x, prm.codes, prm.rows, prm.code_pitch, prm.code_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)) return cudaErrorInvalidValue;
+    map_g = map_x;              // unused without TMA
+    if (TMA && !make_row_map(&map_g, prm.g, prm.rows, prm.n, prm.n, KIND == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T))) return cudaErrorInvalidValue;
     cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, mx_weight_gradient_kernel<KIND, VEC>);
+    cudaError_t e = cudaFuncGetAttributes(&attr, mx_weight_gradient_kernel<KIND, TMA>);
     if (e != cudaSuccess) return e;
     // the register split draws on what the block was launched with
     if (attr.numRegs * 3 < MX_GRAD_REGS_LOW + 2 * MX_GRAD_REGS_WORKER) return cudaErrorLaunchOutOfResources;
-    e = cudaFuncSetAttribute(mx_weight_gradient_kernel<KIND, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    e = cudaFuncSetAttribute(mx_weight_gradient_kernel<KIND, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int units = prm.tiles_n * prm.tiles_k * prm.slices, pairs = sm_count / 2;
-    mx_weight_gradient_kernel<KIND, VEC><<<2 * (units < pairs ? units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(prm);
+    mx_weight_gradient_kernel<KIND, TMA><<<2 * (units < pairs ? units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_g, prm);
     return cudaGetLastError();
 }
 
 template <int KIND>
 static cudaError_t launch_mx_weight_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
     using T = typename MxElement<KIND>::type;
-    return (int64_t)prm.n % 8 == 0 && ((uintptr_t)prm.g & 15) == 0 ? launch_mx_gradient<KIND, true>(s, prm, sm_count) : launch_mx_gradient<KIND, false>(s, prm, sm_count);
+    return (int64_t)prm.n * sizeof(T) % 16 == 0 && ((uintptr_t)prm.g & 15) == 0 ? launch_mx_gradient<KIND, true>(s, prm, sm_count) : launch_mx_gradient<KIND, false>(s, prm, sm_count);
 }
 
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
