@@ -5,6 +5,7 @@
 #include "lowp.cuh"
 #include "tensor_core.cuh"
 
+#include <atomic>
 #include <cstdlib>
 
 namespace syn {
@@ -30,41 +31,58 @@ template <int KIND> __device__ __forceinline__ typename MxElement<KIND>::type mx
 // bytes of the wide tensor per thread and access, the block's largest magnitude by two shuffles.  A row has
 // `per_row` groups, counted over the padded scales (a multiple of 16), so a block never straddles two warps.
 // ------------------------------------------------------------------------------------------------
-struct MxRows {
-    int64_t rows, cols;
-    int64_t per_row, total;         // groups of 8 per row and in all
-    int narrow;                     // total < 2^32: 32-bit division
+// I: int64_t, or uint32_t where the groups of the whole tensor, and a step beyond them, can be counted with it.
+template <typename I> struct MxRows {
+    I rows, per_row, total;         // groups of 8 per row and in all
+    I whole, rest;                  // whole groups of a row, columns of the one that is left
+    I blocks;                       // blocks of a row that exist
+    I hop, hop_rows, hop_groups;    // groups from one step of a thread to its next: in all, in whole rows, and the rest
+    uint32_t code_pitch, scale_pitch;
 };
 
-inline MxRows mx_rows(int64_t rows, int64_t cols) {
-    MxRows r;
-    r.rows = rows; r.cols = cols;
-    r.per_row = mx_scale_bytes(cols) * 4; r.total = rows * r.per_row;
-    r.narrow = r.total < (1ll << 32);
+inline int mx_grid(int64_t total) {
+    const int64_t blocks = (total + MX_THREADS - 1) / MX_THREADS;
+    return (int)(blocks < 148 * 8 ? (blocks < 1 ? 1 : blocks) : 148 * 8);
+}
+template <typename I> inline MxRows<I> mx_rows(int64_t rows, int64_t cols, int format) {
+    const int64_t per_row = mx_scale_bytes(cols) * 4, hop = (int64_t)mx_grid(rows * per_row) * MX_THREADS;
+    MxRows<I> r;
+    r.rows = (I)rows; r.per_row = (I)per_row; r.total = (I)(rows * per_row);
+    r.whole = (I)(cols / 8); r.rest = (I)(cols % 8); r.blocks = (I)mx_blocks(cols);
+    r.hop = (I)hop; r.hop_rows = (I)(hop / per_row); r.hop_groups = (I)(hop % per_row);
+    // a single row never multiplies by its pitch
+    r.code_pitch = rows > 1 ? (uint32_t)mx_code_bytes(format, cols) : 0u; r.scale_pitch = rows > 1 ? (uint32_t)mx_scale_bytes(cols) : 0u;
     return r;
 }
+inline bool mx_narrow_rows(int64_t rows, int64_t cols) { return rows * mx_scale_bytes(cols) * 4 < (1ll << 31); }
 
-struct MxSpot { int64_t row, first; int count; };      // a group: its row, its first column, how many of its 8 columns exist
+// The groups of a thread, `hop` apart: one division at the start, additions afterwards.  Past the last group `count` is
+// 0; threads of a warp leave the loop together, since shuffles need all of them.
+template <typename I> struct MxSpot {
+    I g, row, group;                // the group's number, its row, its number in the row
+    __device__ __forceinline__ void start(const MxRows<I> &r) {
+        g = (I)blockIdx.x * MX_THREADS + threadIdx.x;
+        row = r.rows == 1 ? 0 : g / r.per_row;
+        group = g - row * r.per_row;
+    }
+    __device__ __forceinline__ void next(const MxRows<I> &r) {
+        g += r.hop;
+        row += r.hop_rows; group += r.hop_groups;
+        if (group >= r.per_row) { group -= r.per_row; row++; }
+    }
+    __device__ __forceinline__ bool in(const MxRows<I> &r) const { return (g & ~(I)31) < r.total; }
+    __device__ __forceinline__ int count(const MxRows<I> &r) const { return g >= r.total ? 0 : group < r.whole ? 8 : group == r.whole ? (int)r.rest : 0; }
+    // of this group's first element in rows `pitch` elements apart
+    __device__ __forceinline__ int64_t offset(int64_t pitch) const { return (int64_t)row * pitch + (int64_t)group * 8; }
+};
 
-__device__ __forceinline__ MxSpot mx_spot(const MxRows &r, int64_t g) {
-    MxSpot s;
-    if (g >= r.total) { s.row = 0; s.first = r.cols; s.count = 0; return s; }
-    if (r.rows == 1) s.row = 0;
-    else if (r.narrow) s.row = (uint32_t)g / (uint32_t)r.per_row;
-    else s.row = g / r.per_row;
-    s.first = (g - s.row * r.per_row) * 8;
-    const int64_t left = r.cols - s.first;
-    s.count = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    return s;
-}
-
-// Eight elements from 16-byte aligned memory.
+// Eight elements from memory aligned to their size (32 or 16 bytes).
 template <int KIND> __device__ __forceinline__ void mx_load8(const typename MxElement<KIND>::type *p, float (&v)[8]) {
     if constexpr (KIND == 0) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
     } else {
-        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(p));
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) { v[2 * i] = low_decode<KIND>((uint16_t)(u[i] & 0xffffu)); v[2 * i + 1] = low_decode<KIND>((uint16_t)(u[i] >> 16)); }
@@ -72,27 +90,41 @@ template <int KIND> __device__ __forceinline__ void mx_load8(const typename MxEl
 }
 template <int KIND> __device__ __forceinline__ void mx_store8(typename MxElement<KIND>::type *p, const float (&v)[8]) {
     if constexpr (KIND == 0) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
     } else {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = (uint32_t)low_encode<KIND>(v[2 * i]) | ((uint32_t)low_encode<KIND>(v[2 * i + 1]) << 16);
+        for (int i = 0; i < 4; i++) u[i] = low_pack2<KIND>(v[2 * i], v[2 * i + 1]);
+        float largest = 0.0f;           // NaN if any is
+#pragma unroll
+        for (int i = 0; i < 8; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(v[i])));
+        if (largest != largest) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] = low_canonical_nan2<KIND>(u[i]);
+        }
         *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
     }
 }
 
-// Rows that do not start on 16 bytes: the warp reads (writes) its 256 elements 32 consecutive ones at a time and
+// Rows that do not start on such an address: the warp reads (writes) its 256 elements 32 consecutive ones at a time and
 // hands them over through its part of shared memory; a thread per group would touch every line eight times.
-// `offset`: element offset of this lane's group, `step`: distance of consecutive columns.
+// `offset`: element offset of this lane's group, `step`: distance of consecutive columns.  Where the warp's groups
+// follow one another in memory (one row, or dense rows without a gap between them) the first one's offset serves all.
 template <int KIND> __device__ __forceinline__ void mx_gather8(const typename MxElement<KIND>::type *p, int64_t offset, int64_t step, int count,
                                                                 float *box, int lane, float (&v)[8]) {
+    const int64_t base = __shfl_sync(0xffffffffu, offset, 0);
+    if (__all_sync(0xffffffffu, offset == base + lane * 8 * step && count == 8)) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int owner = i * 4 + (lane >> 3);
-        const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
-        const int have = __shfl_sync(0xffffffffu, count, owner);
-        box[i * 32 + lane] = (lane & 7) < have ? mx_load<KIND>(p + at + (lane & 7) * step) : 0.0f;
+        for (int i = 0; i < 8; i++) box[i * 32 + lane] = mx_load<KIND>(p + base + (i * 32 + lane) * step);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int owner = i * 4 + (lane >> 3);
+            const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
+            const int have = __shfl_sync(0xffffffffu, count, owner);
+            box[i * 32 + lane] = (lane & 7) < have ? mx_load<KIND>(p + at + (lane & 7) * step) : 0.0f;
+        }
     }
     __syncwarp();
     const float4 a = *reinterpret_cast<const float4 *>(box + lane * 8), b = *reinterpret_cast<const float4 *>(box + lane * 8 + 4);
@@ -103,12 +135,18 @@ template <int KIND> __device__ __forceinline__ void mx_scatter8(typename MxEleme
     *reinterpret_cast<float4 *>(box + lane * 8) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4 *>(box + lane * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
     __syncwarp();
+    const int64_t base = __shfl_sync(0xffffffffu, offset, 0);
+    if (__all_sync(0xffffffffu, offset == base + lane * 8 && count == 8)) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int owner = i * 4 + (lane >> 3);
-        const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
-        const int have = __shfl_sync(0xffffffffu, count, owner);
-        if ((lane & 7) < have) p[at + (lane & 7)] = mx_narrow<KIND>(box[i * 32 + lane]);
+        for (int i = 0; i < 8; i++) p[base + i * 32 + lane] = mx_narrow<KIND>(box[i * 32 + lane]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int owner = i * 4 + (lane >> 3);
+            const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
+            const int have = __shfl_sync(0xffffffffu, count, owner);
+            if ((lane & 7) < have) p[at + (lane & 7)] = mx_narrow<KIND>(box[i * 32 + lane]);
+        }
     }
     __syncwarp();
 }
@@ -174,56 +212,68 @@ __global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_
     }
 }
 
-// x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.
-template <int FORMAT, int KIND, bool VEC>
-__global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows r, int64_t row_step, int even,
-                                                                 uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles) {
+// x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.  Positions in 32 bits
+// where they fit: with 64-bit ones the 16-bit types were bound by the instructions of their addresses.
+template <int FORMAT, int KIND, bool VEC, typename I>
+__global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows<I> r, int64_t row_step, int even,
+                                                                 uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles, uint32_t atoms) {
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
     const int lane = threadIdx.x & 31;
-    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK * FORMAT / 8, scale_pitch = r.per_row / 4;
-    // the bound is a multiple of 32, so that whole warps take part in the shuffles
-    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
-        const MxSpot at = mx_spot(r, g);
-        float v[8];
-        int64_t base = at.row * row_step;
-        if (!VEC && !even) {
-            const int64_t r2 = at.row % ix.shape[2], rest = at.row / ix.shape[2];
-            base = r2 * ix.sa[2] + rest % ix.shape[1] * ix.sa[1] + rest / ix.shape[1] * ix.sa[0];
-        }
+    MxSpot<I> at;
+    auto fetch = [&](float (&v)[8]) {
+        const int count = at.count(r);
         if constexpr (VEC) {
-            if (at.count == 8) mx_load8<KIND>(x + base + at.first, v);
+            const auto *p = x + at.offset(row_step);
+            if (count == 8) mx_load8<KIND>(p, v);
             else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = i < at.count ? mx_load<KIND>(x + base + at.first + i) : 0.0f;
+                for (int i = 0; i < 8; i++) v[i] = i < count ? mx_load<KIND>(p + i) : 0.0f;
             }
         } else {
-            mx_gather8<KIND>(x, base + at.first * ix.sa[3], ix.sa[3], at.count, boxes[threadIdx.x >> 5], lane, v);
+            int64_t base = (int64_t)at.row * row_step;
+            if (!even) {
+                const int64_t row = count ? (int64_t)at.row : 0, r2 = row % ix.shape[2], rest = row / ix.shape[2];
+                base = r2 * ix.sa[2] + rest % ix.shape[1] * ix.sa[1] + rest / ix.shape[1] * ix.sa[0];
+            }
+            mx_gather8<KIND>(x, base + (int64_t)at.group * 8 * ix.sa[3], ix.sa[3], count, boxes[threadIdx.x >> 5], lane, v);
         }
-        uint32_t largest = 0;       // bit patterns of magnitudes order like the magnitudes, NaN above infinity
+    };
+    float ahead[8];
+    at.start(r);
+    if (at.in(r)) fetch(ahead);
+    while (at.in(r)) {
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) largest = max(largest, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; i++) v[i] = ahead[i];
+        const I row = at.row, group = at.group;
+        const bool mine = at.g < r.total;
+        at.next(r);
+        if (at.in(r)) fetch(ahead);         // in flight while this group is worked on
+        float most = 0.0f;                  // NaN if any is
+#pragma unroll
+        for (int i = 0; i < 8; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[i])));
+        uint32_t largest = __float_as_uint(most);       // bit patterns of magnitudes order like the magnitudes, NaN above infinity
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        if (g >= r.total) continue;
-        const int64_t group = at.first >> 3;
-        const bool exists = (at.first & ~(int64_t)(MX_BLOCK - 1)) < r.cols;     // else: padding of the scales
+        if (!mine) continue;
+        const I block = group >> 2;
+        const bool exists = block < r.blocks;       // else: padding of the scales
         const uint32_t byte = exists ? mx_scale_byte<FORMAT>(largest) : 0u;
         if ((lane & 3) == 0) {
-            scales[at.row * scale_pitch + (group >> 2)] = (uint8_t)byte;
-            if (tiles) tiles[mx_tile_offset(at.row, group >> 2, mx_tile_atoms(r.cols))] = (uint8_t)byte;
+            scales[(int64_t)row * r.scale_pitch + block] = (uint8_t)byte;
+            if (tiles) tiles[mx_tile_offset(row, block, atoms)] = (uint8_t)byte;
         }
         if (!exists) continue;
-        // the inverse scale 2^(127 - byte) is a normal number for every byte that occurs; a product with it is
-        // exact, or below half the smallest element
-        const float inverse = __uint_as_float((254u - byte) << 23);
         if (byte == 255u) {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] = 0.0f;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] *= inverse;
         }
-        uint8_t *dst = codes + at.row * code_pitch + group * FORMAT;
+        // the inverse scale 2^(127 - byte) is a normal number for every other byte that occurs; a product with it is
+        // exact, or below half the smallest element
+        const float inverse = byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= inverse;
+        uint8_t *dst = codes + (int64_t)row * r.code_pitch + (int64_t)group * FORMAT;
         if constexpr (FORMAT == 4) {
             *reinterpret_cast<uint32_t *>(dst) = mx_encode4x2(v[0], v[1]) | mx_encode4x2(v[2], v[3]) << 8 | mx_encode4x2(v[4], v[5]) << 16 | mx_encode4x2(v[6], v[7]) << 24;
         } else {
@@ -233,97 +283,129 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
 }
 
 // The eight values of a group; the caller has checked that its block exists.
-template <int FORMAT> __device__ __forceinline__ void mx_values8(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t code_pitch,
-                                                                 int64_t scale_pitch, const MxSpot &at, float (&v)[8]) {
-    const int64_t group = at.first >> 3;
-    const float scale = mx_scale_value(scales[at.row * scale_pitch + (group >> 2)]);
-    const uint8_t *src = codes + at.row * code_pitch + group * FORMAT;
+template <int FORMAT> struct MxHeld { uint32_t w[FORMAT / 4]; uint32_t byte; };
+template <int FORMAT, typename I> __device__ __forceinline__ void mx_fetch_held(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, const MxRows<I> &r,
+                                                                                const MxSpot<I> &at, MxHeld<FORMAT> &h) {
+    h.byte = __ldg(scales + (int64_t)at.row * r.scale_pitch + (at.group >> 2));
+    const uint8_t *src = codes + (int64_t)at.row * r.code_pitch + (int64_t)at.group * FORMAT;
+    if constexpr (FORMAT == 4) h.w[0] = __ldg(reinterpret_cast<const uint32_t *>(src));
+    else { const uint2 w = __ldg(reinterpret_cast<const uint2 *>(src)); h.w[0] = w.x; h.w[1] = w.y; }
+}
+template <int FORMAT> __device__ __forceinline__ void mx_values8(const MxHeld<FORMAT> &h, float (&v)[8]) {
+    const float scale = mx_scale_value(h.byte);
     if constexpr (FORMAT == 4) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(src);
 #pragma unroll
-        for (int i = 0; i < 4; i++) mx_decode4x2(w >> (8 * i) & 0xffu, v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; i++) mx_decode4x2(h.w[0] >> (8 * i) & 0xffu, v[2 * i], v[2 * i + 1]);
     } else {
-        const uint2 w = *reinterpret_cast<const uint2 *>(src);
-        mx_decode8x2(w.x & 0xffffu, v[0], v[1]); mx_decode8x2(w.x >> 16, v[2], v[3]);
-        mx_decode8x2(w.y & 0xffffu, v[4], v[5]); mx_decode8x2(w.y >> 16, v[6], v[7]);
+        mx_decode8x2(h.w[0] & 0xffffu, v[0], v[1]); mx_decode8x2(h.w[0] >> 16, v[2], v[3]);
+        mx_decode8x2(h.w[1] & 0xffffu, v[4], v[5]); mx_decode8x2(h.w[1] >> 16, v[6], v[7]);
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] *= scale;
 }
 
-template <int FORMAT, int KIND, bool VEC>
-__global__ void __launch_bounds__(MX_THREADS) mx_restore_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxRows r,
+template <int FORMAT, int KIND, bool VEC, typename I>
+__global__ void __launch_bounds__(MX_THREADS) mx_restore_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, MxRows<I> r, int64_t cols,
                                                                 typename MxElement<KIND>::type *__restrict__ out) {
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
-    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK * FORMAT / 8, scale_pitch = r.per_row / 4;
-    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
-        const MxSpot at = mx_spot(r, g);
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (at.count > 0) mx_values8<FORMAT>(codes, scales, code_pitch, scale_pitch, at, v);
-        const int64_t offset = at.row * r.cols + at.first;
-        if constexpr (VEC) { if (at.count) mx_store8<KIND>(out + offset, v); }      // rows are whole groups here
-        else mx_scatter8<KIND>(out, offset, at.count, boxes[threadIdx.x >> 5], threadIdx.x & 31, v);
+    MxSpot<I> at;
+    MxHeld<FORMAT> ahead = {};
+    at.start(r);
+    if (at.count(r)) mx_fetch_held<FORMAT>(codes, scales, r, at, ahead);
+    while (at.in(r)) {
+        const MxHeld<FORMAT> held = ahead;
+        const int count = at.count(r);
+        const int64_t offset = at.offset(cols);
+        at.next(r);
+        if (at.count(r)) mx_fetch_held<FORMAT>(codes, scales, r, at, ahead);
+        float v[8];
+        mx_values8<FORMAT>(held, v);
+        if constexpr (VEC) { if (count) mx_store8<KIND>(out + offset, v); }      // rows are whole groups here
+        else mx_scatter8<KIND>(out, offset, count, boxes[threadIdx.x >> 5], threadIdx.x & 31, v);
     }
 }
 
-// act'(z) in FLOAT32.  exp(-|z|) keeps every form free of overflow and of cancellation against 1.  Where |z| is
-// above 120 the exponentials are below the smallest number and the slope is 0 or 1 (an infinity, which a scale near
-// the end of its range can make of a finite value, included); NaN stays NaN.
-__device__ __forceinline__ float mx_slope(int act, float z) {
-    if (z != z) return z;
-    if (act == (int)Op::RELU || fabsf(z) > 120.0f) {
-        if (act == (int)Op::TANH || act == (int)Op::SIGMOID) return 0.0f;
-        return z > 0.0f ? 1.0f : 0.0f;
+// exp(-x) for x >= 0: the argument's rounding costs x 2^-24 of a result of exp(-x), less than 2^-25 of 1.
+__device__ __forceinline__ float mx_exp_minus(float x) { return __expf(-x); }
+
+// act'(z) in FLOAT32.  exp(-|z|) keeps every form free of overflow and of cancellation against 1.  Beyond 120 the
+// exponentials are below the smallest number and the slope is 0 or 1, so z (an infinity too, which a scale near the end
+// of its range can make of a finite value) is brought to that range first; NaN stays NaN.
+template <Op ACT> __device__ __forceinline__ float mx_slope(float z) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(-120.0f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(120.0f));
+    if constexpr (ACT == Op::TANH) {
+        const float e = mx_exp_minus(2.0f * fabsf(z)), d = 1.0f + e;
+        return __fdividef(4.0f * e, d * d);
+    } else if constexpr (ACT == Op::SIGMOID) {
+        const float e = mx_exp_minus(fabsf(z)), d = 1.0f + e;
+        return __fdividef(e, d * d);
+    } else if constexpr (ACT == Op::SILU) {
+        const float e = mx_exp_minus(fabsf(z)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
+        const float s = z >= 0.0f ? near : far, t = z >= 0.0f ? far : near;      // sigmoid(z) and 1 - sigmoid(z)
+        return s * fmaf(z, t, 1.0f);
+    } else if constexpr (ACT == Op::GELU_TANH) {    // z sigmoid(2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
+        const float c = 1.5957691216057308f, zz = z * z;
+        const float u = c * z * fmaf(0.044715f, zz, 1.0f);
+        const float e = mx_exp_minus(fabsf(u)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
+        return fmaf(z * (near * far), c * fmaf(0.134145f, zz, 1.0f), u >= 0.0f ? near : far);
+    } else {                                        // GELU: Phi(z) + z phi(z)
+        // Phi(-|z|) = exp(-z^2 / 2) / 2 * (a1 t + .. + a5 t^5), t = 1 / (1 + p |z| / sqrt 2), within 8e-8 (Abramowitz and
+        // Stegun, Handbook of Mathematical Functions, 7.1.26); shares its exponential with the density
+        const float e = mx_exp_minus(0.5f * z * z), t = __fdividef(1.0f, fmaf(0.23164190f, fabsf(z), 1.0f));
+        const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float tail = 0.5f * e * q;
+        return fmaf(0.3989422804014327f * z, e, z >= 0.0f ? 1.0f - tail : tail);
     }
-    switch ((Op)act) {
-        case Op::TANH: { const float e = expf(-2.0f * fabsf(z)), d = 1.0f + e; return __fdividef(4.0f * e, d * d); }
-        case Op::SIGMOID: { const float e = expf(-fabsf(z)), d = 1.0f + e; return __fdividef(e, d * d); }
-        case Op::SILU: {
-            const float e = expf(-fabsf(z)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
-            const float s = z >= 0.0f ? near : far, t = z >= 0.0f ? far : near;      // sigmoid(z) and 1 - sigmoid(z)
-            return s * fmaf(z, t, 1.0f);
-        }
-        case Op::GELU_TANH: {       // z sigmoid(2u), u = sqrt(2 / pi) (z + 0.044715 z^3)
-            const float c = 1.5957691216057308f, zz = z * z;
-            const float u = c * z * fmaf(0.044715f, zz, 1.0f);
-            const float e = expf(-fabsf(u)), near = __fdividef(1.0f, 1.0f + e), far = e * near;
-            const float s = u >= 0.0f ? near : far;
-            return fmaf(z * (near * far), c * fmaf(0.134145f, zz, 1.0f), s);
-        }
-        default:                    // GELU: Phi(z) + z phi(z)
-            return fmaf(0.3989422804014327f * z, expf(-0.5f * z * z), 0.5f * erfcf(-0.7071067811865476f * z));
+}
+template <Op ACT> __device__ __forceinline__ void mx_slopes(float (&z)[8], const float (&up)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (ACT == Op::RELU) z[i] = z[i] > 0.0f ? up[i] : z[i] != z[i] ? z[i] : 0.0f;
+        else z[i] = up[i] * mx_slope<ACT>(z[i]);
     }
 }
 
 // dz = g * act'(z).  A closed ReLU gate gives 0 whatever g holds, like the WHERE of the ordinary gradient rule; a
 // block of NaN gives NaN, so that a step over it is refused rather than taken without its gradient.
-template <int KIND, bool VEC>
+template <int KIND, bool VEC, typename I>
 __global__ void __launch_bounds__(MX_THREADS) mx_activation_gradient_kernel(int act, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                                                                            const typename MxElement<KIND>::type *__restrict__ g_in, MxRows r,
+                                                                            const typename MxElement<KIND>::type *__restrict__ g_in, MxRows<I> r, int64_t cols,
                                                                             typename MxElement<KIND>::type *__restrict__ out) {
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
     const int lane = threadIdx.x & 31;
-    const int64_t code_pitch = mx_blocks(r.cols) * MX_BLOCK, scale_pitch = r.per_row / 4;
-    for (int64_t g = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; g < ((r.total + 31) & ~(int64_t)31); g += (int64_t)gridDim.x * MX_THREADS) {
-        const MxSpot at = mx_spot(r, g);
-        const int64_t offset = at.row * r.cols + at.first;
-        float z[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, up[8];
-        if constexpr (VEC) { if (at.count) mx_load8<KIND>(g_in + offset, up); }
-        else mx_gather8<KIND>(g_in, offset, 1, at.count, boxes[threadIdx.x >> 5], lane, up);
-        if (at.count > 0) mx_values8<8>(codes, scales, code_pitch, scale_pitch, at, z);
+    MxSpot<I> at;
+    MxHeld<8> held_ahead = {};
+    float up_ahead[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    auto fetch = [&]() {
+        const int count = at.count(r);
+        if (count) mx_fetch_held<8>(codes, scales, r, at, held_ahead);
+        if constexpr (VEC) { if (count) mx_load8<KIND>(g_in + at.offset(cols), up_ahead); }
+        else mx_gather8<KIND>(g_in, at.offset(cols), 1, count, boxes[threadIdx.x >> 5], lane, up_ahead);
+    };
+    at.start(r);
+    if (at.in(r)) fetch();
+    while (at.in(r)) {
+        const MxHeld<8> held = held_ahead;
+        float up[8], z[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (act == (int)Op::RELU) z[i] = z[i] > 0.0f ? up[i] : z[i] != z[i] ? z[i] : 0.0f;
-            else z[i] = up[i] * mx_slope(act, z[i]);
+        for (int i = 0; i < 8; i++) up[i] = up_ahead[i];
+        const int count = at.count(r);
+        const int64_t offset = at.offset(cols);
+        at.next(r);
+        if (at.in(r)) fetch();
+        mx_values8<8>(held, z);
+        switch ((Op)act) {
+            case Op::RELU: mx_slopes<Op::RELU>(z, up); break;
+            case Op::TANH: mx_slopes<Op::TANH>(z, up); break;
+            case Op::SIGMOID: mx_slopes<Op::SIGMOID>(z, up); break;
+            case Op::SILU: mx_slopes<Op::SILU>(z, up); break;
+            case Op::GELU_TANH: mx_slopes<Op::GELU_TANH>(z, up); break;
+            default: mx_slopes<Op::GELU>(z, up); break;
         }
-        if constexpr (VEC) { if (at.count) mx_store8<KIND>(out + offset, z); }
-        else mx_scatter8<KIND>(out, offset, at.count, boxes[threadIdx.x >> 5], lane, z);
+        if constexpr (VEC) { if (count) mx_store8<KIND>(out + offset, z); }
+        else mx_scatter8<KIND>(out, offset, count, boxes[threadIdx.x >> 5], lane, z);
     }
-}
-
-int mx_grid(const MxRows &r) {
-    const int64_t blocks = (r.total + MX_THREADS - 1) / MX_THREADS;
-    return (int)(blocks < 148 * 8 ? (blocks < 1 ? 1 : blocks) : 148 * 8);
 }
 
 // Activations of a FLOAT32 sum before its one rounding, from exp(-|z|) like the slopes above; below -120 SILU and
@@ -376,9 +458,8 @@ template <int PAIR> __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t 
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate) : "memory");
 }
-template <int PAIR> __device__ __forceinline__ void mx_copy_atom(uint32_t taddr, uint32_t smem_addr) {
-    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
+__device__ __forceinline__ void mx_copy_atom(uint32_t taddr, uint32_t smem_addr) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(mx_scale_desc(smem_addr)) : "memory");
 }
 // Four bytes global -> shared, the part past `bytes` (0 to 4) zero.
 __device__ __forceinline__ void mx_copy_word(uint32_t dst, const uint8_t *src, int bytes) {
@@ -408,7 +489,16 @@ __device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && global_timer() - start < 100000000ull) { }
 }
 
-// One lane waits for the warp.
+// 24 columns of tensor memory, this warp's 32 lanes.
+__device__ __forceinline__ void tmem_store24(uint32_t taddr, const uint4 (&v)[6]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w),
+                   "r"(v[2].x), "r"(v[2].y), "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr + 16u), "r"(v[4].x), "r"(v[4].y), "r"(v[4].z), "r"(v[4].w), "r"(v[5].x), "r"(v[5].y), "r"(v[5].z), "r"(v[5].w) : "memory");
+}
+
+// One lane waits for the warp: 32 lanes that poll a barrier take issue slots from the rest of the block.
 __device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int lane) {
     if (lane == 0) mbar_wait_cluster(bar, parity, abort_flag);
     __syncwarp();
@@ -508,7 +598,7 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
                 const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes, ps = scale_base + stage * Cfg::kScaleBytes;
                 const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
 #pragma unroll
-                for (int i = 0; i < 4; i++) mx_copy_atom<0>(ts + i * 4, ps + i * MX_ATOM);
+                for (int i = 0; i < 4; i++) mx_copy_atom(ts + i * 4, ps + i * MX_ATOM);
 #pragma unroll
                 for (int k4 = 0; k4 < 4; k4++)
                     mx_mma<0>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 4,
@@ -592,24 +682,30 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
 
 // ---- many rows: two-SM tiles of 256 x 256 -----------------------------------------------------------
 // A cluster of two blocks per tile (cta_group::2, M = 256): each loads its 128 rows of x, half of the tile's 256
-// rows of W, and the scales of its rows of x and of all of W's (tensor memory of both blocks needs those), in tiles
-// that TMA can fetch: gathering them word by word from rows took three quarters of the time.  A
-// one-SM block would move (128 + 256) x 128 bytes of codes into shared memory and the tensor core read them out again
-// within 512 clocks of MMA, more than shared memory delivers; the pair moves a third less.  Accumulators take 256
-// columns of tensor memory and the scales of the stages in flight most of the rest, so there is one accumulator: the
+// rows of W; the scales of its rows of x and of all of W's go into its tensor memory.  A one-SM block would move
+// (128 + 256) x 128 bytes of codes into shared memory and the tensor core read them out again within 512 clocks of
+// MMA, more than shared memory delivers; the pair moves a third less.  Accumulators take 256 columns of tensor memory and the scales of the stages in flight most of the rest, so there is one accumulator: the
 // epilogue warps first copy it to registers, hand it back, and finish the tile under the next one's main loop.
+// Scales: TMA fetches their tiles into a ring of their own, further ahead than the codes, and four warps move them on
+// to tensor memory through registers as soon as a stage's columns are free, so they lie there before the codes land.
+// tcgen05.cp from shared memory shares the tensor pipe with the MMAs: its six copies per k-block cost 60 of 334 us on
+// 37888 x 4096 x 4096.  Gathering the words from rows instead of tiles cost three times the main loop.
 struct MxPairConfig {
     static constexpr int BN = 256;
     static constexpr int kStages = 5;
     static constexpr int kABytes = 128 * 128, kBBytes = 128 * 128;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kScaleBytes = 6 * MX_ATOM;             // two atoms of x's rows, two of each half of W's
-    static constexpr int kScaleCols = 24;
+    static constexpr int kScaleSlots = 8;
+    static constexpr int kScaleCols = 24;                       // of a stage: two atoms of x, two of each half of W
     static constexpr int kTmemCols = 512;
     static constexpr int kStagingBytes = 8 * 4096;
-    static constexpr int kSmemBytes = kStages * (kStageBytes + kScaleBytes) + kStagingBytes + 1024 + 256;
+    static constexpr int kSmemBytes = kStages * kStageBytes + kScaleSlots * kScaleBytes + kStagingBytes + 1024 + 512;
 };
-constexpr int MX_PAIR_THREADS = 384;    // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue
+constexpr int MX_PAIR_THREADS = 512;    // warp 0 TMA of codes, warp 1 MMA, warp 2 TMA of scales, warps 4-7 scales, warps 8-15 epilogue
+// Registers per thread of the three groups after the split; their sum over the four warpgroups is at most the 512 of
+// the launch.
+constexpr int MX_PAIR_REGS_LOW = 40, MX_PAIR_REGS_SCALES = 64, MX_PAIR_REGS_EPILOGUE = 200;
 
 // One warp's 32 rows x 128 columns: bias, activation, one rounding, then boxes of 32 rows x 128 bytes through
 // shared memory (16-byte chunk j of row r at chunk j ^ (r & 7), the 128-byte swizzle) and out by TMA, which clips the
@@ -694,23 +790,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
         const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws, MxLinear prm) {
     using Cfg = MxPairConfig;
     using T = typename MxElement<KIND>::type;
-    constexpr int S = Cfg::kStages, BN = Cfg::BN;
+    constexpr int S = Cfg::kStages, R = Cfg::kScaleSlots, BN = Cfg::BN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * (Cfg::kStageBytes + Cfg::kScaleBytes) + Cfg::kStagingBytes);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 2);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes + R * Cfg::kScaleBytes + Cfg::kStagingBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 2 * R + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem);
     const uint32_t staging_base = smem_base + S * Cfg::kStageBytes, scale_base = staging_base + Cfg::kStagingBytes;
-    // full and accumulator-empty barriers are those of the even block; empty and accumulator-full are each block's own
+    // full (codes), scale (scales in tensor memory) and accumulator-empty barriers are those of the even block; empty,
+    // fetched and taken (scales in shared memory) and accumulator-full are each block's own
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
-    const uint32_t acc_full_bar = bar_base + 8u * (2 * S), acc_empty_bar = bar_base + 8u * (2 * S + 1);
+    auto scale_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };
+    auto fetched_bar = [&](int i) { return bar_base + 8u * (3 * S + i); };
+    auto taken_bar = [&](int i) { return bar_base + 8u * (3 * S + R + i); };
+    const uint32_t acc_full_bar = bar_base + 8u * (3 * S + 2 * R), acc_empty_bar = bar_base + 8u * (3 * S + 2 * R + 1);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), 8); }
+        for (int i = 0; i < R; i++) { mbar_init(fetched_bar(i), 1); mbar_init(taken_bar(i), 4); }
         mbar_init(acc_full_bar, 1); mbar_init(acc_empty_bar, 512);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -729,7 +830,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_PAIR_REGS_LOW));
         if (warp == 0) {
             if (lane == 0) {
                 int stage = 0; uint32_t phase = 0;
@@ -740,22 +841,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                     tile_origin(tile, prm.tiles_m, prm.tiles_n, prm.group_n, mi, ni);
                     const int m0 = mi * 256 + (int)rank * 128, n0 = ni * BN + (int)rank * 128;
                     for (int kb = 0; kb < kb_count; kb++) {
-                        if (!mbar_wait_cluster(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
                         const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
                         const uint32_t leader_full = map_to_rank(full_bar(stage), 0);
-                        const uint32_t ss = scale_base + stage * Cfg::kScaleBytes;
-                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * (Cfg::kStageBytes + Cfg::kScaleBytes));
+                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kStageBytes);
                         tma_load_2d_pair(sa, &map_x, leader_full, kb * (MX_BK / 2), m0);
                         tma_load_2d_pair(sa + Cfg::kABytes, &map_w, leader_full, kb * (MX_BK / 2), n0);
-                        // two atoms, 256 words: always a multiple of 16 bytes
-                        tma_load_2d_pair(ss, &map_xs, leader_full, kb * 256, mi * 2 + (int)rank);
-                        tma_load_2d_pair(ss + 2 * MX_ATOM, &map_ws, leader_full, kb * 256, ni * 2);
                         armed = armed < (1 << 30) ? armed + 1 : armed;
                         if (++stage == S) { stage = 0; phase ^= 1u; }
                     }
                 }
                 // giving up: the even block waits for both blocks' copies in flight; the odd one cannot leave before it
                 if ((!ok || *abort_flag) && rank == 0) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
+            }
+        } else if (warp == 2) {
+            if (lane == 0) {
+                int slot = 0; uint32_t phase = 0;
+                int armed = 0;
+                bool ok = true;
+                for (int tile = pair; tile < total_tiles && ok; tile += pairs) {
+                    int mi, ni;
+                    tile_origin(tile, prm.tiles_m, prm.tiles_n, prm.group_n, mi, ni);
+                    for (int kb = 0; kb < kb_count; kb++) {
+                        if (!mbar_wait(taken_bar(slot), phase ^ 1u, abort_flag)) { ok = false; break; }
+                        // two atoms of every band, 256 words: always a multiple of 16 bytes; bands past the matrix read as zeros
+                        const uint32_t ss = scale_base + slot * Cfg::kScaleBytes;
+                        mbar_expect_tx(fetched_bar(slot), Cfg::kScaleBytes);
+                        tma_load_2d(ss, &map_xs, fetched_bar(slot), kb * 256, mi * 2 + (int)rank);
+                        tma_load_2d(ss + 2 * MX_ATOM, &map_ws, fetched_bar(slot), kb * 256, ni * 2);
+                        armed = armed < (1 << 30) ? armed + 1 : armed;
+                        if (++slot == R) { slot = 0; phase ^= 1u; }
+                    }
+                }
+                if (!ok || *abort_flag) for (int i = armed > R ? armed - R : 0; i < armed; i++) mx_wait_landed(fetched_bar(i % R), (uint32_t)(i / R) & 1u);
             }
         } else if (warp == 1) {
             if (rank == 0 && lane == 0) {
@@ -766,16 +884,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                     if (!mbar_wait_cluster(acc_empty_bar, (done & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
                     for (int kb = 0; kb < kb_count; kb++) {
-                        if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        if (!mbar_wait(scale_bar(stage), phase, abort_flag) || !mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
                         tc_fence_after();
-                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes, ps = scale_base + stage * Cfg::kScaleBytes;
+                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes;
                         const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            mx_copy_atom<1>(ts + i * 4, ps + i * MX_ATOM);
-                            mx_copy_atom<1>(ts + 8 + i * 8, ps + (2 + i) * MX_ATOM);
-                            mx_copy_atom<1>(ts + 12 + i * 8, ps + (4 + i) * MX_ATOM);
-                        }
 #pragma unroll
                         for (int k4 = 0; k4 < 4; k4++)
                             mx_mma<1>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 8,
@@ -788,9 +900,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                 }
             }
         }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_PAIR_REGS_SCALES));
+        // this warp's 32 lanes of tensor memory get the same words as the other three warps'
+        const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + BN;
+        int stage = 0, slot = 0; uint32_t phase = 0, slot_phase = 0;
+        bool ok = true;
+        for (int tile = pair; tile < total_tiles && ok; tile += pairs) {
+            for (int kb = 0; kb < kb_count; kb++) {
+                ok = mx_warp_wait(fetched_bar(slot), slot_phase, abort_flag, lane);
+                if (!ok) break;
+                const uint32_t ps = scale_base + slot * Cfg::kScaleBytes + lane * 16;
+                uint4 v[6];
+                // columns: x half 0, x half 1, W half 0 (both bands), W half 1; in shared memory W's bands come one after the other
+#pragma unroll
+                for (int i = 0; i < 6; i++) {
+                    const int atom = i < 2 ? i : 2 + ((i & 1) << 1) + ((i - 2) >> 1);
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w) : "r"(ps + (uint32_t)(atom * MX_ATOM)) : "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(taken_bar(slot));
+                if (++slot == R) { slot = 0; slot_phase ^= 1u; }
+                // the MMAs that read this stage's columns before have finished
+                ok = mx_warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, lane);
+                if (!ok) break;
+                tc_fence_after();
+                tmem_store24(taddr + (uint32_t)(stage * Cfg::kScaleCols), v);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mx_arrive_rank(scale_bar(stage), 0);
+                if (++stage == S) { stage = 0; phase ^= 1u; }
+            }
+        }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_PAIR_REGS_EPILOGUE));
+        const int quarter = warp & 3, half = (warp - 8) >> 2;
         uint32_t done = 0;
         for (int tile = pair; tile < total_tiles; tile += pairs, done++) {
             int mi, ni;
@@ -805,19 +950,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                 if (c + 2 < prm.n) bias_lane.z = mx_load<KIND>(b + c + 2);
                 if (c + 3 < prm.n) bias_lane.w = mx_load<KIND>(b + c + 3);
             }
-            if (!__all_sync(0xffffffffu, mbar_wait_cluster(acc_full_bar, done & 1u, abort_flag))) break;
+            if (!mx_warp_wait(acc_full_bar, done & 1u, abort_flag, lane)) break;
             tc_fence_after();
             float sum[128];
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                float t[16];
-                tmem_load16(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128 + c * 16), t);
+            for (int c = 0; c < 4; c++) {
+                float t[32];
+                tmem_load32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128 + c * 32), t);
 #pragma unroll
-                for (int i = 0; i < 16; i++) sum[c * 16 + i] = t[i];
+                for (int i = 0; i < 32; i++) sum[c * 32 + i] = t[i];
             }
             tc_fence_before();
             mx_arrive_rank(acc_empty_bar, 0);
-            mx_emit<KIND, GENERAL>(prm, &map_out, staging_base + (uint32_t)((warp - 4) * 4096), row0, col0, sum, bias_lane, lane);
+            mx_emit<KIND, GENERAL>(prm, &map_out, staging_base + (uint32_t)((warp - 8) * 4096), row0, col0, sum, bias_lane, lane);
         }
         staged_drain(lane);
     }
@@ -842,7 +987,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
 // takes three products at the BFLOAT16 rate where a split into TF32 numbers would take three at half of it.
 //   Both operands are contracted along their rows, that is, they are MN-major tiles (64 columns of one row = one
-// 128-byte swizzle row).  TMA brings the rows as they are into a ring of raw slots, eight worker warps per block convert
+// 128-byte swizzle row).  TMA brings the rows as they are into a ring of raw slots, sixteen worker warps per block convert
 // them into operand tiles of that form, so no converted copy of either matrix exists in memory; BFLOAT16 gradients need
 // no conversion and go into the operand tiles at once.  (Rows of g that TMA cannot address, widths that are no multiple
 // of 16 bytes, the workers read themselves, one stage ahead.)  Tensor memory adds with truncation, so it only holds partial sums
@@ -851,8 +996,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // a workspace and are added in ascending order by a second kernel.
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 64;             // rows per stage
-constexpr int MX_GRAD_THREADS = 384;    // warp 0 MMA, warp 2 raw slots, warp 3 gradients that need no conversion, warps 4-11 workers
-constexpr int MX_GRAD_REGS_LOW = 56, MX_GRAD_REGS_WORKER = 224;
+constexpr int MX_GRAD_THREADS = 640;    // warp 0 MMA, warp 2 raw slots, warp 3 gradients that need no conversion, warps 4-19 workers
+constexpr int MX_GRAD_REGS_LOW = 56, MX_GRAD_REGS_WORKER = 104;
 
 template <int KIND> struct MxGradConfig {
     static constexpr int kPieces = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
@@ -877,12 +1022,13 @@ struct MxGrad {
 };
 
 // Two floats as the next piece: the upper 16 bits of each (truncation keeps the remainder exact), which are taken off.
-__device__ __forceinline__ uint32_t mx_piece(float &a, float &b) {
+// At the first piece an infinity leaves no remainder (infinity - infinity would be NaN); a NaN leaves a NaN.
+template <bool FIRST> __device__ __forceinline__ uint32_t mx_piece(float &a, float &b) {
     const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
     const uint32_t word = __byte_perm(ua, ub, 0x7632);
-    // an infinity has no remainder (infinity - infinity would be NaN); a NaN leaves a NaN
-    a = fabsf(a) == __uint_as_float(0x7f800000u) ? 0.0f : __fsub_rn(a, __uint_as_float(ua & 0xffff0000u));
-    b = fabsf(b) == __uint_as_float(0x7f800000u) ? 0.0f : __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
+    const float ra = __fsub_rn(a, __uint_as_float(ua & 0xffff0000u)), rb = __fsub_rn(b, __uint_as_float(ub & 0xffff0000u));
+    a = FIRST && fabsf(a) == __uint_as_float(0x7f800000u) ? 0.0f : ra;
+    b = FIRST && fabsf(b) == __uint_as_float(0x7f800000u) ? 0.0f : rb;
     return word;
 }
 __device__ __forceinline__ void mx_store_chunk(uint32_t tile, int row, int chunk, const uint32_t (&w)[4]) {
@@ -918,7 +1064,7 @@ __device__ __forceinline__ void mx_put_pieces(uint32_t stage, int row, int chunk
         for (int piece = 0; piece < Cfg::kPieces; piece++) {
             uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = mx_piece(f[2 * e], f[2 * e + 1]);
+            for (int e = 0; e < 4; e++) w[e] = piece == 0 ? mx_piece<true>(f[2 * e], f[2 * e + 1]) : mx_piece<false>(f[2 * e], f[2 * e + 1]);
             mx_store_chunk(stage + piece * Cfg::kTileBytes, row, chunk, w);
         }
     }
@@ -954,9 +1100,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 * R + 2 + a); };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), DIRECT ? 17 : 16); mbar_init(empty_bar(s), 1); }
-        for (int i = 0; i < R; i++) { mbar_init(raw_full_bar(i), 33); mbar_init(raw_empty_bar(i), 8); }     // TMA and 32 lanes of scales
-        for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 16); }
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), DIRECT ? 33 : 32); mbar_init(empty_bar(s), 1); }
+        for (int i = 0; i < R; i++) { mbar_init(raw_full_bar(i), 33); mbar_init(raw_empty_bar(i), 16); }     // TMA and 32 lanes of scales
+        for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 32); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1083,10 +1229,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_WORKER));
-        const int worker = warp - 4, row_in_stage = worker * 8 + (lane & 7), group = lane >> 3;
-        const int quarter = warp & 3, half = worker >> 2;
-        float sum[128];
-        uint32_t ahead[4][KIND == 0 ? 8 : 4];               // of g, without TMA
+        // a warp converts 8 rows of one half of the columns, and adds up 32 x 64 results
+        const int worker = warp - 4, row_in_stage = (worker & 7) * 8 + (lane & 7), group = lane >> 3, side = worker >> 3;
+        const int quarter = warp & 3, part = worker >> 2;
+        float sum[64];
+        uint32_t ahead[2][KIND == 0 ? 8 : 4];               // of g, without TMA
         int stage = 0, slot = 0; uint32_t phase = 0, slot_phase = 0;
         auto fetch_ahead = [&](int unit, int i) {
             if constexpr (!TMA) {
@@ -1096,7 +1243,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 const bool here = row < prm.rows;
                 const T *p = (const T *)prm.g + (here ? row : 0) * prm.n;
 #pragma unroll
-                for (int j = 0; j < 4; j++) mx_fetch8<KIND>(p, n0 + (int)rank * 128 + (j * 4 + group) * 8, prm.n, here, ahead[j]);
+                for (int j = 0; j < 2; j++) mx_fetch8<KIND>(p, n0 + (int)rank * 128 + (side * 8 + j * 4 + group) * 8, prm.n, here, ahead[j]);
             }
         };
         bool ok = true;
@@ -1117,37 +1264,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                     const uint32_t twist = (uint32_t)(row_in_stage & 7);
                     if constexpr (!DIRECT) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
+                        for (int j = 0; j < 2; j++) {
+                            const int c = side * 8 + j * 4 + group;
                             if constexpr (RAW_G) {
-                                uint32_t u[KIND == 0 ? 8 : 4];
-                                const int c = j * 4 + group;        // chunk of eight columns: 16 or 32 bytes of the row
+                                uint32_t u[KIND == 0 ? 8 : 4];      // chunk of eight columns: 16 or 32 bytes of the row
                                 if constexpr (KIND == 0) {
                                     const uint32_t box = raw + (uint32_t)((c >> 2) * (MX_ROWS * 128)), q = (uint32_t)(c & 3) * 2u;
                                     mx_read16(box + ((q ^ twist) << 4), u[0], u[1], u[2], u[3]);
                                     mx_read16(box + (((q + 1u) ^ twist) << 4), u[KIND == 0 ? 4 : 0], u[KIND == 0 ? 5 : 1], u[KIND == 0 ? 6 : 2], u[KIND == 0 ? 7 : 3]);
                                 } else mx_read16(raw + (uint32_t)((c >> 3) * (MX_ROWS * 128)) + (((uint32_t)(c & 7) ^ twist) << 4), u[0], u[1], u[2], u[3]);
                                 mx_put_pieces<KIND>(dst, row_in_stage, c, u);
-                            } else mx_put_pieces<KIND>(dst, row_in_stage, j * 4 + group, ahead[j]);
+                            } else mx_put_pieces<KIND>(dst, row_in_stage, c, ahead[j]);
                         }
                     }
-                    uint32_t byte;
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_base + (uint32_t)((slot * MX_ROWS + row_in_stage) * 4 + group)));
+                    // half a block of the checkpoint: 16 bytes
+                    const int c = side * 4 + group;
+                    uint32_t byte, x[4];
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_base + (uint32_t)((slot * MX_ROWS + row_in_stage) * 4 + (c >> 1))));
+                    mx_read16(raw + Cfg::kRawG + (((uint32_t)c ^ twist) << 4), x[0], x[1], x[2], x[3]);
                     const float scale = mx_scale_value(byte);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t x[4];
-                        mx_read16(raw + Cfg::kRawG + ((((uint32_t)group * 2u + h) ^ twist) << 4), x[0], x[1], x[2], x[3]);
+                    for (int q = 0; q < 2; q++) {
+                        uint32_t w[4];
 #pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                float a, b;
-                                mx_decode8x2(x[q * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
-                                w[e] = low_pack2<1>(a * scale, b * scale);
-                            }
-                            mx_store_chunk(dst + Cfg::kPieces * Cfg::kTileBytes, row_in_stage, group * 4 + h * 2 + q, w);
+                        for (int e = 0; e < 4; e++) {
+                            float a, b;
+                            mx_decode8x2(x[q * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
+                            w[e] = low_pack2<1>(a * scale, b * scale);
                         }
+                        mx_store_chunk(dst + Cfg::kPieces * Cfg::kTileBytes, row_in_stage, c * 2 + q, w);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -1167,9 +1312,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 ok = mx_warp_wait(acc_full_bar(buf), (c >> 1) & 1u, abort_flag, lane);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
+                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + part * 64);
 #pragma unroll
-                for (int q = 0; q < 8; q++) {
+                for (int q = 0; q < 4; q++) {
                     float t[16];
                     tmem_load16(taddr + (uint32_t)(q * 16), t);
 #pragma unroll
@@ -1181,15 +1326,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 if (open_last) {
                     int n0, k0;
                     tile_of(open_unit, n0, k0);
-                    const int n = n0 + (int)rank * 128 + quarter * 32 + lane, c0 = k0 + half * 128;
+                    const int n = n0 + (int)rank * 128 + quarter * 32 + lane, c0 = k0 + part * 64;
                     float *out = prm.out + open_unit % prm.slices * prm.slice_floats + (int64_t)n * prm.k + c0;
                     if (n < prm.n) {
                         if ((prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0) {
 #pragma unroll
-                            for (int q = 0; q < 32; q++) if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]);
+                            for (int q = 0; q < 16; q++) if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]);
                         } else {
 #pragma unroll
-                            for (int q = 0; q < 128; q++) if (c0 + q < prm.k) out[q] = sum[q];
+                            for (int q = 0; q < 64; q++) if (c0 + q < prm.k) out[q] = sum[q];
                         }
                     }
                 }
@@ -1234,6 +1379,24 @@ __global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(const float *
 
 }  // namespace
 
+// What a kernel needs once per device before its first launch: leave to use `smem` bytes of shared memory, and a look
+// at its registers per thread (those a register split at run time draws on).
+template <typename Kernel>
+static cudaError_t mx_prepare_kernel(Kernel kernel, int smem, int least_regs, std::atomic<uint64_t> &done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs < least_regs) return cudaErrorLaunchOutOfResources;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 #define MX_KINDS(dtype, CALL) ((dtype) == DType::F32 ? CALL(0) : (dtype) == DType::BF16 ? CALL(1) : (dtype) == DType::F16 ? CALL(2) : cudaErrorInvalidValue)
 
 template <int FORMAT, int KIND>
@@ -1250,12 +1413,20 @@ static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index
         else even &= ix.sa[d] == row_step * extent;
         extent *= ix.shape[d];
     }
-    const bool vec = even && (ix.sa[3] == 1 || cols == 1) && ((uintptr_t)x & 15) == 0 && (rows == 1 || row_step * (int64_t)sizeof(T) % 16 == 0);
+    const bool vec = even && (ix.sa[3] == 1 || cols == 1) && (uintptr_t)x % (8 * sizeof(T)) == 0 && (rows == 1 || row_step % 8 == 0);
     // dense rows of whole scale words are one long row
     const bool flat = vec && !tiles && row_step == cols && cols % (4 * MX_BLOCK) == 0;
-    const MxRows r = flat ? mx_rows(1, rows * cols) : mx_rows(rows, cols);
-    if (vec) mx_quantize_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, 1, codes, scales, tiles);
-    else mx_quantize_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>((const T *)x, ix, r, row_step, even, codes, scales, tiles);
+    const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
+    const int grid = mx_grid(r * mx_scale_bytes(c) * 4);
+    const uint32_t atoms = (uint32_t)mx_tile_atoms(cols);
+    const auto launch = [&](auto kernel, auto shape) { kernel<<<grid, MX_THREADS, 0, s>>>((const T *)x, ix, shape, row_step, even ? 1 : 0, codes, scales, tiles, atoms); };
+    if (mx_narrow_rows(r, c)) {
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
+        else launch(mx_quantize_kernel<FORMAT, KIND, false, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
+    } else {
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
+        else launch(mx_quantize_kernel<FORMAT, KIND, false, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
+    }
     return cudaGetLastError();
 }
 
@@ -1267,21 +1438,27 @@ cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, 
 #undef CALL8
 }
 
-// Groups of a dense [rows, cols] tensor beside a block-scaled one of the same shape, and whether all of them are
-// whole and aligned.
-template <typename T> static MxRows dense_groups(int64_t rows, int64_t cols, const void *a, const void *b, bool &vec) {
-    vec = cols % 8 == 0 && ((uintptr_t)a & 15) == 0 && ((uintptr_t)b & 15) == 0;
-    return vec && cols % (4 * MX_BLOCK) == 0 ? mx_rows(1, rows * cols) : mx_rows(rows, cols);
+// A dense [rows, cols] tensor beside a block-scaled one of the same shape: whether all its groups are whole and aligned,
+// and the shape to count in (dense rows of whole scale words are one long row).
+template <typename T> static bool mx_dense_shape(int64_t &rows, int64_t &cols, const void *a, const void *b) {
+    const bool vec = cols % 8 == 0 && (uintptr_t)a % (8 * sizeof(T)) == 0 && (uintptr_t)b % (8 * sizeof(T)) == 0;
+    if (vec && cols % (4 * MX_BLOCK) == 0) { cols *= rows; rows = 1; }
+    return vec;
 }
 
 template <int FORMAT, int KIND>
 static cudaError_t launch_mx_restore(cudaStream_t s, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *out) {
     using T = typename MxElement<KIND>::type;
     if (rows == 0 || cols == 0) return cudaSuccess;
-    bool vec;
-    const MxRows r = dense_groups<T>(rows, cols, out, out, vec);
-    if (vec) mx_restore_kernel<FORMAT, KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>(codes, scales, r, (T *)out);
-    else mx_restore_kernel<FORMAT, KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>(codes, scales, r, (T *)out);
+    const bool vec = mx_dense_shape<T>(rows, cols, out, out);
+    const auto launch = [&](auto kernel, auto shape) { kernel<<<mx_grid(rows * mx_scale_bytes(cols) * 4), MX_THREADS, 0, s>>>(codes, scales, shape, cols, (T *)out); };
+    if (mx_narrow_rows(rows, cols)) {
+        if (vec) launch(mx_restore_kernel<FORMAT, KIND, true, uint32_t>, mx_rows<uint32_t>(rows, cols, FORMAT));
+        else launch(mx_restore_kernel<FORMAT, KIND, false, uint32_t>, mx_rows<uint32_t>(rows, cols, FORMAT));
+    } else {
+        if (vec) launch(mx_restore_kernel<FORMAT, KIND, true, int64_t>, mx_rows<int64_t>(rows, cols, FORMAT));
+        else launch(mx_restore_kernel<FORMAT, KIND, false, int64_t>, mx_rows<int64_t>(rows, cols, FORMAT));
+    }
     return cudaGetLastError();
 }
 
@@ -1297,10 +1474,15 @@ template <int KIND>
 static cudaError_t launch_mx_activation_gradient(cudaStream_t s, int act, const uint8_t *codes, const uint8_t *scales, const void *g, int64_t rows, int64_t cols, void *out) {
     using T = typename MxElement<KIND>::type;
     if (rows == 0 || cols == 0) return cudaSuccess;
-    bool vec;
-    const MxRows r = dense_groups<T>(rows, cols, g, out, vec);
-    if (vec) mx_activation_gradient_kernel<KIND, true><<<mx_grid(r), MX_THREADS, 0, s>>>(act, codes, scales, (const T *)g, r, (T *)out);
-    else mx_activation_gradient_kernel<KIND, false><<<mx_grid(r), MX_THREADS, 0, s>>>(act, codes, scales, (const T *)g, r, (T *)out);
+    const bool vec = mx_dense_shape<T>(rows, cols, g, out);
+    const auto launch = [&](auto kernel, auto shape) { kernel<<<mx_grid(rows * mx_scale_bytes(cols) * 4), MX_THREADS, 0, s>>>(act, codes, scales, (const T *)g, shape, cols, (T *)out); };
+    if (mx_narrow_rows(rows, cols)) {
+        if (vec) launch(mx_activation_gradient_kernel<KIND, true, uint32_t>, mx_rows<uint32_t>(rows, cols, 8));
+        else launch(mx_activation_gradient_kernel<KIND, false, uint32_t>, mx_rows<uint32_t>(rows, cols, 8));
+    } else {
+        if (vec) launch(mx_activation_gradient_kernel<KIND, true, int64_t>, mx_rows<int64_t>(rows, cols, 8));
+        else launch(mx_activation_gradient_kernel<KIND, false, int64_t>, mx_rows<int64_t>(rows, cols, 8));
+    }
     return cudaGetLastError();
 }
 
@@ -1341,7 +1523,8 @@ static cudaError_t launch_mx_few(cudaStream_t s, const uint8_t *x, const uint8_t
     CUtensorMap map_w, map_x;
     const int64_t k = (int64_t)prm.blocks * MX_BLOCK;
     if (!make_code_map(&map_w, w, prm.n, k, 128) || !make_code_map(&map_x, x, prm.m, k, BN)) return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(mx_linear_few_kernel<BN, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = mx_prepare_kernel(mx_linear_few_kernel<BN, KIND>, Cfg::kSmemBytes, 0, done);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((int64_t)slices * prm.tiles_n * prm.tiles_m));
@@ -1379,12 +1562,9 @@ static cudaError_t launch_mx_pair(cudaStream_t s, const uint8_t *x, const uint8_
     const int groups = (prm.tiles_n + 7) / 8;
     prm.group_n = (prm.tiles_n + groups - 1) / groups;
     const int tiles = prm.tiles_m * prm.tiles_n, pairs = sm_count / 2;
-    cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, mx_linear_pair_kernel<KIND, GENERAL>);
-    if (e != cudaSuccess) return e;
     // the register split draws on what the block was launched with
-    if (attr.numRegs * MX_PAIR_THREADS < 128 * 72 + 256 * 216) return cudaErrorLaunchOutOfResources;
-    e = cudaFuncSetAttribute(mx_linear_pair_kernel<KIND, GENERAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = mx_prepare_kernel(mx_linear_pair_kernel<KIND, GENERAL>, Cfg::kSmemBytes, (MX_PAIR_REGS_LOW + MX_PAIR_REGS_SCALES + 2 * MX_PAIR_REGS_EPILOGUE + 3) / 4, done);
     if (e != cudaSuccess) return e;
     mx_linear_pair_kernel<KIND, GENERAL><<<2 * (tiles < pairs ? tiles : pairs), MX_PAIR_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_w, map_out, map_xs, map_ws, prm);
     return cudaGetLastError();
@@ -1481,12 +1661,9 @@ static cudaError_t launch_mx_gradient(cudaStream_t s, const MxGrad &prm, int sm_
     if (!make_row_map(&map_x, prm.codes, prm.rows, prm.code_pitch, prm.code_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)) return cudaErrorInvalidValue;
     map_g = map_x;              // unused without TMA
     if (TMA && !make_row_map(&map_g, prm.g, prm.rows, prm.n, prm.n, KIND == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T))) return cudaErrorInvalidValue;
-    cudaFuncAttributes attr;
-    cudaError_t e = cudaFuncGetAttributes(&attr, mx_weight_gradient_kernel<KIND, TMA>);
-    if (e != cudaSuccess) return e;
     // the register split draws on what the block was launched with
-    if (attr.numRegs * 3 < MX_GRAD_REGS_LOW + 2 * MX_GRAD_REGS_WORKER) return cudaErrorLaunchOutOfResources;
-    e = cudaFuncSetAttribute(mx_weight_gradient_kernel<KIND, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = mx_prepare_kernel(mx_weight_gradient_kernel<KIND, TMA>, Cfg::kSmemBytes, (MX_GRAD_REGS_LOW + 4 * MX_GRAD_REGS_WORKER + 4) / 5, done);
     if (e != cudaSuccess) return e;
     const int units = prm.tiles_n * prm.tiles_k * prm.slices, pairs = sm_count / 2;
     mx_weight_gradient_kernel<KIND, TMA><<<2 * (units < pairs ? units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_g, prm);

@@ -469,7 +469,10 @@ int32_t prepare_executable(Executable *x) {
         x->gemm_workspace = (float *)p;
         x->gemm_workspace_floats = workspace_floats;
     }
-    if (ctx->gemm_dynamic) {
+    // only tensor-core products take tiles from a counter; without any there is nothing to zero before every run
+    bool counted = false;
+    for (const StepExec &se : x->exec) counted |= se.tc != nullptr;
+    if (ctx->gemm_dynamic && counted) {
         void *p; if (!alloc((uint64_t)plan.steps.size() * 4, &p)) return ALLOCATION_FAILED;
         x->unit_counters = (int *)p;
     }
