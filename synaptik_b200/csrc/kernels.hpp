@@ -221,11 +221,12 @@ cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, 
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
                       const uint8_t *w, const uint8_t *w_scales, const uint8_t *x_tiles, const uint8_t *w_tiles, const void *bias, void *out,
                       int sm_count, int *error_word);
-// out[n, k] = sum over rows of g[row, n] * x[row, k], x held in 8 bits, out FLOAT32.  workspace: that many floats (0 =
-// none needed) for sums over slices of the rows, which a second launch adds.
-int64_t mx_weight_gradient_workspace(int64_t rows, int64_t n, int64_t k, int sm_count);
+// out[n, k] = sum over rows of g[row, n] * x[row, k], x held in 8 bits, out FLOAT32.  workspace: that many bytes, 256-byte
+// aligned, for the operands in the form the tensor cores read and for sums over slices of the rows.
+int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count);
+int mx_weight_gradient_launches(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count);
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
-                               const void *g, float *out, float *workspace, int sm_count, int *error_word);
+                               const void *g, float *out, void *workspace, int sm_count, int *error_word);
 
 }  // namespace kern
 }  // namespace syn

@@ -986,38 +986,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly: 8 + 8 + 8 significand bits for
 // FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
 // takes three products at the BFLOAT16 rate where a split into TF32 numbers would take three at half of it.
+//   mx_pieces_kernel writes the pieces and the checkpoint's values to scratch (8 bytes per element of g, 3 per element of
+// x to move; BFLOAT16 gradients whose rows TMA can address stay where they are), once each.  Converting inside the
+// product, by worker warps between raw and operand tiles, repeats it for every tile and was bound by the workers'
+// instructions and barriers: 1008 us on 8192 x 4096 x 4096 in FLOAT32, 523 us in BFLOAT16.
 //   Both operands are contracted along their rows, that is, they are MN-major tiles (64 columns of one row = one
-// 128-byte swizzle row).  TMA brings the rows as they are into a ring of raw slots, sixteen worker warps per block convert
-// them into operand tiles of that form, so no converted copy of either matrix exists in memory; BFLOAT16 gradients need
-// no conversion and go into the operand tiles at once.  (Rows of g that TMA cannot address, widths that are no multiple
-// of 16 bytes, the workers read themselves, one stage ahead.)  Tensor memory adds with truncation, so it only holds partial sums
-// of MX_CHUNK stages, which the workers, who have the time, add into FP32 registers: two accumulators in turn.
-//   Work is cut into units of one tile and one slice of the rows where that fills the block pairs better; slices go to
-// a workspace and are added in ascending order by a second kernel.
+// 128-byte swizzle row), which TMA loads as they lie.  Tensor memory adds with truncation, so it only holds partial sums
+// of kChunk stages, which the epilogue warps add into FP32 registers: two accumulators in turn.
+//   Tiles that do not fill a wave of block pairs are cut into slices of the rows; their sums go to scratch and are
+// added in ascending order by a last launch.
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 64;             // rows per stage
-constexpr int MX_GRAD_THREADS = 640;    // warp 0 MMA, warp 2 raw slots, warp 3 gradients that need no conversion, warps 4-19 workers
-constexpr int MX_GRAD_REGS_LOW = 56, MX_GRAD_REGS_WORKER = 104;
+constexpr int MX_GRAD_THREADS = 384;    // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue
 
-template <int KIND> struct MxGradConfig {
-    static constexpr int kPieces = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
+template <int PIECES> struct MxGradConfig {
     static constexpr int kTileBytes = MX_ROWS * 128 * 2;                // one operand piece of 128 columns
-    static constexpr int kStageBytes = (kPieces + 1) * kTileBytes;
-    static constexpr int kStages = KIND == 0 ? 2 : KIND == 1 ? 5 : 3;
-    static constexpr int kRawG = KIND == 0 ? MX_ROWS * 128 * 4 : KIND == 1 ? 0 : MX_ROWS * 128 * 2;
-    static constexpr int kRawBytes = kRawG + MX_ROWS * 128;             // rows of g, codes of the checkpoint
-    static constexpr int kRawSlots = KIND == 0 ? 2 : KIND == 1 ? 6 : 3;
-    static constexpr int kChunk = KIND == 0 ? 4 : 8;                    // stages per partial sum in tensor memory
-    static constexpr int kSmemBytes = kStages * kStageBytes + kRawSlots * (kRawBytes + MX_ROWS * 4) + 1024 + 512;
+    static constexpr int kStageBytes = (PIECES + 1) * kTileBytes;
+    static constexpr int kStages = PIECES == 3 ? 3 : PIECES == 2 ? 4 : 6;
+    static constexpr int kChunk = PIECES == 3 ? 4 : 8;                  // stages per partial sum in tensor memory
+    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
 };
 
 struct MxGrad {
-    int64_t rows; int n, k;
-    const uint8_t *codes, *scales; const void *g;
-    int64_t code_pitch, scale_pitch;
-    int tiles_n, tiles_k, slices;
-    int stages, stages_per_slice;       // of MX_ROWS rows
-    float *out; int64_t slice_floats;   // [slices][n][k]
+    int n, k;
+    int64_t rows;
+    int tiles_n, whole_tiles, units;    // units: the whole tiles, then `slices` per tile that is left
+    int slices, stages, stages_per_slice;       // of MX_ROWS rows
+    float *out, *partial;               // partial: [tile that is left][slice][256][256]
     int *error_word;
 };
 
@@ -1031,78 +1026,76 @@ template <bool FIRST> __device__ __forceinline__ uint32_t mx_piece(float &a, flo
     b = FIRST && fabsf(b) == __uint_as_float(0x7f800000u) ? 0.0f : rb;
     return word;
 }
-__device__ __forceinline__ void mx_store_chunk(uint32_t tile, int row, int chunk, const uint32_t (&w)[4]) {
-    const uint32_t dst = tile + (uint32_t)((chunk >> 3) * (MX_ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-}
 
-// Eight columns of one row of g that TMA cannot address.
-template <int KIND>
-__device__ __forceinline__ void mx_fetch8(const typename MxElement<KIND>::type *row, int c, int n, bool here, uint32_t (&v)[KIND == 0 ? 8 : 4]) {
+// The first g_blocks blocks cut g [rows, n] into pieces, planes [PIECES][rows][g_pitch]; the others restore x into [rows, x_pitch].
+// Padding columns are written as zeros.  A thread takes groups of eight columns.
+template <int KIND, bool VEC>
+__global__ void __launch_bounds__(MX_THREADS) mx_pieces_kernel(const typename MxElement<KIND>::type *__restrict__ g, int64_t rows, int64_t n, int64_t g_pitch, uint16_t *__restrict__ g_planes, int g_blocks,
+                                                               const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t x_pitch, int64_t scale_pitch, uint16_t *__restrict__ x_plane) {
+    constexpr int PIECES = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
+    if ((int)blockIdx.x < g_blocks) {
+        __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
+        const int64_t per_row = g_pitch / 8, total = rows * per_row, hop = (int64_t)g_blocks * MX_THREADS;
+        int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x, row = i / per_row, group = i - row * per_row;
+        const int64_t hop_rows = hop / per_row, hop_groups = hop - hop_rows * per_row;
+        for (; (i & ~(int64_t)31) < total; i += hop) {
+            const int64_t left = i < total ? n - group * 8 : 0;
+            const int count = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+            float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (VEC) { if (count) mx_load8<KIND>(g + row * n + group * 8, f); }
+            else mx_gather8<KIND>(g, row * n + group * 8, 1, count, boxes[threadIdx.x >> 5], threadIdx.x & 31, f);
+            if (i < total) {
 #pragma unroll
-    for (int e = 0; e < (KIND == 0 ? 8 : 4); e++) {
-        if constexpr (KIND == 0) v[e] = here && c + e < n ? __float_as_uint(__ldg(row + c + e)) : 0u;
-        else v[e] = (here && c + 2 * e < n ? (uint32_t)__ldg(row + c + 2 * e) : 0u) | (here && c + 2 * e + 1 < n ? (uint32_t)__ldg(row + c + 2 * e + 1) << 16 : 0u);
+                for (int piece = 0; piece < PIECES; piece++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = piece == 0 ? mx_piece<true>(f[2 * e], f[2 * e + 1]) : mx_piece<false>(f[2 * e], f[2 * e + 1]);
+                    *reinterpret_cast<uint4 *>(g_planes + ((int64_t)piece * rows + row) * g_pitch + group * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            row += hop_rows; group += hop_groups;
+            if (group >= per_row) { group -= per_row; row++; }
+        }
+    } else {
+        const int64_t per_row = x_pitch / 8, total = rows * per_row, hop = (int64_t)(gridDim.x - g_blocks) * MX_THREADS;
+        int64_t i = (int64_t)(blockIdx.x - g_blocks) * MX_THREADS + threadIdx.x, row = i / per_row, group = i - row * per_row;
+        const int64_t hop_rows = hop / per_row, hop_groups = hop - hop_rows * per_row;
+        for (; i < total; i += hop) {
+            const uint2 c = __ldg(reinterpret_cast<const uint2 *>(codes + row * x_pitch + group * 8));
+            const float scale = mx_scale_value(__ldg(scales + row * scale_pitch + (group >> 2)));
+            float v[8];
+            mx_decode8x2(c.x & 0xffffu, v[0], v[1]); mx_decode8x2(c.x >> 16, v[2], v[3]);
+            mx_decode8x2(c.y & 0xffffu, v[4], v[5]); mx_decode8x2(c.y >> 16, v[6], v[7]);
+            *reinterpret_cast<uint4 *>(x_plane + row * x_pitch + group * 8) = make_uint4(low_pack2<1>(v[0] * scale, v[1] * scale), low_pack2<1>(v[2] * scale, v[3] * scale),
+                                                                                         low_pack2<1>(v[4] * scale, v[5] * scale), low_pack2<1>(v[6] * scale, v[7] * scale));
+            row += hop_rows; group += hop_groups;
+            if (group >= per_row) { group -= per_row; row++; }
+        }
     }
 }
 
-// Eight columns of one row of g as operand pieces, the leading one first in memory.
-template <int KIND>
-__device__ __forceinline__ void mx_put_pieces(uint32_t stage, int row, int chunk, const uint32_t (&u)[KIND == 0 ? 8 : 4]) {
-    using Cfg = MxGradConfig<KIND>;
-    if constexpr (KIND == 1) mx_store_chunk(stage, row, chunk, u);
-    else {
-        float f[8];
-        if constexpr (KIND == 0) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = __uint_as_float(u[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) low_unpack_half2(u[e], f[2 * e], f[2 * e + 1]);
-        }
-#pragma unroll
-        for (int piece = 0; piece < Cfg::kPieces; piece++) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = piece == 0 ? mx_piece<true>(f[2 * e], f[2 * e + 1]) : mx_piece<false>(f[2 * e], f[2 * e + 1]);
-            mx_store_chunk(stage + piece * Cfg::kTileBytes, row, chunk, w);
-        }
-    }
-}
-__device__ __forceinline__ void mx_read16(uint32_t addr, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
-}
-
-template <int KIND, bool TMA>
+template <int PIECES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) mx_weight_gradient_kernel(
-        const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_g, MxGrad prm) {
-    using Cfg = MxGradConfig<KIND>;
-    using T = typename MxElement<KIND>::type;
-    constexpr int S = Cfg::kStages, R = Cfg::kRawSlots;
-    constexpr bool DIRECT = TMA && KIND == 1;           // g goes into the operand tiles as it is
-    constexpr bool RAW_G = TMA && KIND != 1;
+        const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, MxGrad prm) {
+    using Cfg = MxGradConfig<PIECES>;
+    constexpr int S = Cfg::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes + R * (Cfg::kRawBytes + MX_ROWS * 4));
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 2 * R + 4);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem);
-    const uint32_t raw_base = smem_base + S * Cfg::kStageBytes, scale_base = raw_base + R * Cfg::kRawBytes;
-    // full and accumulator-empty barriers are those of the even block (one arrival per worker warp of both blocks);
-    // empty, accumulator-full and the two of the raw slots are each block's own
+    // full and accumulator-empty barriers are those of the even block; empty and accumulator-full are each block's own
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
-    auto raw_full_bar = [&](int i) { return bar_base + 8u * (2 * S + i); };
-    auto raw_empty_bar = [&](int i) { return bar_base + 8u * (2 * S + R + i); };
-    auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 * R + a); };
-    auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 * R + 2 + a); };
+    auto acc_full_bar = [&](int a) { return bar_base + 8u * (2 * S + a); };
+    auto acc_empty_bar = [&](int a) { return bar_base + 8u * (2 * S + 2 + a); };
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), DIRECT ? 33 : 32); mbar_init(empty_bar(s), 1); }
-        for (int i = 0; i < R; i++) { mbar_init(raw_full_bar(i), 33); mbar_init(raw_empty_bar(i), 16); }     // TMA and 32 lanes of scales
-        for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 32); }
+        for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < 2; a++) { mbar_init(acc_full_bar(a), 1); mbar_init(acc_empty_bar(a), 16); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1116,19 +1109,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int units = prm.tiles_n * prm.tiles_k * prm.slices;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    // stages of a unit; every slice has at least one
-    auto first_stage = [&](int unit) { return unit % prm.slices * prm.stages_per_slice; };
-    auto stage_count = [&](int unit) { const int left = prm.stages - first_stage(unit); return left < prm.stages_per_slice ? left : prm.stages_per_slice; };
-    auto tile_of = [&](int unit, int &n0, int &k0) {        // of the pair's tile
-        const int tile = unit / prm.slices;
+    // a unit's tile and stages; every slice has at least one
+    auto unit_of = [&](int unit, int &n0, int &k0, int &first, int &count) {
+        int tile = unit;
+        first = 0; count = prm.stages;
+        if (unit >= prm.whole_tiles) {
+            const int u = unit - prm.whole_tiles;
+            tile = prm.whole_tiles + u / prm.slices;
+            first = u % prm.slices * prm.stages_per_slice;
+            count = prm.stages - first < prm.stages_per_slice ? prm.stages - first : prm.stages_per_slice;
+        }
         n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * 256;
     };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_LOW));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
+            if (lane == 0) {
+                int stage = 0; uint32_t phase = 0;
+                int armed = 0;
+                bool ok = true;
+                for (int unit = pair; unit < prm.units && ok; unit += pairs) {
+                    int n0, k0, first, count;
+                    unit_of(unit, n0, k0, first, count);
+                    n0 += (int)rank * 128; k0 += (int)rank * 128;
+                    for (int i = 0; i < count; i++) {
+                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                        const uint32_t leader_full = map_to_rank(full_bar(stage), 0), pa = smem_base + stage * Cfg::kStageBytes, pb = pa + PIECES * Cfg::kTileBytes;
+                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kStageBytes);
+                        const int r0 = (first + i) * MX_ROWS;
+                        // boxes of 64 columns (128 bytes) x 64 rows; columns and rows past the matrix read as zeros
+#pragma unroll
+                        for (int half = 0; half < 2; half++) {
+#pragma unroll
+                            for (int piece = 0; piece < PIECES; piece++)
+                                tma_load_3d_pair(pa + piece * Cfg::kTileBytes + half * (MX_ROWS * 128), &map_g, leader_full, n0 + half * 64, r0, piece);
+                            tma_load_2d_pair(pb + half * (MX_ROWS * 128), &map_x, leader_full, k0 + half * 64, r0);
+                        }
+                        armed = armed < (1 << 30) ? armed + 1 : armed;
+                        if (++stage == S) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                // giving up: the even block waits for both blocks' copies in flight; the odd one cannot leave before it
+                if ((!ok || *abort_flag) && rank == 0) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
+            }
+        } else if (warp == 1) {
             if (rank == 0 && lane == 0) {
                 // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
                 const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
@@ -1137,8 +1163,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
                 int stage = 0; uint32_t phase = 0, chunk = 0;
                 bool ok = true;
-                for (int unit = pair; unit < units && ok; unit += pairs) {
-                    const int count = stage_count(unit);
+                for (int unit = pair; unit < prm.units && ok; unit += pairs) {
+                    int n0, k0, first, count;
+                    unit_of(unit, n0, k0, first, count);
                     for (int i0 = 0; i0 < count && ok; i0 += Cfg::kChunk, chunk++) {
                         const int buf = chunk & 1;
                         if (!mbar_wait_cluster(acc_empty_bar(buf), ((chunk >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
@@ -1148,13 +1175,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                         for (int i = i0; i < i1; i++) {
                             if (!mbar_wait_cluster(full_bar(stage), phase, abort_flag)) { ok = false; break; }
                             tc_fence_after();
-                            const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kPieces * Cfg::kTileBytes;
+                            const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + PIECES * Cfg::kTileBytes;
 #pragma unroll
-                            for (int piece = Cfg::kPieces - 1; piece >= 0; piece--)         // small terms first
+                            for (int piece = PIECES - 1; piece >= 0; piece--)         // small terms first
 #pragma unroll
                                 for (int r16 = 0; r16 < MX_ROWS / 16; r16++)
                                     umma_f16_pair(d, desc(pa + piece * Cfg::kTileBytes + r16 * 2048), desc(pb + r16 * 2048), idesc,
-                                                  (i != i0 || piece != Cfg::kPieces - 1 || r16 != 0) ? 1u : 0u);
+                                                  (i != i0 || piece != PIECES - 1 || r16 != 0) ? 1u : 0u);
                             umma_commit_pair(empty_bar(stage));
                             umma_commit_pair(map_to_rank(empty_bar(stage), 1));
                             if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -1163,184 +1190,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                     }
                 }
             }
-        } else if (warp == 2) {
-            // raw slots: one lane's TMA for the rows, every lane two words of scales
-            int slot = 0; uint32_t phase = 0;
-            int armed = 0;
-            bool ok = true;
-            for (int unit = pair; unit < units && ok; unit += pairs) {
-                int n0, k0;
-                tile_of(unit, n0, k0);
-                n0 += (int)rank * 128; k0 += (int)rank * 128;
-                const int count = stage_count(unit);
-                for (int i = 0; i < count; i++) {
-                    ok = mx_warp_wait(raw_empty_bar(slot), phase ^ 1u, abort_flag, lane);
-                    if (!ok) break;
-                    const int r0 = (first_stage(unit) + i) * MX_ROWS;
-                    const uint32_t raw = raw_base + slot * Cfg::kRawBytes;
-                    if (lane == 0) {
-                        mbar_expect_tx(raw_full_bar(slot), (RAW_G ? Cfg::kRawG : 0) + MX_ROWS * 128);
-                        // boxes of 128 bytes x 64 rows; coordinates along a row are multiples of 128 bytes, what lies past the
-                        // matrix reads as zeros
-                        if constexpr (RAW_G) {
-                            constexpr int WIDTH = 128 / sizeof(T);
-#pragma unroll
-                            for (int b = 0; b < 128 / WIDTH; b++) tma_load_2d(raw + b * (MX_ROWS * 128), &map_g, raw_full_bar(slot), n0 + b * WIDTH, r0);
-                        }
-                        tma_load_2d(raw + Cfg::kRawG, &map_x, raw_full_bar(slot), k0, r0);
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int64_t row = r0 + h * 32 + lane;
-                        const bool here = row < prm.rows && k0 < prm.k;
-                        mx_copy_word(scale_base + (uint32_t)(slot * MX_ROWS + h * 32 + lane) * 4u, here ? prm.scales + row * prm.scale_pitch + (k0 >> 5) : prm.scales, here ? 4 : 0);
-                    }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full_bar(slot)) : "memory");
-                    armed = armed < (1 << 30) ? armed + 1 : armed;
-                    if (++slot == R) { slot = 0; phase ^= 1u; }
-                }
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            if (lane == 0 && (!ok || *abort_flag)) for (int i = armed > R ? armed - R : 0; i < armed; i++) mx_wait_landed(raw_full_bar(i % R), (uint32_t)(i / R) & 1u);
-        } else if (warp == 3) {
-            if (DIRECT && lane == 0) {
-                int stage = 0; uint32_t phase = 0;
-                int armed = 0;
-                bool ok = true;
-                for (int unit = pair; unit < units && ok; unit += pairs) {
-                    int n0, k0;
-                    tile_of(unit, n0, k0);
-                    n0 += (int)rank * 128;
-                    const int count = stage_count(unit);
-                    for (int i = 0; i < count; i++) {
-                        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
-                        const uint32_t leader_full = map_to_rank(full_bar(stage), 0), pa = smem_base + stage * Cfg::kStageBytes;
-                        if (rank == 0) mbar_expect_tx(full_bar(stage), 2 * Cfg::kTileBytes);
-                        const int r0 = (first_stage(unit) + i) * MX_ROWS;
-                        tma_load_2d_pair(pa, &map_g, leader_full, n0, r0);
-                        tma_load_2d_pair(pa + MX_ROWS * 128, &map_g, leader_full, n0 + 64, r0);
-                        armed = armed < (1 << 30) ? armed + 1 : armed;
-                        if (++stage == S) { stage = 0; phase ^= 1u; }
-                    }
-                }
-                // giving up: these barriers also wait for the workers, so this may take its whole tenth of a second
-                if ((!ok || *abort_flag) && rank == 0) for (int i = armed > S ? armed - S : 0; i < armed; i++) mx_wait_landed(full_bar(i % S), (uint32_t)(i / S) & 1u);
-            }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_GRAD_REGS_WORKER));
-        // a warp converts 8 rows of one half of the columns, and adds up 32 x 64 results
-        const int worker = warp - 4, row_in_stage = (worker & 7) * 8 + (lane & 7), group = lane >> 3, side = worker >> 3;
-        const int quarter = warp & 3, part = worker >> 2;
-        float sum[64];
-        uint32_t ahead[2][KIND == 0 ? 8 : 4];               // of g, without TMA
-        int stage = 0, slot = 0; uint32_t phase = 0, slot_phase = 0;
-        auto fetch_ahead = [&](int unit, int i) {
-            if constexpr (!TMA) {
-                int n0, k0;
-                tile_of(unit, n0, k0);
-                const int64_t row = (int64_t)(first_stage(unit) + i) * MX_ROWS + row_in_stage;
-                const bool here = row < prm.rows;
-                const T *p = (const T *)prm.g + (here ? row : 0) * prm.n;
-#pragma unroll
-                for (int j = 0; j < 2; j++) mx_fetch8<KIND>(p, n0 + (int)rank * 128 + (side * 8 + j * 4 + group) * 8, prm.n, here, ahead[j]);
-            }
-        };
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        uint32_t chunk = 0;
         bool ok = true;
-        int unit = pair, i0 = 0, count = unit < units ? stage_count(unit) : 0;
-        int open_unit = -1; bool open_first = false, open_last = false;        // the chunk that still lies in tensor memory
-        if (unit < units) fetch_ahead(unit, 0);
-        // A chunk is handed over stage by stage; then the one before it, which the MMAs have finished meanwhile, is added up.
-        for (uint32_t chunk = 0; ok; chunk++) {
-            const bool more = unit < units;
-            const int this_unit = unit;
-            bool first = false, last = false;
-            if (more) {
-                const int i1 = i0 + Cfg::kChunk < count ? i0 + Cfg::kChunk : count;
-                first = i0 == 0; last = i1 == count;
-                for (int i = i0; i < i1; i++) {
-                    if (!mx_warp_wait(empty_bar(stage), phase ^ 1u, abort_flag, lane) || !mx_warp_wait(raw_full_bar(slot), slot_phase, abort_flag, lane)) { ok = false; break; }
-                    const uint32_t dst = smem_base + stage * Cfg::kStageBytes, raw = raw_base + slot * Cfg::kRawBytes + row_in_stage * 128;
-                    const uint32_t twist = (uint32_t)(row_in_stage & 7);
-                    if constexpr (!DIRECT) {
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const int c = side * 8 + j * 4 + group;
-                            if constexpr (RAW_G) {
-                                uint32_t u[KIND == 0 ? 8 : 4];      // chunk of eight columns: 16 or 32 bytes of the row
-                                if constexpr (KIND == 0) {
-                                    const uint32_t box = raw + (uint32_t)((c >> 2) * (MX_ROWS * 128)), q = (uint32_t)(c & 3) * 2u;
-                                    mx_read16(box + ((q ^ twist) << 4), u[0], u[1], u[2], u[3]);
-                                    mx_read16(box + (((q + 1u) ^ twist) << 4), u[KIND == 0 ? 4 : 0], u[KIND == 0 ? 5 : 1], u[KIND == 0 ? 6 : 2], u[KIND == 0 ? 7 : 3]);
-                                } else mx_read16(raw + (uint32_t)((c >> 3) * (MX_ROWS * 128)) + (((uint32_t)(c & 7) ^ twist) << 4), u[0], u[1], u[2], u[3]);
-                                mx_put_pieces<KIND>(dst, row_in_stage, c, u);
-                            } else mx_put_pieces<KIND>(dst, row_in_stage, c, ahead[j]);
-                        }
-                    }
-                    // half a block of the checkpoint: 16 bytes
-                    const int c = side * 4 + group;
-                    uint32_t byte, x[4];
-                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(byte) : "r"(scale_base + (uint32_t)((slot * MX_ROWS + row_in_stage) * 4 + (c >> 1))));
-                    mx_read16(raw + Cfg::kRawG + (((uint32_t)c ^ twist) << 4), x[0], x[1], x[2], x[3]);
-                    const float scale = mx_scale_value(byte);
-#pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float a, b;
-                            mx_decode8x2(x[q * 2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu, a, b);
-                            w[e] = low_pack2<1>(a * scale, b * scale);
-                        }
-                        mx_store_chunk(dst + Cfg::kPieces * Cfg::kTileBytes, row_in_stage, c * 2 + q, w);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) { mx_arrive_rank(full_bar(stage), 0); mbar_arrive(raw_empty_bar(slot)); }
-                    if (++stage == S) { stage = 0; phase ^= 1u; }
-                    if (++slot == R) { slot = 0; slot_phase ^= 1u; }
-                    if (i + 1 < count) fetch_ahead(unit, i + 1);
-                    else if (unit + pairs < units) fetch_ahead(unit + pairs, 0);
-                }
-                if (!ok) break;
-                i0 = i1;
-                if (i0 == count) { unit += pairs; i0 = 0; count = unit < units ? stage_count(unit) : 0; }
-            }
-            if (open_unit >= 0) {
-                const uint32_t c = chunk - 1;
-                const int buf = c & 1;
-                ok = mx_warp_wait(acc_full_bar(buf), (c >> 1) & 1u, abort_flag, lane);
+        for (int unit = pair; unit < prm.units && ok; unit += pairs) {
+            int n0, k0, first, count;
+            unit_of(unit, n0, k0, first, count);
+            float sum[128];
+            for (int i0 = 0; i0 < count; i0 += Cfg::kChunk, chunk++) {
+                const int buf = chunk & 1;
+                ok = mx_warp_wait(acc_full_bar(buf), (chunk >> 1) & 1u, abort_flag, lane);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + part * 64);
+                const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
+                if (i0 == 0) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    float t[16];
-                    tmem_load16(taddr + (uint32_t)(q * 16), t);
+                    for (int q = 0; q < 8; q++) {
+                        float t[16];
+                        tmem_load16(taddr + (uint32_t)(q * 16), t);
 #pragma unroll
-                    for (int e = 0; e < 16; e++) sum[q * 16 + e] = open_first ? t[e] : __fadd_rn(sum[q * 16 + e], t[e]);
+                        for (int e = 0; e < 16; e++) sum[q * 16 + e] = t[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        float t[16];
+                        tmem_load16(taddr + (uint32_t)(q * 16), t);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) sum[q * 16 + e] = __fadd_rn(sum[q * 16 + e], t[e]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mx_arrive_rank(acc_empty_bar(buf), 0);
-                if (open_last) {
-                    int n0, k0;
-                    tile_of(open_unit, n0, k0);
-                    const int n = n0 + (int)rank * 128 + quarter * 32 + lane, c0 = k0 + part * 64;
-                    float *out = prm.out + open_unit % prm.slices * prm.slice_floats + (int64_t)n * prm.k + c0;
-                    if (n < prm.n) {
-                        if ((prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0) {
+            }
+            if (!ok) break;
+            const int row = (int)rank * 128 + quarter * 32 + lane, col = half * 128;     // in the tile
+            if (unit >= prm.whole_tiles) {
+                float *out = prm.partial + (int64_t)(unit - prm.whole_tiles) * 65536 + row * 256 + col;
 #pragma unroll
-                            for (int q = 0; q < 16; q++) if (c0 + q * 4 < prm.k) *reinterpret_cast<float4 *>(out + q * 4) = make_float4(sum[q * 4], sum[q * 4 + 1], sum[q * 4 + 2], sum[q * 4 + 3]);
-                        } else {
+                for (int q = 0; q < 16; q++) {
+                    float v[8];
 #pragma unroll
-                            for (int q = 0; q < 64; q++) if (c0 + q < prm.k) out[q] = sum[q];
-                        }
+                    for (int e = 0; e < 8; e++) v[e] = sum[q * 8 + e];
+                    mx_store8<0>(out + q * 8, v);
+                }
+            } else if (n0 + row < prm.n) {
+                float *out = prm.out + (int64_t)(n0 + row) * prm.k + k0 + col;
+                const int left = prm.k - k0 - col;
+                if ((prm.k & 7) == 0 && ((uintptr_t)prm.out & 31) == 0) {
+#pragma unroll
+                    for (int q = 0; q < 16; q++) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[e] = sum[q * 8 + e];
+                        if (q * 8 < left) mx_store8<0>(out + q * 8, v);
                     }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 128; q++) if (q < left) out[q] = sum[q];
                 }
             }
-            if (!more) break;
-            open_unit = this_unit; open_first = first; open_last = last;
         }
     }
 
@@ -1356,24 +1269,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     }
 }
 
-// out = the slices' sums in ascending order.
-__global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(const float *__restrict__ ws, int slices, int64_t count, float *__restrict__ out) {
-    for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i * 4 < count; i += (int64_t)gridDim.x * MX_THREADS) {
-        const int64_t at = i * 4;
-        if (at + 3 < count && (count & 3) == 0 && ((uintptr_t)out & 15) == 0) {
-            float4 a = __ldg(reinterpret_cast<const float4 *>(ws + at));
-            for (int q = 1; q < slices; q++) {
-                const float4 b = __ldg(reinterpret_cast<const float4 *>(ws + q * count + at));
-                a.x = __fadd_rn(a.x, b.x); a.y = __fadd_rn(a.y, b.y); a.z = __fadd_rn(a.z, b.z); a.w = __fadd_rn(a.w, b.w);
-            }
-            *reinterpret_cast<float4 *>(out + at) = a;
-        } else {
-            for (int e = 0; e < 4 && at + e < count; e++) {
-                float a = ws[at + e];
-                for (int q = 1; q < slices; q++) a = __fadd_rn(a, ws[q * count + at + e]);
-                out[at + e] = a;
-            }
-        }
+// The tiles that were cut into slices: their sums in ascending order.  blockIdx.y: the tile; a thread adds four columns.
+__global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(MxGrad prm) {
+    const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * 256;
+    const int i = blockIdx.x * MX_THREADS + threadIdx.x, row = i >> 6, col = (i & 63) * 4;
+    if (n0 + row >= prm.n || k0 + col >= prm.k) return;
+    const float *p = prm.partial + (int64_t)blockIdx.y * prm.slices * 65536 + row * 256 + col;
+    float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+    for (int q = 1; q < prm.slices; q++) {
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(p + (int64_t)q * 65536));
+        a.x = __fadd_rn(a.x, b.x); a.y = __fadd_rn(a.y, b.y); a.z = __fadd_rn(a.z, b.z); a.w = __fadd_rn(a.w, b.w);
+    }
+    float *out = prm.out + (int64_t)(n0 + row) * prm.k + k0 + col;
+    if ((prm.k & 3) == 0 && ((uintptr_t)prm.out & 15) == 0) *reinterpret_cast<float4 *>(out) = a;
+    else {
+        const float v[4] = {a.x, a.y, a.z, a.w};
+        for (int e = 0; e < 4; e++) if (k0 + col + e < prm.k) out[e] = v[e];
     }
 }
 
@@ -1621,80 +1532,117 @@ cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n
 #undef CALL
 }
 
-// Slices of the rows: the choice with the least time in stages, counting a slice's own cost (filling the pipeline, and
-// the second pass over its share of the result) as two stages of 64 rows.
-static int mx_gradient_slices(int64_t rows, int64_t n, int64_t k, int sm_count) {
-    const int64_t tiles = ((n + 255) / 256) * ((k + 255) / 256), pairs = sm_count / 2 > 0 ? sm_count / 2 : 1, stages = (rows + MX_ROWS - 1) / MX_ROWS;
-    int best = 1;
-    double best_cost = 1e300;
-    for (int64_t s = 1; s <= 64 && s <= stages; s++) {
-        const int64_t per = (stages + s - 1) / s;
-        if ((stages + per - 1) / per != s) continue;            // some slice would be empty
-        const double cost = (double)((tiles * s + pairs - 1) / pairs) * ((double)per + 2.0) + (s > 1 ? 4.0 + 0.25 * (double)(tiles * s) / (double)pairs : 0.0);
-        if (cost < best_cost) { best_cost = cost; best = (int)s; }
+// How the tiles are spread over the block pairs, and what scratch that takes.
+struct MxGradPlan {
+    int pieces, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
+    int64_t g_pitch, g_bytes, x_bytes, partial_bytes;       // of the planes and partial sums, each a multiple of 256
+};
+static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
+    MxGradPlan p = {};
+    p.pieces = dtype == DType::F32 ? 3 : dtype == DType::BF16 ? 1 : 2;
+    p.tiles_n = (int)((n + 255) / 256); p.tiles = p.tiles_n * (int)((k + 255) / 256);
+    p.stages = (int)((rows + MX_ROWS - 1) / MX_ROWS);
+    const int pairs = sm_count / 2 > 0 ? sm_count / 2 : 1;
+    p.whole_tiles = p.tiles / pairs * pairs;
+    // Tiles left over: the number of slices with the least estimated time.  A stage takes 0.3 us per piece, a unit's start
+    // and end about 1.5 us, the last launch 3 us and 0.1 us per slice of a tile (512 KB to write and read).
+    const int left = p.tiles - p.whole_tiles;
+    p.slices = 1;
+    double best = 1e300;
+    for (int s = 1; left > 0 && s <= 64 && s <= p.stages; s++) {
+        const int per = (p.stages + s - 1) / s;
+        if ((p.stages + per - 1) / per != s) continue;          // some slice would be empty
+        const double cost = (double)(((int64_t)left * s + pairs - 1) / pairs) * (0.3 * p.pieces * per + 1.5) + (s > 1 ? 3.0 + 0.1 * left * s : 0.0);
+        if (cost < best) { best = cost; p.slices = s; }
     }
-    return best;
+    if (p.slices == 1) p.whole_tiles = p.tiles;
+    p.stages_per_slice = p.stages > 0 ? (p.stages + p.slices - 1) / p.slices : 0;
+    const auto rounded = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
+    p.g_pitch = (n + 7) / 8 * 8;
+    p.g_bytes = rounded(p.pieces * rows * p.g_pitch * 2);
+    p.x_bytes = rounded(rows * mx_code_bytes(8, k) * 2);
+    p.partial_bytes = p.slices > 1 ? (int64_t)left * p.slices * 65536 * 4 : 0;
+    return p;
 }
 
-int64_t mx_weight_gradient_workspace(int64_t rows, int64_t n, int64_t k, int sm_count) {
-    const int slices = mx_gradient_slices(rows, n, k, sm_count);
-    return slices > 1 ? (int64_t)slices * n * k : 0;
+// BFLOAT16 rows that TMA can address are read where they are.
+static bool mx_gradient_direct(DType dtype, int64_t n) { return dtype == DType::BF16 && n % 8 == 0; }
+
+int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
+    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, sm_count);
+    return p.g_bytes + p.x_bytes + p.partial_bytes;
+}
+int mx_weight_gradient_launches(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
+    return rows == 0 ? 1 : mx_gradient_plan(dtype, rows, n, k, sm_count).slices > 1 ? 3 : 2;
 }
 
-// Tensor map over [rows, cols] of elements of `bytes` bytes: boxes of 128 bytes x 64 rows, 128-byte swizzle.
-static bool make_row_map(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t pitch, CUtensorMapDataType type, int bytes) {
+// Tensor map over BFLOAT16 planes [planes][rows][pitch] of `cols` columns: boxes of 64 columns x 64 rows, 128-byte swizzle.
+static bool make_piece_map(CUtensorMap *map, const void *base, int64_t planes, int64_t rows, int64_t cols, int64_t pitch) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)(pitch * bytes)};
-    cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), (cuuint32_t)MX_ROWS};
-    cuuint32_t elem[2] = {1, 1};
-    return fn(map, type, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)(rows * pitch) * 2};
+    cuuint32_t box[3] = {64, MX_ROWS, 1};
+    cuuint32_t elem[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, planes > 0 ? 3 : 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KIND, bool TMA>
-static cudaError_t launch_mx_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
-    using Cfg = MxGradConfig<KIND>;
-    using T = typename MxElement<KIND>::type;
-    CUtensorMap map_x, map_g;
-    if (!make_row_map(&map_x, prm.codes, prm.rows, prm.code_pitch, prm.code_pitch, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)) return cudaErrorInvalidValue;
-    map_g = map_x;              // unused without TMA
-    if (TMA && !make_row_map(&map_g, prm.g, prm.rows, prm.n, prm.n, KIND == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T))) return cudaErrorInvalidValue;
+template <int PIECES>
+static cudaError_t launch_mx_gradient(cudaStream_t s, const CUtensorMap &map_g, const CUtensorMap &map_x, const MxGrad &prm, int sm_count) {
+    using Cfg = MxGradConfig<PIECES>;
     // the register split draws on what the block was launched with
     static std::atomic<uint64_t> done{0};
-    cudaError_t e = mx_prepare_kernel(mx_weight_gradient_kernel<KIND, TMA>, Cfg::kSmemBytes, (MX_GRAD_REGS_LOW + 4 * MX_GRAD_REGS_WORKER + 4) / 5, done);
+    cudaError_t e = mx_prepare_kernel(mx_weight_gradient_kernel<PIECES>, Cfg::kSmemBytes, (72 + 2 * 216 + 2) / 3, done);
     if (e != cudaSuccess) return e;
-    const int units = prm.tiles_n * prm.tiles_k * prm.slices, pairs = sm_count / 2;
-    mx_weight_gradient_kernel<KIND, TMA><<<2 * (units < pairs ? units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_g, prm);
+    const int pairs = sm_count / 2;
+    mx_weight_gradient_kernel<PIECES><<<2 * (prm.units < pairs ? prm.units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(map_g, map_x, prm);
     return cudaGetLastError();
 }
 
 template <int KIND>
-static cudaError_t launch_mx_weight_gradient(cudaStream_t s, const MxGrad &prm, int sm_count) {
+static cudaError_t launch_mx_pieces(cudaStream_t s, const void *g, int64_t rows, int64_t n, const MxGradPlan &p, uint16_t *g_planes, bool direct,
+                                    const uint8_t *codes, const uint8_t *scales, int64_t x_pitch, int64_t scale_pitch, uint16_t *x_plane) {
     using T = typename MxElement<KIND>::type;
-    return (int64_t)prm.n * sizeof(T) % 16 == 0 && ((uintptr_t)prm.g & 15) == 0 ? launch_mx_gradient<KIND, true>(s, prm, sm_count) : launch_mx_gradient<KIND, false>(s, prm, sm_count);
+    // blocks in proportion to the bytes moved
+    const int64_t g_work = direct ? 0 : rows * p.g_pitch / 8, x_work = rows * x_pitch / 8;
+    const int64_t most = 148 * 8;
+    const double share = (double)g_work * (sizeof(T) + 2.0 * p.pieces) / ((double)g_work * (sizeof(T) + 2.0 * p.pieces) + (double)x_work * 3.0);
+    const auto blocks = [&](int64_t work, double part) {
+        const int64_t want = (work + MX_THREADS - 1) / MX_THREADS, limit = (int64_t)(most * part) < 1 ? 1 : (int64_t)(most * part);
+        return (int)(want < limit ? want : limit);
+    };
+    const int g_blocks = g_work ? blocks(g_work, share) : 0, x_blocks = blocks(x_work, 1.0 - share);
+    const bool vec = n % 8 == 0 && (uintptr_t)g % (8 * sizeof(T)) == 0;
+    if (vec) mx_pieces_kernel<KIND, true><<<g_blocks + x_blocks, MX_THREADS, 0, s>>>((const T *)g, rows, n, p.g_pitch, g_planes, g_blocks, codes, scales, x_pitch, scale_pitch, x_plane);
+    else mx_pieces_kernel<KIND, false><<<g_blocks + x_blocks, MX_THREADS, 0, s>>>((const T *)g, rows, n, p.g_pitch, g_planes, g_blocks, codes, scales, x_pitch, scale_pitch, x_plane);
+    return cudaGetLastError();
 }
 
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
-                               const void *g, float *out, float *workspace, int sm_count, int *error_word) {
+                               const void *g, float *out, void *workspace, int sm_count, int *error_word) {
     if (n == 0 || k == 0) return cudaSuccess;
     if (rows == 0) return cudaMemsetAsync(out, 0, (size_t)n * k * 4, s);
-    if (sm_count < 2) return cudaErrorInvalidValue;
-    MxGrad prm = {};
-    prm.rows = rows; prm.n = (int)n; prm.k = (int)k; prm.codes = codes; prm.scales = scales; prm.g = g;
-    prm.code_pitch = mx_code_bytes(8, k); prm.scale_pitch = mx_scale_bytes(k);
-    prm.tiles_n = (int)((n + 255) / 256); prm.tiles_k = (int)((k + 255) / 256);
-    prm.slices = mx_gradient_slices(rows, n, k, sm_count);
-    prm.stages = (int)((rows + MX_ROWS - 1) / MX_ROWS); prm.stages_per_slice = (prm.stages + prm.slices - 1) / prm.slices;
-    prm.out = prm.slices > 1 ? workspace : out; prm.slice_floats = n * k; prm.error_word = error_word;
-    if ((int64_t)prm.tiles_n * prm.tiles_k * prm.slices >= (1ll << 30) || !prm.out) return cudaErrorInvalidValue;
-#define CALL(KIND) launch_mx_weight_gradient<KIND>(s, prm, sm_count)
-    const cudaError_t e = MX_KINDS(dtype, CALL);
+    if (sm_count < 2 || !workspace) return cudaErrorInvalidValue;
+    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, sm_count);
+    const int64_t x_pitch = mx_code_bytes(8, k), units = p.whole_tiles + (int64_t)(p.tiles - p.whole_tiles) * p.slices;
+    if (units >= (1ll << 30)) return cudaErrorInvalidValue;
+    uint16_t *g_planes = (uint16_t *)workspace, *x_plane = (uint16_t *)((uint8_t *)workspace + p.g_bytes);
+    const bool direct = mx_gradient_direct(dtype, n) && ((uintptr_t)g & 15) == 0;
+#define CALL(KIND) launch_mx_pieces<KIND>(s, g, rows, n, p, g_planes, direct, codes, scales, x_pitch, mx_scale_bytes(k), x_plane)
+    cudaError_t e = MX_KINDS(dtype, CALL);
 #undef CALL
-    if (e != cudaSuccess || prm.slices == 1) return e;
-    const int64_t blocks = (n * k / 4 + MX_THREADS) / MX_THREADS;
-    mx_add_slices_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(workspace, prm.slices, n * k, out);
+    if (e != cudaSuccess) return e;
+    CUtensorMap map_g, map_x;
+    if (!make_piece_map(&map_g, direct ? g : g_planes, p.pieces, rows, n, direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
+    MxGrad prm = {};
+    prm.n = (int)n; prm.k = (int)k; prm.rows = rows;
+    prm.tiles_n = p.tiles_n; prm.whole_tiles = p.whole_tiles; prm.units = (int)units;
+    prm.slices = p.slices; prm.stages = p.stages; prm.stages_per_slice = p.stages_per_slice;
+    prm.out = out; prm.partial = (float *)((uint8_t *)workspace + p.g_bytes + p.x_bytes); prm.error_word = error_word;
+    e = p.pieces == 3 ? launch_mx_gradient<3>(s, map_g, map_x, prm, sm_count) : p.pieces == 2 ? launch_mx_gradient<2>(s, map_g, map_x, prm, sm_count) : launch_mx_gradient<1>(s, map_g, map_x, prm, sm_count);
+    if (e != cudaSuccess || p.slices == 1) return e;
+    mx_add_slices_kernel<<<dim3(65536 / 4 / MX_THREADS, (unsigned)(p.tiles - p.whole_tiles)), MX_THREADS, 0, s>>>(prm);
     return cudaGetLastError();
 }
 

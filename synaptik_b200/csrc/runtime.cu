@@ -449,7 +449,7 @@ int32_t prepare_executable(Executable *x) {
                 tiles.ptr = (uint8_t *)p;
             }
         } else if (st.kind == StepKind::MX_WEIGHT_GRADIENT) {
-            workspace_floats = std::max(workspace_floats, kern::mx_weight_gradient_workspace(st.m, st.n, st.k, ctx->sm_count));
+            workspace_floats = std::max(workspace_floats, kern::mx_weight_gradient_workspace(plan.views[st.b].dtype, st.m, st.n, st.k, ctx->sm_count) / 4);
         } else if (st.kind == StepKind::GEMM && st.engine == GemmEngine::NARROW_REDUCE) {
             void *p; if (!alloc((uint64_t)kern::narrow_reduce_partial_floats(st.m, st.n, st.k) * 4, &p)) return ALLOCATION_FAILED;
             se.narrow_partials = (float *)p;
@@ -759,7 +759,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
             case StepKind::MX_WEIGHT_GRADIENT:
                 LAUNCH(kern::mx_weight_gradient(s, plan.views[st.b].dtype, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
                                                 ptr(st.b), (float *)ptr(st.out), x->gemm_workspace, ctx->sm_count, ctx->error_dev));
-                if (kern::mx_weight_gradient_workspace(st.m, st.n, st.k, ctx->sm_count) > 0) x->launches++;
+                x->launches += kern::mx_weight_gradient_launches(plan.views[st.b].dtype, st.m, st.n, st.k, ctx->sm_count) - 1;
                 break;
             case StepKind::MX_ACTIVATION_GRADIENT:
                 LAUNCH(kern::mx_activation_gradient(s, st.act, plan.views[st.b].dtype, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
