@@ -215,15 +215,17 @@ cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const u
                                    int64_t rows, int64_t cols, void *out);
 // out[m, n] = act(x[m, k] . w[n, k]^T + bias[n]), both operands in 4 bits, k a multiple of 32.  Where mx_linear_tiled
 // says so the product runs on two-SM tiles and needs the scales of both operands in tiles (else x_tiles = w_tiles = null).
+// after_x: the launch before this one in the stream was the mx_quantize that makes x; the product may then start early.
 bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count);
 int64_t mx_tile_bytes(int64_t rows, int64_t k);
 cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles);
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
                       const uint8_t *w, const uint8_t *w_scales, const uint8_t *x_tiles, const uint8_t *w_tiles, const void *bias, void *out,
-                      int sm_count, int *error_word);
+                      bool after_x, int sm_count, int *error_word);
 // out[n, k] = sum over rows of g[row, n] * x[row, k], x held in 8 bits, out FLOAT32.  workspace: that many bytes, 256-byte
-// aligned, for the operands in the form the tensor cores read and for sums over slices of the rows.
-int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count);
+// aligned, for the operands in the form the tensor cores read and for sums over slices of the rows (aligned: g starts on
+// a multiple of 16 bytes).
+int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, bool aligned, int sm_count);
 int mx_weight_gradient_launches(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count);
 cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales,
                                const void *g, float *out, void *workspace, int sm_count, int *error_word);

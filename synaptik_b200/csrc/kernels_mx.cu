@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <cstdlib>
+#include <type_traits>
 
 namespace syn {
 namespace kern {
@@ -219,6 +220,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
                                                                  uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles, uint32_t atoms) {
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
     const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the product that reads the codes (see mx_dependent_wait)
     MxSpot<I> at;
     auto fetch = [&](float (&v)[8]) {
         const int count = at.count(r);
@@ -483,6 +485,12 @@ __device__ __forceinline__ void mx_copy_scales(uint32_t dst, int atoms, const ui
 __device__ __forceinline__ void mx_arrive_rank(uint32_t bar, uint32_t rank) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, rank)) : "memory");
 }
+// Programmatic dependent launch: a kernel launched with mx_launch_dependent may start while the one before it still runs,
+// and does what does not depend on it; `wait` returns when that one has finished.  `release` in the earlier kernel lets
+// the later one's blocks in as soon as there is room.  Both do nothing without such a launch.
+__device__ __forceinline__ void mx_dependent_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void mx_dependent_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Waits, for at most a tenth of a second and whatever the abort flag says, for copies whose barrier nothing else arrives on.
 __device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
     const uint64_t start = global_timer();
@@ -513,6 +521,7 @@ struct MxLinear {
     int act;
     int tiles_m, tiles_n, group_n;
     int staged;                         // rows of `out` can be written by TMA
+    int after_x;                        // the launch before this one is the quantisation of x
     int *error_word;
 };
 
@@ -575,11 +584,20 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
             int stage = 0; uint32_t phase = 0;
             int armed = 0;
             bool ok = true;
+            // W does not depend on the launch before this one: its first stages are on their way before x is waited for
+            const int early = kb1 - kb0 < S ? kb1 - kb0 : S;
+            for (int i = 0; i < early; i++) {
+                mbar_expect_tx(full_bar(i), Cfg::kStageBytes);
+                tma_load_2d(smem_base + i * Cfg::kStageBytes, &map_w, full_bar(i), (kb0 + i) * (MX_BK / 2), n0);
+            }
+            mx_dependent_wait();
             for (int kb = kb0; kb < kb1; kb++) {
-                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
                 const uint32_t sa = smem_base + stage * Cfg::kStageBytes;
-                mbar_expect_tx(full_bar(stage), Cfg::kStageBytes);
-                tma_load_2d(sa, &map_w, full_bar(stage), kb * (MX_BK / 2), n0);
+                if (kb - kb0 >= early) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                    mbar_expect_tx(full_bar(stage), Cfg::kStageBytes);
+                    tma_load_2d(sa, &map_w, full_bar(stage), kb * (MX_BK / 2), n0);
+                }
                 tma_load_2d(sa + Cfg::kABytes, &map_x, full_bar(stage), kb * (MX_BK / 2), m0);
                 armed++;
                 if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -613,6 +631,7 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
         const int thread = threadIdx.x - 64;
         int stage = 0; uint32_t phase = 0;
         bool ok = true;
+        mx_dependent_wait();
         auto arrive = [&](int kb) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1033,6 +1052,7 @@ template <int KIND, bool VEC>
 __global__ void __launch_bounds__(MX_THREADS) mx_pieces_kernel(const typename MxElement<KIND>::type *__restrict__ g, int64_t rows, int64_t n, int64_t g_pitch, uint16_t *__restrict__ g_planes, int g_blocks,
                                                                const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int64_t x_pitch, int64_t scale_pitch, uint16_t *__restrict__ x_plane) {
     constexpr int PIECES = KIND == 0 ? 3 : KIND == 1 ? 1 : 2;
+    mx_dependent_release();
     if ((int)blockIdx.x < g_blocks) {
         __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
         const int64_t per_row = g_pitch / 8, total = rows * per_row, hop = (int64_t)g_blocks * MX_THREADS;
@@ -1109,6 +1129,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    mx_dependent_release();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // a unit's tile and stages; every slice has at least one
     auto unit_of = [&](int unit, int &n0, int &k0, int &first, int &count) {
@@ -1127,6 +1148,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
             if (lane == 0) {
+                mx_dependent_wait();        // the operands
                 int stage = 0; uint32_t phase = 0;
                 int armed = 0;
                 bool ok = true;
@@ -1269,8 +1291,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
     }
 }
 
+// Small products (mx_gradient_small): three launches and two-SM tiles would cost more than the work.  A block of 32 warps
+// makes partial sums of 8 n x 32 k results over its share of the rows: a lane per column of x (one block of the
+// checkpoint), the warps take rows in turn, eight at a time in flight.  The warps' FP32 sums are added in a fixed order
+// through shared memory, those of a cluster's blocks, also in order, through the first one's view of theirs.
+constexpr int MX_SMALL_N = 8, MX_SMALL_THREADS = 1024, MX_SMALL_FLIGHT = 8;
+template <int KIND>
+__global__ void __launch_bounds__(MX_SMALL_THREADS) mx_weight_gradient_small_kernel(int64_t rows, int n, int k, const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                                                    int64_t code_pitch, int64_t scale_pitch, const typename MxElement<KIND>::type *__restrict__ g, float *__restrict__ out, int slices) {
+    __shared__ float sums[32][MX_SMALL_N][32];
+    __shared__ float totals[MX_SMALL_N][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int slice = blockIdx.x % slices, block = blockIdx.x / slices, n0 = blockIdx.y * MX_SMALL_N;
+    const int64_t begin = rows * slice / slices, end = rows * (slice + 1) / slices;
+    float sum[MX_SMALL_N] = {};
+    for (int64_t r0 = begin + warp; r0 < end; r0 += MX_SMALL_FLIGHT * 32) {
+        uint32_t code[MX_SMALL_FLIGHT], byte[MX_SMALL_FLIGHT];
+        float up[MX_SMALL_FLIGHT];
+#pragma unroll
+        for (int q = 0; q < MX_SMALL_FLIGHT; q++) {
+            const int64_t row = r0 + q * 32;
+            const bool here = row < end;
+            code[q] = here ? __ldg(codes + row * code_pitch + block * MX_BLOCK + lane) : 0u;
+            byte[q] = here ? __ldg(scales + row * scale_pitch + block) : 0u;
+            up[q] = here && lane < MX_SMALL_N && n0 + lane < n ? mx_load<KIND>(g + row * n + n0 + lane) : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < MX_SMALL_FLIGHT; q++) {
+            float x, unused;
+            mx_decode8x2(code[q], x, unused);
+            x *= mx_scale_value(byte[q]);
+#pragma unroll
+            for (int e = 0; e < MX_SMALL_N; e++) sum[e] = fmaf(__shfl_sync(0xffffffffu, up[q], e), x, sum[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < MX_SMALL_N; e++) sums[warp][e][lane] = sum[e];
+    __syncthreads();
+    if (warp < MX_SMALL_N) {
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 32; w++) total += sums[w][warp][lane];
+        totals[warp][lane] = total;
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (slice == 0 && warp < MX_SMALL_N) {
+        float total = totals[warp][lane];
+        for (int q = 1; q < slices; q++) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(smem_u32(&totals[warp][lane]), (uint32_t)q)) : "memory");
+            total += v;
+        }
+        const int col = block * MX_BLOCK + lane;
+        if (n0 + warp < n && col < k) out[(int64_t)(n0 + warp) * k + col] = total;
+    }
+    __syncwarp();
+    cluster_sync_all();         // no block leaves while another reads its sums
+}
+
 // The tiles that were cut into slices: their sums in ascending order.  blockIdx.y: the tile; a thread adds four columns.
 __global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(MxGrad prm) {
+    mx_dependent_wait();
     const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * 256;
     const int i = blockIdx.x * MX_THREADS + threadIdx.x, row = i >> 6, col = (i & 63) * 4;
     if (n0 + row >= prm.n || k0 + col >= prm.k) return;
@@ -1306,6 +1388,18 @@ static cudaError_t mx_prepare_kernel(Kernel kernel, int smem, int least_regs, st
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
     return e;
+}
+
+// A launch that may overlap the end of the one before it (see mx_dependent_wait).
+template <typename... Args>
+static cudaError_t mx_launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t s, std::common_type_t<Args>... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 #define MX_KINDS(dtype, CALL) ((dtype) == DType::F32 ? CALL(0) : (dtype) == DType::BF16 ? CALL(1) : (dtype) == DType::F16 ? CALL(2) : cudaErrorInvalidValue)
@@ -1442,10 +1536,12 @@ static cudaError_t launch_mx_few(cudaStream_t s, const uint8_t *x, const uint8_t
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = Cfg::kSmemBytes;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {(unsigned)slices, 1, 1};
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = prm.after_x ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, mx_linear_few_kernel<BN, KIND>, map_w, map_x, prm, slices);
 }
 
@@ -1487,10 +1583,13 @@ static int forced_mx_pair() {
     return v;
 }
 
+// Two-SM tiles where the one-SM tiles of 128 x 128 would take more than one wave: measured with the quantisation of x, K =
+// 4096: 512 x 4096 (128 tiles) 34.6 us on one-SM tiles and 32.8 on two-SM ones, 4096 x 128 (32) 31.9 and 41.4, 1024 x 4096
+// (256) 60.6 and 34.2, 1 x 4096 15.4 and 29.7.
 bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count) {
     if (sm_count < 2) return false;
     if (forced_mx_pair() >= 0) return forced_mx_pair() == 1;
-    return m > 256;
+    return m > 128 && ((m + 127) / 128) * ((n + 127) / 128) > sm_count;
 }
 int64_t mx_tile_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * mx_tile_atoms(k) * MX_ATOM; }
 cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles) {
@@ -1521,9 +1620,10 @@ static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint
 
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,
                       const uint8_t *w, const uint8_t *w_scales, const uint8_t *x_tiles, const uint8_t *w_tiles, const void *bias, void *out,
-                      int sm_count, int *error_word) {
+                      bool after_x, int sm_count, int *error_word) {
     if (m == 0 || n == 0) return cudaSuccess;
     MxLinear prm = {};
+    prm.after_x = after_x ? 1 : 0;
     prm.m = (int)m; prm.n = (int)n; prm.blocks = (int)(k / MX_BLOCK); prm.k_blocks = (int)((k + MX_BK - 1) / MX_BK);
     prm.scale_pitch = mx_scale_bytes(k); prm.xs = x_scales; prm.ws = w_scales;
     prm.bias = bias; prm.out = out; prm.act = act; prm.error_word = error_word;
@@ -1532,12 +1632,42 @@ cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n
 #undef CALL
 }
 
+// Slices of the rows for the plain kernel: at least one pass of all warps each.
+static int mx_small_slices(int64_t rows) {
+    int s = 1;
+    while (s < 8 && rows >= (int64_t)s * 2 * MX_SMALL_FLIGHT * 32) s *= 2;
+    return s;
+}
+// Where the plain kernel is the faster one: its blocks get an SM each and its warps pass over the rows once or twice.
+// Measured, FLOAT32: 1024 x 32 x 128 (64 blocks) 15.4 us against 21.5 us on tiles, 1024 x 128 x 128 (256) 21.6 and 21.3,
+// 65536 x 32 x 32 (32 blocks, 32 passes) 99 and 43.
+static bool mx_gradient_small(int64_t rows, int64_t n, int64_t k, int sm_count) {
+    const int64_t s = mx_small_slices(rows), blocks = mx_blocks(k) * ((n + MX_SMALL_N - 1) / MX_SMALL_N) * s;
+    return rows > 0 && blocks <= sm_count && rows <= 2 * s * MX_SMALL_FLIGHT * 32;
+}
+
+template <int KIND>
+static cudaError_t launch_mx_gradient_small(cudaStream_t s, int64_t rows, int64_t n, int64_t k, const uint8_t *codes, const uint8_t *scales, const void *g, float *out) {
+    using T = typename MxElement<KIND>::type;
+    const int slices = mx_small_slices(rows);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(mx_blocks(k) * slices), (unsigned)((n + MX_SMALL_N - 1) / MX_SMALL_N));
+    cfg.blockDim = dim3(MX_SMALL_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)slices, 1, 1};
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, mx_weight_gradient_small_kernel<KIND>, rows, (int)n, (int)k, codes, scales, mx_code_bytes(8, k), mx_scale_bytes(k), (const T *)g, out, slices);
+}
+
 // How the tiles are spread over the block pairs, and what scratch that takes.
 struct MxGradPlan {
     int pieces, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
+    bool direct;                        // BFLOAT16 rows that TMA can address are read where they are
     int64_t g_pitch, g_bytes, x_bytes, partial_bytes;       // of the planes and partial sums, each a multiple of 256
 };
-static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
+static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t k, bool aligned, int sm_count) {
     MxGradPlan p = {};
     p.pieces = dtype == DType::F32 ? 3 : dtype == DType::BF16 ? 1 : 2;
     p.tiles_n = (int)((n + 255) / 256); p.tiles = p.tiles_n * (int)((k + 255) / 256);
@@ -1559,21 +1689,20 @@ static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t
     p.stages_per_slice = p.stages > 0 ? (p.stages + p.slices - 1) / p.slices : 0;
     const auto rounded = [](int64_t bytes) { return (bytes + 255) / 256 * 256; };
     p.g_pitch = (n + 7) / 8 * 8;
-    p.g_bytes = rounded(p.pieces * rows * p.g_pitch * 2);
+    p.direct = dtype == DType::BF16 && n % 8 == 0 && aligned;
+    p.g_bytes = p.direct ? 0 : rounded(p.pieces * rows * p.g_pitch * 2);
     p.x_bytes = rounded(rows * mx_code_bytes(8, k) * 2);
     p.partial_bytes = p.slices > 1 ? (int64_t)left * p.slices * 65536 * 4 : 0;
     return p;
 }
 
-// BFLOAT16 rows that TMA can address are read where they are.
-static bool mx_gradient_direct(DType dtype, int64_t n) { return dtype == DType::BF16 && n % 8 == 0; }
-
-int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
-    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, sm_count);
+int64_t mx_weight_gradient_workspace(DType dtype, int64_t rows, int64_t n, int64_t k, bool aligned, int sm_count) {
+    if (mx_gradient_small(rows, n, k, sm_count)) return 0;
+    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, aligned, sm_count);
     return p.g_bytes + p.x_bytes + p.partial_bytes;
 }
 int mx_weight_gradient_launches(DType dtype, int64_t rows, int64_t n, int64_t k, int sm_count) {
-    return rows == 0 ? 1 : mx_gradient_plan(dtype, rows, n, k, sm_count).slices > 1 ? 3 : 2;
+    return rows == 0 || mx_gradient_small(rows, n, k, sm_count) ? 1 : mx_gradient_plan(dtype, rows, n, k, true, sm_count).slices > 1 ? 3 : 2;
 }
 
 // Tensor map over BFLOAT16 planes [planes][rows][pitch] of `cols` columns: boxes of 64 columns x 64 rows, 128-byte swizzle.
@@ -1596,16 +1725,15 @@ static cudaError_t launch_mx_gradient(cudaStream_t s, const CUtensorMap &map_g, 
     cudaError_t e = mx_prepare_kernel(mx_weight_gradient_kernel<PIECES>, Cfg::kSmemBytes, (72 + 2 * 216 + 2) / 3, done);
     if (e != cudaSuccess) return e;
     const int pairs = sm_count / 2;
-    mx_weight_gradient_kernel<PIECES><<<2 * (prm.units < pairs ? prm.units : pairs), MX_GRAD_THREADS, Cfg::kSmemBytes, s>>>(map_g, map_x, prm);
-    return cudaGetLastError();
+    return mx_launch_dependent(mx_weight_gradient_kernel<PIECES>, dim3((unsigned)(2 * (prm.units < pairs ? prm.units : pairs))), MX_GRAD_THREADS, Cfg::kSmemBytes, s, map_g, map_x, prm);
 }
 
 template <int KIND>
-static cudaError_t launch_mx_pieces(cudaStream_t s, const void *g, int64_t rows, int64_t n, const MxGradPlan &p, uint16_t *g_planes, bool direct,
+static cudaError_t launch_mx_pieces(cudaStream_t s, const void *g, int64_t rows, int64_t n, const MxGradPlan &p, uint16_t *g_planes,
                                     const uint8_t *codes, const uint8_t *scales, int64_t x_pitch, int64_t scale_pitch, uint16_t *x_plane) {
     using T = typename MxElement<KIND>::type;
     // blocks in proportion to the bytes moved
-    const int64_t g_work = direct ? 0 : rows * p.g_pitch / 8, x_work = rows * x_pitch / 8;
+    const int64_t g_work = p.direct ? 0 : rows * p.g_pitch / 8, x_work = rows * x_pitch / 8;
     const int64_t most = 148 * 8;
     const double share = (double)g_work * (sizeof(T) + 2.0 * p.pieces) / ((double)g_work * (sizeof(T) + 2.0 * p.pieces) + (double)x_work * 3.0);
     const auto blocks = [&](int64_t work, double part) {
@@ -1623,18 +1751,22 @@ cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_
                                const void *g, float *out, void *workspace, int sm_count, int *error_word) {
     if (n == 0 || k == 0) return cudaSuccess;
     if (rows == 0) return cudaMemsetAsync(out, 0, (size_t)n * k * 4, s);
+    if (mx_gradient_small(rows, n, k, sm_count)) {
+#define CALL(KIND) launch_mx_gradient_small<KIND>(s, rows, n, k, codes, scales, g, out)
+        return MX_KINDS(dtype, CALL);
+#undef CALL
+    }
     if (sm_count < 2 || !workspace) return cudaErrorInvalidValue;
-    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, sm_count);
+    const MxGradPlan p = mx_gradient_plan(dtype, rows, n, k, ((uintptr_t)g & 15) == 0, sm_count);
     const int64_t x_pitch = mx_code_bytes(8, k), units = p.whole_tiles + (int64_t)(p.tiles - p.whole_tiles) * p.slices;
     if (units >= (1ll << 30)) return cudaErrorInvalidValue;
     uint16_t *g_planes = (uint16_t *)workspace, *x_plane = (uint16_t *)((uint8_t *)workspace + p.g_bytes);
-    const bool direct = mx_gradient_direct(dtype, n) && ((uintptr_t)g & 15) == 0;
-#define CALL(KIND) launch_mx_pieces<KIND>(s, g, rows, n, p, g_planes, direct, codes, scales, x_pitch, mx_scale_bytes(k), x_plane)
+#define CALL(KIND) launch_mx_pieces<KIND>(s, g, rows, n, p, g_planes, codes, scales, x_pitch, mx_scale_bytes(k), x_plane)
     cudaError_t e = MX_KINDS(dtype, CALL);
 #undef CALL
     if (e != cudaSuccess) return e;
     CUtensorMap map_g, map_x;
-    if (!make_piece_map(&map_g, direct ? g : g_planes, p.pieces, rows, n, direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
+    if (!make_piece_map(&map_g, p.direct ? g : g_planes, p.pieces, rows, n, p.direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
     MxGrad prm = {};
     prm.n = (int)n; prm.k = (int)k; prm.rows = rows;
     prm.tiles_n = p.tiles_n; prm.whole_tiles = p.whole_tiles; prm.units = (int)units;
@@ -1642,8 +1774,7 @@ cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_
     prm.out = out; prm.partial = (float *)((uint8_t *)workspace + p.g_bytes + p.x_bytes); prm.error_word = error_word;
     e = p.pieces == 3 ? launch_mx_gradient<3>(s, map_g, map_x, prm, sm_count) : p.pieces == 2 ? launch_mx_gradient<2>(s, map_g, map_x, prm, sm_count) : launch_mx_gradient<1>(s, map_g, map_x, prm, sm_count);
     if (e != cudaSuccess || p.slices == 1) return e;
-    mx_add_slices_kernel<<<dim3(65536 / 4 / MX_THREADS, (unsigned)(p.tiles - p.whole_tiles)), MX_THREADS, 0, s>>>(prm);
-    return cudaGetLastError();
+    return mx_launch_dependent(mx_add_slices_kernel, dim3(65536 / 4 / MX_THREADS, (unsigned)(p.tiles - p.whole_tiles)), MX_THREADS, 0, s, prm);
 }
 
 }  // namespace kern

@@ -449,7 +449,7 @@ int32_t prepare_executable(Executable *x) {
                 tiles.ptr = (uint8_t *)p;
             }
         } else if (st.kind == StepKind::MX_WEIGHT_GRADIENT) {
-            workspace_floats = std::max(workspace_floats, kern::mx_weight_gradient_workspace(plan.views[st.b].dtype, st.m, st.n, st.k, ctx->sm_count) / 4);
+            workspace_floats = std::max(workspace_floats, kern::mx_weight_gradient_workspace(plan.views[st.b].dtype, st.m, st.n, st.k, plan.views[st.b].offset * dtype_bytes(plan.views[st.b].dtype) % 16 == 0, ctx->sm_count) / 4);
         } else if (st.kind == StepKind::GEMM && st.engine == GemmEngine::NARROW_REDUCE) {
             void *p; if (!alloc((uint64_t)kern::narrow_reduce_partial_floats(st.m, st.n, st.k) * 4, &p)) return ALLOCATION_FAILED;
             se.narrow_partials = (float *)p;
@@ -741,6 +741,10 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 break;
             case StepKind::MX_LINEAR: {
                 const uint8_t *tiles[2] = {nullptr, nullptr};
+                // nothing else may come between, and W must not be what that launch makes
+                const Step *before = i > 0 ? &plan.steps[i - 1] : nullptr;
+                const bool after_x = before && before->kind == StepKind::MX_QUANTIZE && before->m > 0 && before->out == st.a && before->out2 == st.scale_a
+                                     && st.b != st.a && st.scale_b != st.scale_a && !time_steps && !x->comm;
                 for (int operand = 0; operand < 2; operand++) {
                     const int value = operand ? st.scale_b : st.scale_a;
                     auto it = x->mx_tiles.find(value);
@@ -753,7 +757,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 }
                 LAUNCH(kern::mx_linear(s, plan.views[st.out].dtype, st.act, st.m, st.n, st.k, (const uint8_t *)ptr(st.a), (const uint8_t *)ptr(st.scale_a),
                                        (const uint8_t *)ptr(st.b), (const uint8_t *)ptr(st.scale_b), tiles[0], tiles[1], ptr(st.bias), ptr(st.out),
-                                       ctx->sm_count, ctx->error_dev));
+                                       after_x, ctx->sm_count, ctx->error_dev));
                 break;
             }
             case StepKind::MX_WEIGHT_GRADIENT:
