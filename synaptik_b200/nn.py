@@ -67,14 +67,20 @@ class Model:
 
     def __init__(self, dims: Sequence[int], context: native.Context | None = None, seed: int = 0,
                  comm: native.Comm | None = None, world_size: int = 1, bias: bool = True, activation: str = "relu",
-                 dtype: str = "f32"):
+                 dtype: str = "f32", checkpoints: str | None = None):
         if activation not in ("relu", "tanh", "sigmoid", "silu", "gelu_tanh", "gelu"):
             raise ValueError("activation must be 'relu', 'tanh', 'sigmoid', 'silu', 'gelu_tanh' or 'gelu'")
-        if dtype not in ("f32", "bf16", "f16"):
-            raise ValueError("dtype must be 'f32', 'bf16' or 'f16'")
+        if dtype not in ("f32", "bf16", "f16", "mx4"):
+            raise ValueError("dtype must be 'f32', 'bf16', 'f16' or 'mx4'")
+        if checkpoints not in (None, "mx8"):
+            raise ValueError("checkpoints must be None or 'mx8'")
         # 16-bit storage (DataType.BFLOAT16 / FLOAT16): parameters, input and output are held as 16-bit values,
-        # every node computes in FLOAT32 and narrows once; inference only (compute)
+        # every node computes in FLOAT32 and narrows once; inference only (compute).  "mx4": weights in 4 bits with a scale
+        # per 32 inputs, biases, input and output BFLOAT16; every layer quantises its input too; inference only
         self.dtype = dtype
+        self.storage = "bf16" if dtype == "mx4" else dtype
+        # "mx8": training keeps the layers' inputs for the backward pass in 8 bits instead of FLOAT32
+        self.checkpoints = checkpoints
         self.dims = list(dims)
         self.bias = bias
         self.activation = activation
@@ -89,7 +95,8 @@ class Model:
             w = glorot_uniform(rng, self.dims[l + 1], self.dims[l])
             b = np.zeros(self.dims[l + 1], dtype=np.float32)
             for array in ((w, b) if bias else (w,)):
-                self.param_buffers.append(self.context.upload(program.to_storage(self.dtype, array)))
+                self.param_buffers.append(self._mx_upload(array) if dtype == "mx4" and array.ndim == 2 else
+                                          self.context.upload(program.to_storage(self.storage, array)))
                 self.param_shapes.append(array.shape)
         self._inference = {}
         self._training = {}
@@ -98,8 +105,45 @@ class Model:
         self._optimizer = None
 
     # ---- parameters -----------------------------------------------------------------------
+    def _run_once(self, graph: program.GraphBuilder, inputs, outputs) -> None:
+        exe = native.Executable(self.context, graph.build())
+        try:
+            exe.run(inputs, outputs)
+        finally:
+            exe.close()
+
+    def _mx_upload(self, array: np.ndarray, into=None):
+        """A weight quantised to 4 bits on the device: its (codes, scales) buffers."""
+        g = program.GraphBuilder()
+        held = g.mx_quantize(g.feed(program.F32, array.shape), "mx4")
+        g.publish(held.codes)
+        g.publish(held.scales)
+        out = into or (self.context.buffer(held.codes.nbytes), self.context.buffer(held.scales.nbytes))
+        source = self.context.upload(np.ascontiguousarray(array, dtype=np.float32))
+        try:
+            self._run_once(g, [source], list(out))
+        finally:
+            source.close()
+        return out
+
+    def _mx_download(self, held, shape) -> np.ndarray:
+        g = program.GraphBuilder()
+        g.publish(g.mx_restore(g.mx_feed("mx4", shape)))
+        out = self.context.buffer(int(np.prod(shape)) * 4)
+        try:
+            self._run_once(g, list(held), [out])
+            return out.download(np.float32, shape)
+        finally:
+            out.close()
+
+    def _parameter_feeds(self) -> List[native.Buffer]:
+        return [b for held in self.param_buffers for b in (held if isinstance(held, tuple) else (held,))]
+
     def parameters(self) -> List[np.ndarray]:
-        """The parameters as FLOAT32 arrays (exactly the stored values, also for 16-bit storage)."""
+        """The parameters as FLOAT32 arrays (exactly the stored values, also for 16-bit and 4-bit storage)."""
+        if self.dtype == "mx4":
+            return [self._mx_download(b, s) if isinstance(b, tuple) else program.from_storage("bf16", b.download(np.uint16, s))
+                    for b, s in zip(self.param_buffers, self.param_shapes)]
         if self.dtype != "f32":
             return [program.from_storage(self.dtype, b.download(np.uint16, s)) for b, s in zip(self.param_buffers, self.param_shapes)]
         return [b.download(np.float32, s) for b, s in zip(self.param_buffers, self.param_shapes)]
@@ -109,14 +153,20 @@ class Model:
             array = np.ascontiguousarray(array, dtype=np.float32)
             if array.shape != tuple(shape):
                 raise ValueError(f"parameter shape {array.shape} != {shape}")
-            buf.upload(program.to_storage(self.dtype, array))
+            if isinstance(buf, tuple):
+                self._mx_upload(array, buf)
+            else:
+                buf.upload(program.to_storage(self.storage, array))
 
     # ---- inference ------------------------------------------------------------------------
     def _inference_state(self, lead, arg_max: bool):
         key = (tuple(lead), arg_max)
         if key not in self._inference:
-            graph = program.mlp_inference_graph(self.dims, tuple(lead), arg_max, bias=self.bias, activation=self.activation,
-                                                dtype=program.STORAGE_DTYPES[self.dtype])
+            if self.dtype == "mx4":
+                graph = program.mlp_mx_inference_graph(self.dims, tuple(lead), arg_max, bias=self.bias, activation=self.activation)
+            else:
+                graph = program.mlp_inference_graph(self.dims, tuple(lead), arg_max, bias=self.bias, activation=self.activation,
+                                                    dtype=program.STORAGE_DTYPES[self.dtype])
             exe = native.Executable(self.context, graph.image)
             batch = int(np.prod(lead))
             width = 4 if self.dtype == "f32" else 2
@@ -134,10 +184,10 @@ class Model:
         if x.ndim < 2 or x.shape[-1] != self.dims[0]:
             raise ValueError(f"input shape {x.shape} does not end in {self.dims[0]} features")
         exe, xbuf, outs = self._inference_state(x.shape[:-1], arg_max)
-        xbuf.upload(program.to_storage(self.dtype, x))
-        exe.run([xbuf] + self.param_buffers, outs)
+        xbuf.upload(program.to_storage(self.storage, x))
+        exe.run([xbuf] + self._parameter_feeds(), outs)
         if self.dtype != "f32":
-            result = program.from_storage(self.dtype, outs[0].download(np.uint16, tuple(x.shape[:-1]) + (self.dims[-1],)))
+            result = program.from_storage(self.storage, outs[0].download(np.uint16, tuple(x.shape[:-1]) + (self.dims[-1],)))
         else:
             result = outs[0].download(np.float32, tuple(x.shape[:-1]) + (self.dims[-1],))
         if arg_max:
@@ -163,7 +213,8 @@ class Model:
         if self._loss is None:
             raise RuntimeError("configure_training first")
         if batch not in self._training:
-            graph = program.mlp_training_graph(self.dims, batch, self._loss, bias=self.bias, activation=self.activation)
+            graph = program.mlp_training_graph(self.dims, batch, self._loss, bias=self.bias, activation=self.activation,
+                                               checkpoints=self.checkpoints)
             exe = native.Executable(self.context, graph.image)
             x = self.context.buffer(batch * self.dims[0] * 4)
             t = self.context.buffer(batch * 4 if self._loss == "ce" else batch * self.dims[-1] * 4)

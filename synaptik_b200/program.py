@@ -599,11 +599,47 @@ def mlp_inference_graph(dims: Sequence[int], batch, arg_max: bool = False, bias:
     return MlpGraph(g.build(), names, pubs, shapes)
 
 
+def mlp_mx_inference_graph(dims: Sequence[int], batch, arg_max: bool = False, bias: bool = True, activation: str = "relu") -> MlpGraph:
+    """Model.compute of a Linear/activation stack with weights in 4 bits ("mx4"): feeds x, then (codes, scales, b) per
+    layer; x, biases and output BFLOAT16.  Every layer quantises its input and multiplies 4-bit operands (MX_QUANTIZE,
+    MX_LINEAR with bias and activation); the values between the layers are BFLOAT16."""
+    g = GraphBuilder()
+    lead = tuple(batch) if isinstance(batch, (tuple, list)) else (int(batch),)
+    if arg_max and len(lead) != 1:
+        raise ValueError("row arg-max needs a [batch, features] input")
+    a = g.feed(BF16, lead + (dims[0],))
+    names, shapes = ["x"], {"x": a.shape}
+    params = []
+    for l in range(len(dims) - 1):
+        w = g.mx_feed("mx4", (dims[l + 1], dims[l]))
+        b = g.feed(BF16, (dims[l + 1],)) if bias else None
+        for name, value in [(f"w{l}.codes", w.codes), (f"w{l}.scales", w.scales)] + ([(f"b{l}", b)] if bias else []):
+            names.append(name)
+            shapes[name] = value.shape
+        params.append((w, b))
+    for l, (w, b) in enumerate(params):
+        a = g.mx_linear(g.mx_quantize(a, "mx4"), w, b, activation if l + 2 < len(dims) else None, BF16)
+    g.publish(a)
+    pubs = ["output"]
+    shapes["output"] = a.shape
+    if arg_max:
+        g.publish(g.arg_max(a, 1))
+        pubs.append("arg_max")
+        shapes["arg_max"] = (lead[0],)
+    return MlpGraph(g.build(), names, pubs, shapes)
+
+
 def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_dtype: int = I32, bias: bool = True,
-                       publish_activations: bool = False, activation: str = "relu") -> MlpGraph:
+                       publish_activations: bool = False, activation: str = "relu", checkpoints: str | None = None) -> MlpGraph:
     """The TRAINING_STEP graph TrainingSession compiles: forward, objective, and one gradient per
     parameter in trainingParameters() order (weight, bias per layer), published after the loss
-    (TrainingSession.java:953-987).  Feeds: x, target, seed, then (w, b) per layer."""
+    (TrainingSession.java:953-987).  Feeds: x, target, seed, then (w, b) per layer.
+
+    ``checkpoints="mx8"`` (no counterpart in the reference): the backward pass reads the layers' inputs, and the
+    pre-activations of activations other than ReLU, from 8-bit checkpoints taken in the forward pass, so nothing keeps
+    the FLOAT32 tensors; the forward pass and the objective are the same."""
+    if checkpoints not in (None, "mx8"):
+        raise ValueError("checkpoints must be None or 'mx8'")
     g = GraphBuilder()
     layers = len(dims) - 1
     x = g.feed(F32, (batch, dims[0]))
@@ -623,12 +659,17 @@ def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_
             shapes[f"b{l}"] = b.shape
         params.append((w, b))
     acts, zs, wts = [x], [], []
+    held_inputs, held_zs = [], []       # 8-bit checkpoints, where asked for
     a = x
     for l, (w, b) in enumerate(params):
+        if checkpoints:
+            held_inputs.append(g.mx_quantize(a, checkpoints))
         wt, z = g.linear(a, w, b)
         wts.append(wt)
         zs.append(z)
         a = g.activation(activation, z) if l + 1 < layers else z
+        if checkpoints:
+            held_zs.append(g.mx_quantize(z, checkpoints) if activation != "relu" and l + 1 < layers else None)
         acts.append(a)
     if loss == "ce":
         objective = g.index_cross_entropy(a, target)
@@ -639,9 +680,16 @@ def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_
     g.publish(objective)
     grads = [None] * (2 * layers)
     for l in range(layers - 1, -1, -1):
-        dx, dw, db = g.linear_backward(acts[l], wts[l], dz, need_dx=l > 0, bias=bias)
+        if checkpoints:
+            dw = g.mx_weight_gradient(held_inputs[l], dz)
+            db = g.sum_to_shape(dz, (dz.shape[1],)) if bias else None
+            dx = g.matmul(dz, g.permute(wts[l], (1, 0))) if l > 0 else None
+        else:
+            dx, dw, db = g.linear_backward(acts[l], wts[l], dz, need_dx=l > 0, bias=bias)
         grads[2 * l], grads[2 * l + 1] = dw, db
-        if l > 0:
+        if l > 0 and checkpoints:       # a ReLU's own output is positive exactly where its input is
+            dz = g.mx_activation_gradient(activation, held_inputs[l] if activation == "relu" else held_zs[l - 1], dx)
+        elif l > 0:
             dz = g.activation_backward(activation, zs[l - 1], acts[l], dx)
     pubs = ["loss"]
     shapes["loss"] = ()

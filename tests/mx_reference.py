@@ -4,7 +4,7 @@ import math
 
 import numpy as np
 
-import helpers
+import helpers  # noqa: F401
 from synaptik_b200 import program
 from synaptik_b200.program import BF16, F16, F32
 
