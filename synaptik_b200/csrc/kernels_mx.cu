@@ -17,6 +17,12 @@ namespace {
 constexpr int MX_THREADS = 256;
 constexpr int MX_WARPS = MX_THREADS / 32;
 
+// Programmatic dependent launch: a kernel launched with mx_launch_dependent may start while the one before it still runs,
+// and does what does not depend on it; `wait` returns when that one has finished.  `release` in the earlier kernel lets
+// the later one's blocks in as soon as there is room.  Both do nothing without such a launch.
+__device__ __forceinline__ void mx_dependent_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void mx_dependent_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Storage type of a floating tensor: 0 FLOAT32, 1 BFLOAT16, 2 FLOAT16 (the KIND of lowp.cuh).
 template <int KIND> struct MxElement { using type = uint16_t; };
 template <> struct MxElement<0> { using type = float; };
@@ -32,9 +38,9 @@ template <int KIND> __device__ __forceinline__ typename MxElement<KIND>::type mx
 // bytes of the wide tensor per thread and access, the block's largest magnitude by two shuffles.  A row has
 // `per_row` groups, counted over the padded scales (a multiple of 16), so a block never straddles two warps.
 // ------------------------------------------------------------------------------------------------
-// I: int64_t, or uint32_t where the groups of the whole tensor, and a step beyond them, can be counted with it.
+// Groups of `group` elements (8, or 16 where that is said).  I: int64_t, or uint32_t where the groups of the whole tensor, and a step beyond them, can be counted with it.
 template <typename I> struct MxRows {
-    I rows, per_row, total;         // groups of 8 per row and in all
+    I rows, per_row, total;         // groups per row and in all
     I whole, rest;                  // whole groups of a row, columns of the one that is left
     I blocks;                       // blocks of a row that exist
     I hop, hop_rows, hop_groups;    // groups from one step of a thread to its next: in all, in whole rows, and the rest
@@ -45,11 +51,11 @@ inline int mx_grid(int64_t total) {
     const int64_t blocks = (total + MX_THREADS - 1) / MX_THREADS;
     return (int)(blocks < 148 * 8 ? (blocks < 1 ? 1 : blocks) : 148 * 8);
 }
-template <typename I> inline MxRows<I> mx_rows(int64_t rows, int64_t cols, int format) {
-    const int64_t per_row = mx_scale_bytes(cols) * 4, hop = (int64_t)mx_grid(rows * per_row) * MX_THREADS;
+template <typename I> inline MxRows<I> mx_rows(int64_t rows, int64_t cols, int format, int group = 8) {
+    const int64_t per_row = mx_scale_bytes(cols) * (MX_BLOCK / group), hop = (int64_t)mx_grid(rows * per_row) * MX_THREADS;
     MxRows<I> r;
     r.rows = (I)rows; r.per_row = (I)per_row; r.total = (I)(rows * per_row);
-    r.whole = (I)(cols / 8); r.rest = (I)(cols % 8); r.blocks = (I)mx_blocks(cols);
+    r.whole = (I)(cols / group); r.rest = (I)(cols % group); r.blocks = (I)mx_blocks(cols);
     r.hop = (I)hop; r.hop_rows = (I)(hop / per_row); r.hop_groups = (I)(hop % per_row);
     // a single row never multiplies by its pitch
     r.code_pitch = rows > 1 ? (uint32_t)mx_code_bytes(format, cols) : 0u; r.scale_pitch = rows > 1 ? (uint32_t)mx_scale_bytes(cols) : 0u;
@@ -72,9 +78,9 @@ template <typename I> struct MxSpot {
         if (group >= r.per_row) { group -= r.per_row; row++; }
     }
     __device__ __forceinline__ bool in(const MxRows<I> &r) const { return (g & ~(I)31) < r.total; }
-    __device__ __forceinline__ int count(const MxRows<I> &r) const { return g >= r.total ? 0 : group < r.whole ? 8 : group == r.whole ? (int)r.rest : 0; }
+    template <int E = 8> __device__ __forceinline__ int count(const MxRows<I> &r) const { return g >= r.total ? 0 : group < r.whole ? E : group == r.whole ? (int)r.rest : 0; }
     // of this group's first element in rows `pitch` elements apart
-    __device__ __forceinline__ int64_t offset(int64_t pitch) const { return (int64_t)row * pitch + (int64_t)group * 8; }
+    template <int E = 8> __device__ __forceinline__ int64_t offset(int64_t pitch) const { return (int64_t)row * pitch + (int64_t)group * E; }
 };
 
 // Eight elements from memory aligned to their size (32 or 16 bytes).
@@ -106,6 +112,15 @@ template <int KIND> __device__ __forceinline__ void mx_store8(typename MxElement
         }
         *reinterpret_cast<uint4 *>(p) = make_uint4(u[0], u[1], u[2], u[3]);
     }
+}
+
+// Sixteen elements of a 16-bit type from memory aligned to 32 bytes.
+template <int KIND> __device__ __forceinline__ void mx_load16(const uint16_t *p, float (&v)[16]) {
+    uint32_t u[8];
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "l"(p));
+#pragma unroll
+    for (int i = 0; i < 8; i++) { v[2 * i] = low_decode<KIND>((uint16_t)(u[i] & 0xffffu)); v[2 * i + 1] = low_decode<KIND>((uint16_t)(u[i] >> 16)); }
 }
 
 // Rows that do not start on such an address: the warp reads (writes) its 256 elements 32 consecutive ones at a time and
@@ -213,23 +228,26 @@ __global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_
     }
 }
 
-// x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.  Positions in 32 bits
-// where they fit: with 64-bit ones the 16-bit types were bound by the instructions of their addresses.
+// x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.  A thread takes 32 aligned
+// bytes (8 FLOAT32 or 16 16-bit elements) where rows allow, 8 elements through shared memory elsewhere.  Positions in 32
+// bits where they fit: with 64-bit ones and 8 elements the 16-bit types were bound by the instructions around them.
 template <int FORMAT, int KIND, bool VEC, typename I>
 __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows<I> r, int64_t row_step, int even,
                                                                  uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles, uint32_t atoms) {
+    constexpr int E = VEC && KIND != 0 ? 16 : 8, LANES = MX_BLOCK / E;      // lanes per block
     __shared__ float boxes[VEC ? 1 : MX_WARPS][VEC ? 1 : 256];
     const int lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the product that reads the codes (see mx_dependent_wait)
+    mx_dependent_release();             // the product that reads the codes
     MxSpot<I> at;
-    auto fetch = [&](float (&v)[8]) {
-        const int count = at.count(r);
+    auto fetch = [&](float (&v)[E]) {
+        const int count = at.template count<E>(r);
         if constexpr (VEC) {
-            const auto *p = x + at.offset(row_step);
-            if (count == 8) mx_load8<KIND>(p, v);
-            else {
+            const auto *p = x + at.template offset<E>(row_step);
+            if (count == E) {
+                if constexpr (E == 16) mx_load16<KIND>(p, v); else mx_load8<KIND>(p, v);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = i < count ? mx_load<KIND>(p + i) : 0.0f;
+                for (int i = 0; i < E; i++) v[i] = i < count ? mx_load<KIND>(p + i) : 0.0f;
             }
         } else {
             int64_t base = (int64_t)at.row * row_step;
@@ -240,47 +258,51 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
             mx_gather8<KIND>(x, base + (int64_t)at.group * 8 * ix.sa[3], ix.sa[3], count, boxes[threadIdx.x >> 5], lane, v);
         }
     };
-    float ahead[8];
+    float ahead[E];
     at.start(r);
     if (at.in(r)) fetch(ahead);
     while (at.in(r)) {
-        float v[8];
+        float v[E];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = ahead[i];
+        for (int i = 0; i < E; i++) v[i] = ahead[i];
         const I row = at.row, group = at.group;
         const bool mine = at.g < r.total;
         at.next(r);
         if (at.in(r)) fetch(ahead);         // in flight while this group is worked on
         float most = 0.0f;                  // NaN if any is
 #pragma unroll
-        for (int i = 0; i < 8; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[i])));
+        for (int i = 0; i < E; i++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(v[i])));
         uint32_t largest = __float_as_uint(most);       // bit patterns of magnitudes order like the magnitudes, NaN above infinity
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, d));
         if (!mine) continue;
-        const I block = group >> 2;
+        const I block = group / LANES;
         const bool exists = block < r.blocks;       // else: padding of the scales
         const uint32_t byte = exists ? mx_scale_byte<FORMAT>(largest) : 0u;
-        if ((lane & 3) == 0) {
+        if (lane % LANES == 0) {
             scales[(int64_t)row * r.scale_pitch + block] = (uint8_t)byte;
             if (tiles) tiles[mx_tile_offset(row, block, atoms)] = (uint8_t)byte;
         }
         if (!exists) continue;
         if (byte == 255u) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0.0f;
+            for (int i = 0; i < E; i++) v[i] = 0.0f;
         }
         // the inverse scale 2^(127 - byte) is a normal number for every other byte that occurs; a product with it is
         // exact, or below half the smallest element
         const float inverse = byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= inverse;
-        uint8_t *dst = codes + (int64_t)row * r.code_pitch + (int64_t)group * FORMAT;
-        if constexpr (FORMAT == 4) {
-            *reinterpret_cast<uint32_t *>(dst) = mx_encode4x2(v[0], v[1]) | mx_encode4x2(v[2], v[3]) << 8 | mx_encode4x2(v[4], v[5]) << 16 | mx_encode4x2(v[6], v[7]) << 24;
-        } else {
-            *reinterpret_cast<uint2 *>(dst) = make_uint2(mx_encode8x2(v[0], v[1]) | mx_encode8x2(v[2], v[3]) << 16, mx_encode8x2(v[4], v[5]) | mx_encode8x2(v[6], v[7]) << 16);
+        for (int i = 0; i < E; i++) v[i] *= inverse;
+        uint32_t words[E * FORMAT / 32];
+#pragma unroll
+        for (int w = 0; w < E * FORMAT / 32; w++) {
+            if constexpr (FORMAT == 4) words[w] = mx_encode4x2(v[8 * w], v[8 * w + 1]) | mx_encode4x2(v[8 * w + 2], v[8 * w + 3]) << 8 | mx_encode4x2(v[8 * w + 4], v[8 * w + 5]) << 16 | mx_encode4x2(v[8 * w + 6], v[8 * w + 7]) << 24;
+            else words[w] = mx_encode8x2(v[4 * w], v[4 * w + 1]) | mx_encode8x2(v[4 * w + 2], v[4 * w + 3]) << 16;
         }
+        uint8_t *dst = codes + (int64_t)row * r.code_pitch + (int64_t)group * (E * FORMAT / 8);
+        if constexpr (E * FORMAT == 32) *reinterpret_cast<uint32_t *>(dst) = words[0];
+        else if constexpr (E * FORMAT == 64) *reinterpret_cast<uint2 *>(dst) = make_uint2(words[0], words[1]);
+        else *reinterpret_cast<uint4 *>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
     }
 }
 
@@ -485,12 +507,6 @@ __device__ __forceinline__ void mx_copy_scales(uint32_t dst, int atoms, const ui
 __device__ __forceinline__ void mx_arrive_rank(uint32_t bar, uint32_t rank) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(map_to_rank(bar, rank)) : "memory");
 }
-// Programmatic dependent launch: a kernel launched with mx_launch_dependent may start while the one before it still runs,
-// and does what does not depend on it; `wait` returns when that one has finished.  `release` in the earlier kernel lets
-// the later one's blocks in as soon as there is room.  Both do nothing without such a launch.
-__device__ __forceinline__ void mx_dependent_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void mx_dependent_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Waits, for at most a tenth of a second and whatever the abort flag says, for copies whose barrier nothing else arrives on.
 __device__ __forceinline__ void mx_wait_landed(uint32_t bar, uint32_t parity) {
     const uint64_t start = global_timer();
@@ -681,12 +697,13 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
         float sum;
         if (slices == 1) sum = partial[r * 128 + (threadIdx.x & 127)];
         else {
-            sum = 0.0f;
-            for (int q = 0; q < slices; q++) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(map_to_rank(mine + (uint32_t)r * 512u, (uint32_t)q)) : "memory");
-                sum = q ? __fadd_rn(sum, v) : v;
-            }
+            float v[8];         // all on their way before the first is added
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+                if (q < slices) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[q]) : "r"(map_to_rank(mine + (uint32_t)r * 512u, (uint32_t)q)));
+            sum = v[0];
+#pragma unroll
+            for (int q = 1; q < 8; q++) if (q < slices) sum = __fadd_rn(sum, v[q]);
         }
         if (col < prm.n) ((T *)prm.out)[(int64_t)(m0 + r) * prm.n + col] = mx_narrow<KIND>(mx_activate(prm.act, prm.bias ? __fadd_rn(sum, b) : sum));
     }
@@ -1418,18 +1435,19 @@ static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index
         else even &= ix.sa[d] == row_step * extent;
         extent *= ix.shape[d];
     }
-    const bool vec = even && (ix.sa[3] == 1 || cols == 1) && (uintptr_t)x % (8 * sizeof(T)) == 0 && (rows == 1 || row_step % 8 == 0);
+    constexpr int E = KIND == 0 ? 8 : 16;       // elements of 32 bytes
+    const bool vec = even && (ix.sa[3] == 1 || cols == 1) && (uintptr_t)x % 32 == 0 && (rows == 1 || row_step % E == 0);
     // dense rows of whole scale words are one long row
     const bool flat = vec && !tiles && row_step == cols && cols % (4 * MX_BLOCK) == 0;
     const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
-    const int grid = mx_grid(r * mx_scale_bytes(c) * 4);
+    const int grid = mx_grid(r * mx_scale_bytes(c) * (vec ? MX_BLOCK / E : 4));
     const uint32_t atoms = (uint32_t)mx_tile_atoms(cols);
     const auto launch = [&](auto kernel, auto shape) { kernel<<<grid, MX_THREADS, 0, s>>>((const T *)x, ix, shape, row_step, even ? 1 : 0, codes, scales, tiles, atoms); };
     if (mx_narrow_rows(r, c)) {
-        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT, E));
         else launch(mx_quantize_kernel<FORMAT, KIND, false, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
     } else {
-        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, int64_t>, mx_rows<int64_t>(r, c, FORMAT, E));
         else launch(mx_quantize_kernel<FORMAT, KIND, false, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
     }
     return cudaGetLastError();

@@ -370,7 +370,46 @@ int32_t prepare_executable(Executable *x) {
         *out = p;
         return true;
     };
-    for (int64_t bytes : plan.scratch_bytes) { void *p; if (!alloc((uint64_t)bytes, &p)) return ALLOCATION_FAILED; x->scratch.push_back(p); }
+    // Programs with 8-bit checkpoints let scratch values, and operand planes, whose steps do not overlap share memory:
+    // the steps run one after another on one stream, and the checkpoint is what the backward pass reads instead of
+    // the FLOAT32 tensor.  (Other programs keep every intermediate in memory of its own.)
+    bool share = false;
+    for (const Step &st : plan.steps) share |= st.kind == StepKind::MX_QUANTIZE && st.scalar_bits == 8;
+    typedef std::pair<int, int> Interval;                   // first and last step
+    const Interval never(INT_MAX, -1);
+    std::map<std::pair<int, int>, Interval> touched;        // by (slot kind, index)
+    for (size_t i = 0; share && i < plan.steps.size(); i++) {
+        const Step &st = plan.steps[i];
+        for (int v : {st.a, st.b, st.c, st.bias, st.mask, st.scale_a, st.scale_b, st.out, st.out2, st.out3}) {
+            if (v < 0) continue;
+            Interval &t = touched.emplace(std::make_pair((int)plan.views[v].slot, plan.views[v].index), never).first->second;
+            t.first = std::min(t.first, (int)i); t.second = std::max(t.second, (int)i);
+        }
+    }
+    struct Shared { void *ptr; uint64_t bytes; std::vector<Interval> taken; };
+    std::vector<Shared> pool;
+    auto alloc_for = [&](uint64_t bytes, Interval when, void **out) -> bool {
+        if (!share || when.second < 0) return alloc(bytes, out);
+        Shared *best = nullptr;
+        for (Shared &s : pool) {
+            bool free = s.bytes >= bytes && s.bytes <= 2 * bytes;       // a small value does not hold a large block
+            for (const Interval &t : s.taken) free &= t.second < when.first || when.second < t.first;
+            if (free && (!best || s.bytes < best->bytes)) best = &s;
+        }
+        if (!best) {
+            void *p; if (!alloc(bytes, &p)) return false;
+            pool.push_back(Shared{p, bytes, {}});
+            best = &pool.back();
+        }
+        best->taken.push_back(when);
+        *out = best->ptr;
+        return true;
+    };
+    for (size_t i = 0; i < plan.scratch_bytes.size(); i++) {
+        auto t = touched.find(std::make_pair((int)SlotKind::SCRATCH, (int)i));
+        void *p; if (!alloc_for((uint64_t)plan.scratch_bytes[i], t == touched.end() ? never : t->second, &p)) return ALLOCATION_FAILED;
+        x->scratch.push_back(p);
+    }
     if (!plan.constant_values.empty()) {
         std::vector<uint64_t> host(plan.constant_values.size(), 0);
         for (size_t i = 0; i < host.size(); i++) {
@@ -391,6 +430,19 @@ int32_t prepare_executable(Executable *x) {
         if (v.slot == SlotKind::PUBLICATION) x->publication_bytes[v.index] = std::max(x->publication_bytes[v.index], view_span_bytes(v));
     }
     x->exec.resize(plan.steps.size());
+    // Planes live from the first step that touches the value (which may write them beside it) to the last product that
+    // reads them.
+    std::map<PlaneKey, Interval> plane_steps;
+    for (size_t i = 0; share && i < plan.steps.size(); i++) {
+        const Step &st = plan.steps[i];
+        if (st.kind != StepKind::GEMM || st.engine != GemmEngine::TENSOR_CORE || dtype_low(plan.views[st.a].dtype)) continue;
+        for (int v : {st.a, st.b}) for (int orientation : {0, 1}) {
+            const View &w = plan.views[v];
+            const Interval &t = touched[std::make_pair((int)w.slot, w.index)];
+            Interval &p = plane_steps.emplace(plane_key(w, orientation), never).first->second;
+            p.first = std::min(p.first, t.first); p.second = std::max(p.second, (int)i);
+        }
+    }
     int64_t workspace_floats = 0;               // one workspace serves every sliced GEMM: the steps run in stream order
     auto planes_for = [&](int value, int orientation, int64_t rows, int64_t k) -> int {
         PlaneKey key = plane_key(plan.views[value], orientation);
@@ -399,7 +451,9 @@ int32_t prepare_executable(Executable *x) {
         Planes p;
         p.rows = rows; p.kp = kern::padded_k(k); p.pitch = kern::plane_pitch(p.kp);
         void *hi, *lo;
-        if (!alloc((uint64_t)rows * p.pitch * 4, &hi) || !alloc((uint64_t)rows * p.pitch * 4, &lo)) return -1;
+        // padding columns have to stay zero, so planes that have any share nothing
+        const Interval when = share && p.kp == k ? plane_steps[key] : never;
+        if (!alloc_for((uint64_t)rows * p.pitch * 4, when, &hi) || !alloc_for((uint64_t)rows * p.pitch * 4, when, &lo)) return -1;
         // padding columns are zero from the start: the pass that fills planes beside the column sums
         // only writes the real columns
         if (cudaMemsetAsync(hi, 0, (uint64_t)rows * p.pitch * 4, ctx->stream) != cudaSuccess

@@ -179,3 +179,25 @@ def test_one_tensor_as_both_operands(ctx):
         got, = ref.helpers.run_image(ctx, g, [x])
         v = ref.values(*ref.quantize(x, "mx4"), "mx4", 96)
         assert (np.abs(got - v @ v.T) <= 7 * 2.0 ** -23 * (np.abs(v) @ np.abs(v).T)).all()
+
+
+def test_checkpoints_take_less_memory(ctx):
+    """A training program with 8-bit checkpoints reuses the memory of what its backward pass no longer reads."""
+    torch = pytest.importorskip("torch")
+    dims, batch = [256, 1024, 1024, 1024, 1024, 16], 8192
+    used, grads = {}, {}
+    rng = np.random.default_rng(0)
+    x, target = rng.standard_normal((batch, dims[0])).astype(np.float32), rng.integers(0, dims[-1], batch)
+    for kind in (None, "mx8"):
+        model = nn.Model(dims, ctx, seed=4, checkpoints=kind)
+        model.configure_training("ce", nn.Sgd(0.01))
+        ctx.synchronize()
+        free = torch.cuda.mem_get_info(0)[0]
+        model.training_state(batch)
+        used[kind] = free - torch.cuda.mem_get_info(0)[0]
+        grads[kind] = model.gradients(x, target)
+        model.close()
+    assert used["mx8"] < 0.7 * used[None], used
+    assert grads["mx8"][0] == grads[None][0]
+    for a, b in zip(grads["mx8"][1], grads[None][1]):
+        assert np.linalg.norm(a - b) <= 0.25 * np.linalg.norm(b)
