@@ -127,21 +127,26 @@ template <int KIND> __device__ __forceinline__ void mx_load16(const uint16_t *p,
 // hands them over through its part of shared memory; a thread per group would touch every line eight times.
 // `offset`: element offset of this lane's group, `step`: distance of consecutive columns.  Where the warp's groups
 // follow one another in memory (one row, or dense rows without a gap between them) the first one's offset serves all.
-template <int KIND> __device__ __forceinline__ void mx_gather8(const typename MxElement<KIND>::type *p, int64_t offset, int64_t step, int count,
-                                                                float *box, int lane, float (&v)[8]) {
+// mx_gather8 only starts the loads (element i * 32 + lane of the warp's 256), mx_exchange8 hands them over, so that the
+// work on one group can lie between the two of the next.
+template <int KIND> __device__ __forceinline__ void mx_gather8(const typename MxElement<KIND>::type *p, int64_t offset, int64_t step, int count, int lane, float (&raw)[8]) {
     const int64_t base = __shfl_sync(0xffffffffu, offset, 0);
     if (__all_sync(0xffffffffu, offset == base + lane * 8 * step && count == 8)) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) box[i * 32 + lane] = mx_load<KIND>(p + base + (i * 32 + lane) * step);
+        for (int i = 0; i < 8; i++) raw[i] = mx_load<KIND>(p + base + (i * 32 + lane) * step);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int owner = i * 4 + (lane >> 3);
             const int64_t at = __shfl_sync(0xffffffffu, offset, owner);
             const int have = __shfl_sync(0xffffffffu, count, owner);
-            box[i * 32 + lane] = (lane & 7) < have ? mx_load<KIND>(p + at + (lane & 7) * step) : 0.0f;
+            raw[i] = (lane & 7) < have ? mx_load<KIND>(p + at + (lane & 7) * step) : 0.0f;
         }
     }
+}
+__device__ __forceinline__ void mx_exchange8(const float (&raw)[8], float *box, int lane, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) box[i * 32 + lane] = raw[i];
     __syncwarp();
     const float4 a = *reinterpret_cast<const float4 *>(box + lane * 8), b = *reinterpret_cast<const float4 *>(box + lane * 8 + 4);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -255,7 +260,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
                 const int64_t row = count ? (int64_t)at.row : 0, r2 = row % ix.shape[2], rest = row / ix.shape[2];
                 base = r2 * ix.sa[2] + rest % ix.shape[1] * ix.sa[1] + rest / ix.shape[1] * ix.sa[0];
             }
-            mx_gather8<KIND>(x, base + (int64_t)at.group * 8 * ix.sa[3], ix.sa[3], count, boxes[threadIdx.x >> 5], lane, v);
+            mx_gather8<KIND>(x, base + (int64_t)at.group * 8 * ix.sa[3], ix.sa[3], count, lane, v);
         }
     };
     float ahead[E];
@@ -263,8 +268,10 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
     if (at.in(r)) fetch(ahead);
     while (at.in(r)) {
         float v[E];
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = ahead[i];
+            for (int i = 0; i < E; i++) v[i] = ahead[i];
+        } else mx_exchange8(ahead, boxes[threadIdx.x >> 5], lane, v);
         const I row = at.row, group = at.group;
         const bool mine = at.g < r.total;
         at.next(r);
@@ -405,15 +412,17 @@ __global__ void __launch_bounds__(MX_THREADS) mx_activation_gradient_kernel(int 
         const int count = at.count(r);
         if (count) mx_fetch_held<8>(codes, scales, r, at, held_ahead);
         if constexpr (VEC) { if (count) mx_load8<KIND>(g_in + at.offset(cols), up_ahead); }
-        else mx_gather8<KIND>(g_in, at.offset(cols), 1, count, boxes[threadIdx.x >> 5], lane, up_ahead);
+        else mx_gather8<KIND>(g_in, at.offset(cols), 1, count, lane, up_ahead);
     };
     at.start(r);
     if (at.in(r)) fetch();
     while (at.in(r)) {
         const MxHeld<8> held = held_ahead;
         float up[8], z[8];
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) up[i] = up_ahead[i];
+            for (int i = 0; i < 8; i++) up[i] = up_ahead[i];
+        } else mx_exchange8(up_ahead, boxes[threadIdx.x >> 5], lane, up);
         const int count = at.count(r);
         const int64_t offset = at.offset(cols);
         at.next(r);
@@ -1080,7 +1089,11 @@ __global__ void __launch_bounds__(MX_THREADS) mx_pieces_kernel(const typename Mx
             const int count = left >= 8 ? 8 : left > 0 ? (int)left : 0;
             float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (VEC) { if (count) mx_load8<KIND>(g + row * n + group * 8, f); }
-            else mx_gather8<KIND>(g, row * n + group * 8, 1, count, boxes[threadIdx.x >> 5], threadIdx.x & 31, f);
+            else {
+                float raw[8];
+                mx_gather8<KIND>(g, row * n + group * 8, 1, count, threadIdx.x & 31, raw);
+                mx_exchange8(raw, boxes[threadIdx.x >> 5], threadIdx.x & 31, f);
+            }
             if (i < total) {
 #pragma unroll
                 for (int piece = 0; piece < PIECES; piece++) {
