@@ -244,8 +244,21 @@ def test_linear_special_values(ctx, m):
     assert np.isnan(got[m // 2]).all() and np.isnan(got[:, 9]).all()
     good = np.isfinite(want)
     s = np.abs(xv) @ np.abs(wv).T
-    assert (np.abs(got - want)[good] <= (12 * 2.0 ** -23 * s)[good]).all()
+    assert (np.abs(got[good] - want[good]) <= 12 * 2.0 ** -23 * s[good]).all()
     assert np.array_equal(got[~good & ~np.isnan(want)], want[~good & ~np.isnan(want)])
+
+
+@pytest.mark.parametrize("m", [3, 200, 3000])
+@pytest.mark.parametrize("k", [32, 96, 288, 800])
+def test_linear_ignores_what_pads_the_scales(ctx, m, k):
+    """Bytes of a row of scales past its last block, NaN among them, do not reach the result."""
+    rng = np.random.default_rng(m + k)
+    n = 1000
+    x, w = (*random_held(rng, "mx4", (m, k)), (m, k)), (*random_held(rng, "mx4", (n, k)), (n, k))
+    want = linear(ctx, "f32", x, w, None, None)
+    for held in (x, w):
+        held[1][:, k // 32:] = 255
+    assert np.array_equal(linear(ctx, "f32", x, w, None, None), want)
 
 
 @pytest.mark.parametrize("kind,m,k,n", [("f32", 700, 512, 600), ("bf16", 1500, 2048, 4096), ("f16", 4100, 800, 1016)])

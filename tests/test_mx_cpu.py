@@ -135,3 +135,19 @@ def test_builder_refuses_what_does_not_fit():
         g.mx_weight_gradient(g.mx_feed("mx4", (4, 32)), g.feed(F32, (4, 8)))
     with pytest.raises(ValueError):
         g.mx_activation_gradient("relu", g.mx_feed("mx8", (4, 32)), g.feed(F32, (4, 31)))
+
+
+def test_model_graphs():
+    plan = native.describe(program.mlp_mx_inference_graph([784, 256, 10], 32, arg_max=True).image)
+    assert [line.split()[0] for line in plan.splitlines()] == ["mx_quantize", "mx_linear", "mx_quantize", "mx_linear", "arg_max"]
+    assert "act=RELU" in plan.splitlines()[1] and "act=" not in plan.splitlines()[3]
+    for activation, held in [("relu", 3), ("gelu", 5)]:       # every layer's input; for GELU the two pre-activations too
+        graph = program.mlp_training_graph([784, 256, 256, 10], 64, activation=activation, checkpoints="mx8")
+        plan = native.describe(graph.image)
+        steps = [line.split()[0] for line in plan.splitlines()]
+        assert steps.count("mx_quantize") == held and steps.count("mx_weight_gradient") == 3 and steps.count("mx_activation_gradient") == 2
+        assert graph.publications == program.mlp_training_graph([784, 256, 256, 10], 64, activation=activation).publications
+    with pytest.raises(ValueError):
+        program.mlp_training_graph([4, 4], 4, checkpoints="mx4")
+    with pytest.raises(ValueError):
+        program.mlp_mx_inference_graph([4, 4], (2, 3), arg_max=True)
