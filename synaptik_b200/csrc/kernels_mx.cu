@@ -1026,7 +1026,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 
 // ------------------------------------------------------------------------------------------------
 // Weight gradient from an 8-bit checkpoint: D[n, k] = sum over rows of g[row, n] x[row, k] on the tensor cores
-// (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k.
+// (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k (128 where k is no more; four
+// tiles of 224 for 784 columns start off 128-byte lines and took 12 % longer than four of 256).
 //   An E4M3 element under a power-of-two scale is a BFLOAT16 number as it stands (below 2^-133 it rounds), so the
 // checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly: 8 + 8 + 8 significand bits for
 // FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
@@ -1049,12 +1050,15 @@ template <int PIECES> struct MxGradConfig {
     static constexpr int kStageBytes = (PIECES + 1) * kTileBytes;
     static constexpr int kStages = PIECES == 3 ? 3 : PIECES == 2 ? 4 : 6;
     static constexpr int kChunk = PIECES == 3 ? 4 : 8;                  // stages per partial sum in tensor memory
-    static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 256;
+    static constexpr int kStagingBytes = 8 * 4096;                      // a box of 32 rows x 32 columns per epilogue warp
+    static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 };
 
 struct MxGrad {
     int n, k;
     int64_t rows;
+    int bn;                             // columns of a tile, 128 or 256
+    int staged;                         // rows of `out` can be written by TMA
     int tiles_n, whole_tiles, units;    // units: the whole tiles, then `slices` per tile that is left
     int slices, stages, stages_per_slice;       // of MX_ROWS rows
     float *out, *partial;               // partial: [tile that is left][slice][256][256]
@@ -1126,12 +1130,13 @@ __global__ void __launch_bounds__(MX_THREADS) mx_pieces_kernel(const typename Mx
 
 template <int PIECES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) mx_weight_gradient_kernel(
-        const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, MxGrad prm) {
+        const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_out,
+        const __grid_constant__ CUtensorMap map_partial, MxGrad prm) {
     using Cfg = MxGradConfig<PIECES>;
     constexpr int S = Cfg::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes + Cfg::kStagingBytes);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 4);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1171,7 +1176,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
             first = u % prm.slices * prm.stages_per_slice;
             count = prm.stages - first < prm.stages_per_slice ? prm.stages - first : prm.stages_per_slice;
         }
-        n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * 256;
+        n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * prm.bn;
     };
 
     if (warp < 4) {
@@ -1185,7 +1190,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 for (int unit = pair; unit < prm.units && ok; unit += pairs) {
                     int n0, k0, first, count;
                     unit_of(unit, n0, k0, first, count);
-                    n0 += (int)rank * 128; k0 += (int)rank * 128;
+                    n0 += (int)rank * 128; k0 += (int)rank * (prm.bn / 2);
                     for (int i = 0; i < count; i++) {
                         if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
                         const uint32_t leader_full = map_to_rank(full_bar(stage), 0), pa = smem_base + stage * Cfg::kStageBytes, pb = pa + PIECES * Cfg::kTileBytes;
@@ -1208,8 +1213,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
             }
         } else if (warp == 1) {
             if (rank == 0 && lane == 0) {
-                // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
+                // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x bn
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(prm.bn >> 3) << 17) | ((256u >> 4) << 24);
                 // groups of 64 columns 8 KB apart (leading offset), groups of 8 rows 1 KB (stride offset), 128-byte swizzle
                 const uint64_t fixed = ((uint64_t)((MX_ROWS * 128u) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
                 auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
@@ -1280,33 +1285,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 if (lane == 0) mx_arrive_rank(acc_empty_bar(buf), 0);
             }
             if (!ok) break;
-            const int row = (int)rank * 128 + quarter * 32 + lane, col = half * 128;     // in the tile
-            if (unit >= prm.whole_tiles) {
-                float *out = prm.partial + (int64_t)(unit - prm.whole_tiles) * 65536 + row * 256 + col;
+            // out through boxes of 32 x 32 in shared memory (16-byte chunk j of row r at chunk j ^ (r & 7)) and TMA, which clips
+            // the edges; rows of `out` that TMA cannot address are copied from the box, a row per instruction
+            const bool partial = unit >= prm.whole_tiles;
+            const int row0 = (int)rank * 128 + quarter * 32, row_limit = partial ? 32 : prm.n - n0 - row0;
+            const uint32_t box = smem_base + (uint32_t)(S * Cfg::kStageBytes + (warp - 4) * 4096);
 #pragma unroll
-                for (int q = 0; q < 16; q++) {
-                    float v[8];
+            for (int b = 0; b < 4; b++) {
+                const int col = half * 128 + b * 32;        // in the tile
+                if (col >= prm.bn || row_limit <= 0 || (!partial && k0 + col >= prm.k)) break;      // warp-uniform
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // the previous box has been read
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = sum[q * 8 + e];
-                    mx_store8<0>(out + q * 8, v);
-                }
-            } else if (n0 + row < prm.n) {
-                float *out = prm.out + (int64_t)(n0 + row) * prm.k + k0 + col;
-                const int left = prm.k - k0 - col;
-                if ((prm.k & 7) == 0 && ((uintptr_t)prm.out & 31) == 0) {
-#pragma unroll
-                    for (int q = 0; q < 16; q++) {
-                        float v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = sum[q * 8 + e];
-                        if (q * 8 < left) mx_store8<0>(out + q * 8, v);
+                for (int j = 0; j < 8; j++)
+                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(box + (uint32_t)(lane * 128 + ((j ^ (lane & 7)) << 4))),
+                                 "f"(sum[b * 32 + j * 4]), "f"(sum[b * 32 + j * 4 + 1]), "f"(sum[b * 32 + j * 4 + 2]), "f"(sum[b * 32 + j * 4 + 3]) : "memory");
+                if (partial || prm.staged) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (partial) tma_store_2d(&map_partial, box, col, (unit - prm.whole_tiles) * 256 + row0);
+                        else tma_store_2d(&map_out, box, k0 + col, n0 + row0);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 } else {
-#pragma unroll
-                    for (int q = 0; q < 128; q++) if (q < left) out[q] = sum[q];
+                    __syncwarp();
+                    float *out = prm.out + (int64_t)(n0 + row0) * prm.k + k0 + col;
+                    for (int r = 0; r < 32 && r < row_limit; r++) {
+                        float v;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(box + (uint32_t)(r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)));
+                        if (k0 + col + lane < prm.k) out[(int64_t)r * prm.k + lane] = v;
+                    }
+                    __syncwarp();
                 }
             }
         }
+        staged_drain(lane);
     }
 
     tc_fence_before();
@@ -1383,9 +1397,9 @@ __global__ void __launch_bounds__(MX_SMALL_THREADS) mx_weight_gradient_small_ker
 // The tiles that were cut into slices: their sums in ascending order.  blockIdx.y: the tile; a thread adds four columns.
 __global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(MxGrad prm) {
     mx_dependent_wait();
-    const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * 256;
+    const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * prm.bn;
     const int i = blockIdx.x * MX_THREADS + threadIdx.x, row = i >> 6, col = (i & 63) * 4;
-    if (n0 + row >= prm.n || k0 + col >= prm.k) return;
+    if (n0 + row >= prm.n || col >= prm.bn || k0 + col >= prm.k) return;
     const float *p = prm.partial + (int64_t)blockIdx.y * prm.slices * 65536 + row * 256 + col;
     float4 a = __ldg(reinterpret_cast<const float4 *>(p));
     for (int q = 1; q < prm.slices; q++) {
@@ -1639,8 +1653,12 @@ static cudaError_t launch_mx_linear(cudaStream_t s, const uint8_t *x, const uint
     prm.tiles_n = (prm.n + 127) / 128; prm.tiles_m = (prm.m + bn - 1) / bn;
     const int64_t tiles = (int64_t)prm.tiles_n * prm.tiles_m;
     if (tiles >= (1ll << 28)) return cudaErrorInvalidValue;
+    // Slices of the contraction while blocks are left over, each of at least `least` k-blocks: adding up the slices costs
+    // time with the rows of a tile.  Measured: 203 x 4096 x 1000 in slices of 4 and 2 k-blocks 20.5 and 24.5 us, 16 x 784 x
+    // 4096 in slices of 4, 2 and 1 14.3, 12.7 and 12.3 us.
+    const int least = bn <= 32 ? 1 : bn == 64 ? 2 : 4;
     int slices = 1;
-    while (slices < 8 && tiles * slices * 2 <= sm_count && prm.k_blocks >= slices * 2) slices *= 2;
+    while (slices < 8 && tiles * slices * 2 <= sm_count && prm.k_blocks >= slices * 2 * least) slices *= 2;
     switch (bn) {
         case 16: return launch_mx_few<16, KIND>(s, x, w, prm, slices);
         case 32: return launch_mx_few<32, KIND>(s, x, w, prm, slices);
@@ -1694,14 +1712,16 @@ static cudaError_t launch_mx_gradient_small(cudaStream_t s, int64_t rows, int64_
 
 // How the tiles are spread over the block pairs, and what scratch that takes.
 struct MxGradPlan {
-    int pieces, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
+    int pieces, bn, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
     bool direct;                        // BFLOAT16 rows that TMA can address are read where they are
     int64_t g_pitch, g_bytes, x_bytes, partial_bytes;       // of the planes and partial sums, each a multiple of 256
 };
 static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t k, bool aligned, int sm_count) {
     MxGradPlan p = {};
     p.pieces = dtype == DType::F32 ? 3 : dtype == DType::BF16 ? 1 : 2;
-    p.tiles_n = (int)((n + 255) / 256); p.tiles = p.tiles_n * (int)((k + 255) / 256);
+    const int tiles_k = (int)((k + 255) / 256);
+    p.bn = k <= 128 ? 128 : 256;
+    p.tiles_n = (int)((n + 255) / 256); p.tiles = p.tiles_n * tiles_k;
     p.stages = (int)((rows + MX_ROWS - 1) / MX_ROWS);
     const int pairs = sm_count / 2 > 0 ? sm_count / 2 : 1;
     p.whole_tiles = p.tiles / pairs * pairs;
@@ -1748,15 +1768,27 @@ static bool make_piece_map(CUtensorMap *map, const void *base, int64_t planes, i
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tensor map over dense FLOAT32 [rows, cols]: boxes of 32 x 32, 128-byte swizzle.
+static bool make_result_map(CUtensorMap *map, const void *base, int64_t rows, int64_t cols) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)cols * 4};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t elem[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int PIECES>
-static cudaError_t launch_mx_gradient(cudaStream_t s, const CUtensorMap &map_g, const CUtensorMap &map_x, const MxGrad &prm, int sm_count) {
+static cudaError_t launch_mx_gradient(cudaStream_t s, const CUtensorMap &map_g, const CUtensorMap &map_x, const CUtensorMap &map_out, const CUtensorMap &map_partial, const MxGrad &prm, int sm_count) {
     using Cfg = MxGradConfig<PIECES>;
     // the register split draws on what the block was launched with
     static std::atomic<uint64_t> done{0};
     cudaError_t e = mx_prepare_kernel(mx_weight_gradient_kernel<PIECES>, Cfg::kSmemBytes, (72 + 2 * 216 + 2) / 3, done);
     if (e != cudaSuccess) return e;
     const int pairs = sm_count / 2;
-    return mx_launch_dependent(mx_weight_gradient_kernel<PIECES>, dim3((unsigned)(2 * (prm.units < pairs ? prm.units : pairs))), MX_GRAD_THREADS, Cfg::kSmemBytes, s, map_g, map_x, prm);
+    return mx_launch_dependent(mx_weight_gradient_kernel<PIECES>, dim3((unsigned)(2 * (prm.units < pairs ? prm.units : pairs))), MX_GRAD_THREADS, Cfg::kSmemBytes, s, map_g, map_x, map_out, map_partial, prm);
 }
 
 template <int KIND>
@@ -1799,11 +1831,14 @@ cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_
     CUtensorMap map_g, map_x;
     if (!make_piece_map(&map_g, p.direct ? g : g_planes, p.pieces, rows, n, p.direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
     MxGrad prm = {};
-    prm.n = (int)n; prm.k = (int)k; prm.rows = rows;
+    prm.n = (int)n; prm.k = (int)k; prm.rows = rows; prm.bn = p.bn;
     prm.tiles_n = p.tiles_n; prm.whole_tiles = p.whole_tiles; prm.units = (int)units;
     prm.slices = p.slices; prm.stages = p.stages; prm.stages_per_slice = p.stages_per_slice;
     prm.out = out; prm.partial = (float *)((uint8_t *)workspace + p.g_bytes + p.x_bytes); prm.error_word = error_word;
-    e = p.pieces == 3 ? launch_mx_gradient<3>(s, map_g, map_x, prm, sm_count) : p.pieces == 2 ? launch_mx_gradient<2>(s, map_g, map_x, prm, sm_count) : launch_mx_gradient<1>(s, map_g, map_x, prm, sm_count);
+    CUtensorMap map_out = map_x, map_partial = map_x;           // unused where they are not made
+    prm.staged = k % 4 == 0 && ((uintptr_t)out & 15) == 0 && make_result_map(&map_out, out, n, k);
+    if (p.slices > 1 && !make_result_map(&map_partial, prm.partial, (units - p.whole_tiles) * 256, 256)) return cudaErrorInvalidValue;
+    e = p.pieces == 3 ? launch_mx_gradient<3>(s, map_g, map_x, map_out, map_partial, prm, sm_count) : p.pieces == 2 ? launch_mx_gradient<2>(s, map_g, map_x, map_out, map_partial, prm, sm_count) : launch_mx_gradient<1>(s, map_g, map_x, map_out, map_partial, prm, sm_count);
     if (e != cudaSuccess || p.slices == 1) return e;
     return mx_launch_dependent(mx_add_slices_kernel, dim3(65536 / 4 / MX_THREADS, (unsigned)(p.tiles - p.whole_tiles)), MX_THREADS, 0, s, prm);
 }

@@ -303,7 +303,8 @@ def test_weight_gradient_over_leading_dimensions(ctx, kind):
     check_weight_gradient(ctx, kind, (3, 41), 70, 40)
 
 
-@pytest.mark.parametrize("kind,rows,k,n", [("f32", 5000, 520, 512), ("bf16", 9000, 784, 512), ("f16", 3000, 1024, 1000)])
+@pytest.mark.parametrize("kind,rows,k,n", [("f32", 5000, 520, 512), ("bf16", 9000, 784, 512), ("f16", 3000, 1024, 1000), ("f32", 20, 2500, 3300),
+                                           ("bf16", 70, 4097, 2600), ("f16", 130, 3300, 2049), ("f32", 700, 1500, 4000)])
 def test_weight_gradient_long(ctx, kind, rows, k, n):
     check_weight_gradient(ctx, kind, (rows,), k, n)
 
