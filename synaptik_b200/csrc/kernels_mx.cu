@@ -1026,8 +1026,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 
 // ------------------------------------------------------------------------------------------------
 // Weight gradient from an 8-bit checkpoint: D[n, k] = sum over rows of g[row, n] x[row, k] on the tensor cores
-// (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k (128 where k is no more; four
-// tiles of 224 for 784 columns start off 128-byte lines and took 12 % longer than four of 256).
+// (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k (784 columns as
+// four tiles of 224 start off 128-byte lines and took 12 % longer than four of 256).
 //   An E4M3 element under a power-of-two scale is a BFLOAT16 number as it stands (below 2^-133 it rounds), so the
 // checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly: 8 + 8 + 8 significand bits for
 // FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
@@ -1057,7 +1057,6 @@ template <int PIECES> struct MxGradConfig {
 struct MxGrad {
     int n, k;
     int64_t rows;
-    int bn;                             // columns of a tile, 128 or 256
     int staged;                         // rows of `out` can be written by TMA
     int tiles_n, whole_tiles, units;    // units: the whole tiles, then `slices` per tile that is left
     int slices, stages, stages_per_slice;       // of MX_ROWS rows
@@ -1176,7 +1175,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
             first = u % prm.slices * prm.stages_per_slice;
             count = prm.stages - first < prm.stages_per_slice ? prm.stages - first : prm.stages_per_slice;
         }
-        n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * prm.bn;
+        n0 = tile % prm.tiles_n * 256; k0 = tile / prm.tiles_n * 256;
     };
 
     if (warp < 4) {
@@ -1190,7 +1189,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
                 for (int unit = pair; unit < prm.units && ok; unit += pairs) {
                     int n0, k0, first, count;
                     unit_of(unit, n0, k0, first, count);
-                    n0 += (int)rank * 128; k0 += (int)rank * (prm.bn / 2);
+                    n0 += (int)rank * 128; k0 += (int)rank * 128;
                     for (int i = 0; i < count; i++) {
                         if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
                         const uint32_t leader_full = map_to_rank(full_bar(stage), 0), pa = smem_base + stage * Cfg::kStageBytes, pb = pa + PIECES * Cfg::kTileBytes;
@@ -1213,8 +1212,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
             }
         } else if (warp == 1) {
             if (rank == 0 && lane == 0) {
-                // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x bn
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((uint32_t)(prm.bn >> 3) << 17) | ((256u >> 4) << 24);
+                // BFLOAT16 operands, FP32 accumulators, both MN-major, 256 x 256
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
                 // groups of 64 columns 8 KB apart (leading offset), groups of 8 rows 1 KB (stride offset), 128-byte swizzle
                 const uint64_t fixed = ((uint64_t)((MX_ROWS * 128u) >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
                 auto desc = [&](uint32_t addr) { return fixed | (uint64_t)((addr & 0x3ffffu) >> 4); };
@@ -1257,28 +1256,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
             int n0, k0, first, count;
             unit_of(unit, n0, k0, first, count);
             float sum[128];
+#pragma unroll
+            for (int q = 0; q < 128; q++) sum[q] = 0.0f;
             for (int i0 = 0; i0 < count; i0 += Cfg::kChunk, chunk++) {
                 const int buf = chunk & 1;
                 ok = mx_warp_wait(acc_full_bar(buf), (chunk >> 1) & 1u, abort_flag, lane);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * 256 + half * 128);
-                if (i0 == 0) {
 #pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        float t[16];
-                        tmem_load16(taddr + (uint32_t)(q * 16), t);
+                for (int q = 0; q < 8; q++) {
+                    float t[16];
+                    tmem_load16(taddr + (uint32_t)(q * 16), t);
 #pragma unroll
-                        for (int e = 0; e < 16; e++) sum[q * 16 + e] = t[e];
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; q++) {
-                        float t[16];
-                        tmem_load16(taddr + (uint32_t)(q * 16), t);
-#pragma unroll
-                        for (int e = 0; e < 16; e++) sum[q * 16 + e] = __fadd_rn(sum[q * 16 + e], t[e]);
-                    }
+                    for (int e = 0; e < 16; e++) sum[q * 16 + e] = __fadd_rn(sum[q * 16 + e], t[e]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -1293,7 +1284,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_GRAD_THREADS, 1) 
 #pragma unroll
             for (int b = 0; b < 4; b++) {
                 const int col = half * 128 + b * 32;        // in the tile
-                if (col >= prm.bn || row_limit <= 0 || (!partial && k0 + col >= prm.k)) break;      // warp-uniform
+                if (row_limit <= 0 || (!partial && k0 + col >= prm.k)) break;      // warp-uniform
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");       // the previous box has been read
                 __syncwarp();
 #pragma unroll
@@ -1397,9 +1388,9 @@ __global__ void __launch_bounds__(MX_SMALL_THREADS) mx_weight_gradient_small_ker
 // The tiles that were cut into slices: their sums in ascending order.  blockIdx.y: the tile; a thread adds four columns.
 __global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(MxGrad prm) {
     mx_dependent_wait();
-    const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * prm.bn;
+    const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * 256;
     const int i = blockIdx.x * MX_THREADS + threadIdx.x, row = i >> 6, col = (i & 63) * 4;
-    if (n0 + row >= prm.n || col >= prm.bn || k0 + col >= prm.k) return;
+    if (n0 + row >= prm.n || k0 + col >= prm.k) return;
     const float *p = prm.partial + (int64_t)blockIdx.y * prm.slices * 65536 + row * 256 + col;
     float4 a = __ldg(reinterpret_cast<const float4 *>(p));
     for (int q = 1; q < prm.slices; q++) {
@@ -1712,7 +1703,7 @@ static cudaError_t launch_mx_gradient_small(cudaStream_t s, int64_t rows, int64_
 
 // How the tiles are spread over the block pairs, and what scratch that takes.
 struct MxGradPlan {
-    int pieces, bn, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
+    int pieces, tiles_n, tiles, whole_tiles, slices, stages, stages_per_slice;
     bool direct;                        // BFLOAT16 rows that TMA can address are read where they are
     int64_t g_pitch, g_bytes, x_bytes, partial_bytes;       // of the planes and partial sums, each a multiple of 256
 };
@@ -1720,7 +1711,6 @@ static MxGradPlan mx_gradient_plan(DType dtype, int64_t rows, int64_t n, int64_t
     MxGradPlan p = {};
     p.pieces = dtype == DType::F32 ? 3 : dtype == DType::BF16 ? 1 : 2;
     const int tiles_k = (int)((k + 255) / 256);
-    p.bn = k <= 128 ? 128 : 256;
     p.tiles_n = (int)((n + 255) / 256); p.tiles = p.tiles_n * tiles_k;
     p.stages = (int)((rows + MX_ROWS - 1) / MX_ROWS);
     const int pairs = sm_count / 2 > 0 ? sm_count / 2 : 1;
@@ -1831,7 +1821,7 @@ cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_
     CUtensorMap map_g, map_x;
     if (!make_piece_map(&map_g, p.direct ? g : g_planes, p.pieces, rows, n, p.direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
     MxGrad prm = {};
-    prm.n = (int)n; prm.k = (int)k; prm.rows = rows; prm.bn = p.bn;
+    prm.n = (int)n; prm.k = (int)k; prm.rows = rows;
     prm.tiles_n = p.tiles_n; prm.whole_tiles = p.whole_tiles; prm.units = (int)units;
     prm.slices = p.slices; prm.stages = p.stages; prm.stages_per_slice = p.stages_per_slice;
     prm.out = out; prm.partial = (float *)((uint8_t *)workspace + p.g_bytes + p.x_bytes); prm.error_word = error_word;
