@@ -1049,7 +1049,7 @@ template <int PIECES> struct MxGradConfig {
     static constexpr int kTileBytes = MX_ROWS * 128 * 2;                // one operand piece of 128 columns
     static constexpr int kStageBytes = (PIECES + 1) * kTileBytes;
     static constexpr int kStages = PIECES == 3 ? 3 : PIECES == 2 ? 4 : 6;
-    static constexpr int kChunk = PIECES == 3 ? 4 : 8;                  // stages per partial sum in tensor memory
+    static constexpr int kChunk = PIECES == 3 ? 4 : PIECES == 2 ? 8 : 16;      // stages per partial sum in tensor memory: at most 64 MMAs
     static constexpr int kStagingBytes = 8 * 4096;                      // a box of 32 rows x 32 columns per epilogue warp
     static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 };
