@@ -201,3 +201,38 @@ def test_checkpoints_take_less_memory(ctx):
     assert grads["mx8"][0] == grads[None][0]
     for a, b in zip(grads["mx8"][1], grads[None][1]):
         assert np.linalg.norm(a - b) <= 0.25 * np.linalg.norm(b)
+
+
+def test_two_threads_with_a_context_each(ctx):
+    """Programs of both tensor-core products run from two threads at once, each on its own context."""
+    import threading
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((700, 320)).astype(np.float32)
+    w = rng.standard_normal((1100, 320)).astype(np.float32)
+    up = rng.standard_normal((700, 600)).astype(np.float32)
+    results, failures = {}, []
+
+    def work(name):
+        try:
+            c = native.Context(0)
+            got = []
+            for _ in range(5):
+                g = program.GraphBuilder()
+                xv, wv, uv = g.feed(program.F32, x.shape), g.feed(program.F32, w.shape), g.feed(program.F32, up.shape)
+                g.publish(g.mx_linear(g.mx_quantize(xv, "mx4"), g.mx_quantize(wv, "mx4")))
+                g.publish(g.mx_weight_gradient(g.mx_quantize(xv, "mx8"), uv))
+                got.append(ref.helpers.run_image(c, g, [x, w, up]))
+            c.close()
+            results[name] = got
+        except Exception as e:      # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    first = results[0][0]
+    for got in results[0] + results[1]:
+        assert all(np.array_equal(a, b) for a, b in zip(first, got))
