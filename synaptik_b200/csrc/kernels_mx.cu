@@ -221,8 +221,11 @@ __device__ __forceinline__ int64_t mx_tile_offset(int64_t row, int64_t block, in
     return ((row >> 7) * atoms + (block >> 2)) * MX_ATOM + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 // The same from scales that exist already: a thread moves one word of four rows.  Bytes past the last block are not
-// taken over: against codes of zero a scale of NaN would still make NaN.
+// taken over: against codes of zero a scale of NaN would still make NaN.  Launched behind the quantisation of the other
+// operand it works beside it, and ends after it, so that the product only has to wait for this launch.  Quantisation,
+// tiling and product so overlapped, 4096 x 4096 BFLOAT16 weights: 1024 rows 34.0 -> 28.9 us, 8192 rows 106 -> 102 us.
 __global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_t *__restrict__ scales, int64_t rows, int64_t blocks, uint8_t *__restrict__ tiles) {
+    mx_dependent_release();
     const int64_t words = (blocks + 3) / 4, atoms = mx_tile_atoms(blocks * MX_BLOCK), total = (rows + 127) / 128 * 32 * words;
     for (int64_t i = blockIdx.x * (int64_t)MX_THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * MX_THREADS) {
         const int64_t line = i / words, word = i - line * words, band = line >> 5, r = band * 128 + (line & 31);
@@ -233,6 +236,7 @@ __global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_
         for (int q = 0; q < 4; q++) v[q] = r + 32 * q < rows ? *reinterpret_cast<const uint32_t *>(scales + (r + 32 * q) * words * 4 + word * 4) & keep : 0u;
         *reinterpret_cast<uint4 *>(tiles + (band * atoms + word) * MX_ATOM + (line & 31) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
     }
+    mx_dependent_wait();
 }
 
 // x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.  A thread takes 32 aligned
@@ -883,6 +887,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MX_PAIR_REGS_LOW));
         if (warp == 0) {
             if (lane == 0) {
+                mx_dependent_wait();        // x, and the scales in tiles
                 int stage = 0; uint32_t phase = 0;
                 int armed = 0;
                 bool ok = true;
@@ -906,6 +911,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
             }
         } else if (warp == 2) {
             if (lane == 0) {
+                mx_dependent_wait();
                 int slot = 0; uint32_t phase = 0;
                 int armed = 0;
                 bool ok = true;
@@ -1616,7 +1622,9 @@ static cudaError_t launch_mx_pair(cudaStream_t s, const uint8_t *x, const uint8_
     static std::atomic<uint64_t> done{0};
     cudaError_t e = mx_prepare_kernel(mx_linear_pair_kernel<KIND, GENERAL>, Cfg::kSmemBytes, (MX_PAIR_REGS_LOW + MX_PAIR_REGS_SCALES + 2 * MX_PAIR_REGS_EPILOGUE + 3) / 4, done);
     if (e != cudaSuccess) return e;
-    mx_linear_pair_kernel<KIND, GENERAL><<<2 * (tiles < pairs ? tiles : pairs), MX_PAIR_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_w, map_out, map_xs, map_ws, prm);
+    const unsigned grid = (unsigned)(2 * (tiles < pairs ? tiles : pairs));
+    if (prm.after_x) return mx_launch_dependent(mx_linear_pair_kernel<KIND, GENERAL>, dim3(grid), MX_PAIR_THREADS, Cfg::kSmemBytes, s, map_x, map_w, map_out, map_xs, map_ws, prm);
+    mx_linear_pair_kernel<KIND, GENERAL><<<grid, MX_PAIR_THREADS, Cfg::kSmemBytes, s>>>(map_x, map_w, map_out, map_xs, map_ws, prm);
     return cudaGetLastError();
 }
 
@@ -1635,10 +1643,12 @@ bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count) {
     return m > 128 && ((m + 127) / 128) * ((n + 127) / 128) > sm_count;
 }
 int64_t mx_tile_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * mx_tile_atoms(k) * MX_ATOM; }
-cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles) {
+cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles, bool after_x) {
     if (rows == 0) return cudaSuccess;
     const int64_t blocks = ((rows + 127) / 128 * 32 * ((mx_blocks(k) + 3) / 4) + MX_THREADS - 1) / MX_THREADS;
-    mx_tile_scales_kernel<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), MX_THREADS, 0, s>>>(scales, rows, mx_blocks(k), tiles);
+    const unsigned grid = (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
+    if (after_x) return mx_launch_dependent(mx_tile_scales_kernel, dim3(grid), MX_THREADS, 0, s, scales, rows, mx_blocks(k), tiles);
+    mx_tile_scales_kernel<<<grid, MX_THREADS, 0, s>>>(scales, rows, mx_blocks(k), tiles);
     return cudaGetLastError();
 }
 

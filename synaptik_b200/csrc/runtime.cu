@@ -804,7 +804,8 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                     auto it = x->mx_tiles.find(value);
                     if (it == x->mx_tiles.end() || !kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) continue;
                     if (it->second.last_run != x->run_counter) {
-                        LAUNCH(kern::mx_tile_scales(s, (const uint8_t *)ptr(value), operand ? st.n : st.m, st.k, it->second.ptr));
+                        // W's may be tiled beside the launch that makes x; x's own scales are that launch's output
+                        LAUNCH(kern::mx_tile_scales(s, (const uint8_t *)ptr(value), operand ? st.n : st.m, st.k, it->second.ptr, after_x && operand == 1));
                         it->second.last_run = x->run_counter;
                     }
                     tiles[operand] = it->second.ptr;

@@ -361,3 +361,43 @@ def test_same_bits_every_time(ctx):
     for _ in range(3):
         assert np.array_equal(first, weight_gradient(ctx, "f32", held, (3000, 200), up, 150))
         assert np.array_equal(product, linear(ctx, "f32", x, w, None, None))
+
+
+@pytest.mark.parametrize("m", [40, 300, 2600])
+@pytest.mark.parametrize("order", ["weights fed", "weights first", "x first"])
+def test_quantised_operands_are_complete_before_the_product(ctx, order, m):
+    """Runs in a row whose inputs alternate: no product reads what an earlier run, or only part of this one, has written.
+    Codes and scales are exact and no sum depends on the run, so the results are those of a product of fed codes."""
+    k, n = 288, 2100
+    rng = np.random.default_rng(m)
+    xs = [mixed(rng, m, k) for _ in range(2)]
+    ws = [mixed(rng, n, k) for _ in range(2)]
+    held = [[(*ref.quantize(v.astype(np.float64), "mx4"), v.shape) for v in (x, w)] for x, w in zip(xs, ws)]
+    want = [linear(ctx, "f32", x, w, None, "relu") for x, w in held]
+    g = GraphBuilder()
+    x = g.feed(F32, (m, k))
+    if order == "weights fed":
+        w = g.mx_feed("mx4", (n, k))
+        q = g.mx_quantize(x, "mx4")
+    else:
+        w = g.feed(F32, (n, k))
+        if order == "weights first":
+            w = g.mx_quantize(w, "mx4")
+            q = g.mx_quantize(x, "mx4")
+        else:
+            q = g.mx_quantize(x, "mx4")
+            w = g.mx_quantize(w, "mx4")
+    g.publish(g.mx_linear(q, w, None, "relu", F32))
+    ex = native.Executable(ctx, g.build())
+    feeds = [[ctx.upload(xs[i]), *([ctx.upload(held[i][1][0]), ctx.upload(held[i][1][1])] if order == "weights fed" else [ctx.upload(ws[i])])] for i in range(2)]
+    outs = [ctx.buffer(4 * m * n) for _ in range(8)]
+    try:
+        for run, out in enumerate(outs):
+            ex.enqueue(feeds[run % 2], [out])
+        ex.finish()
+        for run, out in enumerate(outs):
+            assert np.array_equal(out.download(np.float32, (m, n)), want[run % 2].astype(np.float32)), run
+    finally:
+        ex.close()
+        for b in outs + feeds[0] + feeds[1]:
+            b.close()
