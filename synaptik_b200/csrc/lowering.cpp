@@ -813,6 +813,8 @@ Status lower_program(const Program &source, const LoweringOptions &options, Plan
         return false;
     };
 
+    auto same_storage = [&](int u, int v) { return plan.views[u].slot == plan.views[v].slot && plan.views[u].index == plan.views[v].index; };
+
     // engine and operand checks of one GEMM step whose views are assigned
     auto prepare_gemm = [&](Step &st) -> Status {
         {
@@ -1111,6 +1113,13 @@ Status lower_program(const Program &source, const LoweringOptions &options, Plan
                 st.kind = StepKind::MX_LINEAR; st.a = in0; st.scale_a = n.inputs[1]; st.b = n.inputs[2]; st.scale_b = n.inputs[3]; st.out = out0;
                 st.n = ov.shape.back(); st.m = ov.elements() / st.n; st.k = g.values[in0].shape.back() * 2;
                 st.act = (int)n.attrs[0];
+                // The weight is read before the launch in front has ended, so that launch must not make it.  What counts is
+                // the storage: a view (CONTIGUOUS, PERMUTE, EXPAND) of what the quantisation makes is a value of its own.
+                if (!plan.steps.empty() && plan.steps.back().kind == StepKind::MX_QUANTIZE && plan.steps.back().m > 0) {
+                    const Step &made = plan.steps.back();
+                    st.overlaps_quantize = same_storage(st.a, made.out) && same_storage(st.scale_a, made.out2);
+                    for (int w : {st.b, st.scale_b}) st.overlaps_quantize &= !same_storage(w, made.out) && !same_storage(w, made.out2);
+                }
                 finish_step(st);
                 break;
             case Op::MX_WEIGHT_GRADIENT:
@@ -1174,6 +1183,7 @@ std::string describe_plan(const Program &g, const Plan &plan) {
         if (st.kind == StepKind::MX_LINEAR || st.kind == StepKind::MX_WEIGHT_GRADIENT) os << " k=" << st.k << (st.bias >= 0 ? " bias" : "");
         if (st.kind >= StepKind::MX_LINEAR && st.act) os << " act=" << op_name((Op)st.act);
         if (st.kind != StepKind::GEMM && st.kind != StepKind::CROSS_ENTROPY && st.m) os << " m=" << st.m << " n=" << st.n;
+        if (st.overlaps_quantize) os << " overlaps_quantize";
         os << " nodes=[";
         for (size_t i = 0; i < st.nodes.size(); i++) os << (i ? "," : "") << op_name(g.nodes[st.nodes[i]].op);
         os << "]";

@@ -795,10 +795,8 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 break;
             case StepKind::MX_LINEAR: {
                 const uint8_t *tiles[2] = {nullptr, nullptr};
-                // nothing else may come between, and W must not be what that launch makes
-                const Step *before = i > 0 ? &plan.steps[i - 1] : nullptr;
-                const bool after_x = before && before->kind == StepKind::MX_QUANTIZE && before->m > 0 && before->out == st.a && before->out2 == st.scale_a
-                                     && st.b != st.a && st.scale_b != st.scale_a && !time_steps && !x->comm;
+                // no event or collective may come between the two launches
+                const bool after_x = st.overlaps_quantize && !time_steps && !x->comm;
                 for (int operand = 0; operand < 2; operand++) {
                     const int value = operand ? st.scale_b : st.scale_a;
                     auto it = x->mx_tiles.find(value);

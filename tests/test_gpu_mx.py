@@ -401,3 +401,31 @@ def test_quantised_operands_are_complete_before_the_product(ctx, order, m):
         ex.close()
         for b in outs + feeds[0] + feeds[1]:
             b.close()
+
+
+@pytest.mark.parametrize("m", [40, 2600])
+@pytest.mark.parametrize("view", ["contiguous", "permute", "expand"])
+def test_a_view_of_the_quantised_input_as_weight_is_complete_before_the_product(ctx, view, m):
+    """x . x^T whose weight is a view of what the launch in front makes, in runs in a row whose inputs alternate."""
+    k = 288
+    rng = np.random.default_rng(m)
+    xs = [mixed(rng, m, k) for _ in range(2)]
+    held = [(*ref.quantize(v.astype(np.float64), "mx4"), v.shape) for v in xs]
+    want = [linear(ctx, "f32", h, h, None, "relu").astype(np.float32) for h in held]
+    g = GraphBuilder()
+    q = g.mx_quantize(g.feed(F32, (m, k)), "mx4")
+    make = {"contiguous": g.contiguous, "permute": lambda v: g.permute(v, (0, 1)), "expand": lambda v: g.expand(v, v.shape)}[view]
+    g.publish(g.mx_linear(q, program.MxValue("mx4", (m, k), make(q.codes), make(q.scales)), None, "relu", F32))
+    ex = native.Executable(ctx, g.build())
+    feeds = [ctx.upload(x) for x in xs]
+    outs = [ctx.buffer(4 * m * m) for _ in range(8)]
+    try:
+        for run, out in enumerate(outs):
+            ex.enqueue([feeds[run % 2]], [out])
+        ex.finish()
+        for run, out in enumerate(outs):
+            assert np.array_equal(out.download(np.float32, (m, m)), want[run % 2]), run
+    finally:
+        ex.close()
+        for b in outs + feeds:
+            b.close()

@@ -151,3 +151,51 @@ def test_model_graphs():
         program.mlp_training_graph([4, 4], 4, checkpoints="mx4")
     with pytest.raises(ValueError):
         program.mlp_mx_inference_graph([4, 4], (2, 3), arg_max=True)
+
+
+def weight_from(q, how):
+    """A weight over the memory of the quantised tensor q, wholly or in part."""
+    def build(g):
+        fed = g.mx_feed("mx4", q.shape)
+        view = {"contiguous": g.contiguous, "permute": lambda v: g.permute(v, (0, 1)), "expand": lambda v: g.expand(v, v.shape)}
+        if how == "same":
+            return q
+        if how == "fed":
+            return fed
+        if how == "codes only":
+            return program.MxValue("mx4", q.shape, g.contiguous(q.codes), fed.scales)
+        if how == "scales only":
+            return program.MxValue("mx4", q.shape, fed.codes, g.contiguous(q.scales))
+        if how == "twice":
+            return program.MxValue("mx4", q.shape, g.contiguous(g.permute(q.codes, (0, 1))), g.permute(g.contiguous(q.scales), (0, 1)))
+        return program.MxValue("mx4", q.shape, view[how](q.codes), view[how](q.scales))
+    return build
+
+
+@pytest.mark.parametrize("how,overlaps", [("fed", True), ("same", False), ("contiguous", False), ("permute", False), ("expand", False), ("twice", False),
+                                          ("codes only", False), ("scales only", False)])
+def test_a_product_only_overlaps_the_quantisation_that_does_not_make_its_weight(how, overlaps):
+    """The product reads its weight before the launch in front has ended: not where that launch writes the weight's memory."""
+    g = GraphBuilder()
+    x = g.feed(F32, (40, 96))
+    shape = program.MxValue("mx4", (40, 96), None, None)
+    if how == "fed":
+        weight = weight_from(shape, how)(g)
+        q = g.mx_quantize(x, "mx4")
+    else:
+        q = g.mx_quantize(x, "mx4")
+        weight = weight_from(q, how)(g)
+    g.publish(g.mx_linear(q, weight))
+    plan = native.describe(g.build()).splitlines()
+    assert [line.split()[0] for line in plan] == ["mx_quantize", "mx_linear"]
+    assert ("overlaps_quantize" in plan[1]) == overlaps, plan
+
+
+def test_a_product_does_not_overlap_what_is_not_its_quantisation():
+    g = GraphBuilder()
+    x, y = g.feed(F32, (40, 96)), g.feed(F32, (50, 96))
+    q = g.mx_quantize(x, "mx4")
+    w = g.mx_quantize(y, "mx4")             # the weight is made last
+    g.publish(g.mx_linear(q, w))
+    g.publish(g.mx_linear(w, q))            # behind a product, not behind its quantisation
+    assert "overlaps_quantize" not in native.describe(g.build())
