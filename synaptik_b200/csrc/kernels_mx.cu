@@ -1399,15 +1399,17 @@ __global__ void __launch_bounds__(MX_SMALL_THREADS) mx_weight_gradient_small_ker
 }
 
 // The tiles that were cut into slices: their sums in ascending order.  blockIdx.y: the tile; a thread adds four columns.
+// Loads from L2: the launch in front may still write the sums when this one starts, and the read-only path (ld.global.nc)
+// is only defined for memory that nothing writes while the kernel runs.
 __global__ void __launch_bounds__(MX_THREADS) mx_add_slices_kernel(MxGrad prm) {
     mx_dependent_wait();
     const int tile = prm.whole_tiles + blockIdx.y, n0 = tile % prm.tiles_n * 256, k0 = tile / prm.tiles_n * 256;
     const int i = blockIdx.x * MX_THREADS + threadIdx.x, row = i >> 6, col = (i & 63) * 4;
     if (n0 + row >= prm.n || k0 + col >= prm.k) return;
     const float *p = prm.partial + (int64_t)blockIdx.y * prm.slices * 65536 + row * 256 + col;
-    float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+    float4 a = __ldcg(reinterpret_cast<const float4 *>(p));
     for (int q = 1; q < prm.slices; q++) {
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(p + (int64_t)q * 65536));
+        const float4 b = __ldcg(reinterpret_cast<const float4 *>(p + (int64_t)q * 65536));
         a.x = __fadd_rn(a.x, b.x); a.y = __fadd_rn(a.y, b.y); a.z = __fadd_rn(a.z, b.z); a.w = __fadd_rn(a.w, b.w);
     }
     float *out = prm.out + (int64_t)(n0 + row) * prm.k + k0 + col;

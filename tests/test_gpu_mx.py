@@ -429,3 +429,30 @@ def test_a_view_of_the_quantised_input_as_weight_is_complete_before_the_product(
         ex.close()
         for b in outs + feeds:
             b.close()
+
+
+@pytest.mark.parametrize("kind,rows,k,n", [("f32", 2600, 520, 512), ("bf16", 4000, 300, 512), ("f16", 3000, 784, 200)])
+def test_sums_of_slices_are_complete_before_they_are_added(ctx, kind, rows, k, n):
+    """Weight gradients cut into slices of the rows, in runs in a row whose gradients alternate: each run has the bits of
+    a run by itself."""
+    rng = np.random.default_rng(rows)
+    held = random_held(rng, "mx8", (rows, k))
+    fed = [ref.stored(kind, rng.standard_normal((rows, n)))[0] for _ in range(2)]
+    want = [weight_gradient(ctx, kind, held, (rows, k), f, n).astype(np.float32) for f in fed]
+    assert not np.array_equal(want[0], want[1])
+    g = GraphBuilder()
+    g.publish(g.mx_weight_gradient(g.mx_feed("mx8", (rows, k)), g.feed(ref.STORAGE[kind], (rows, n))))
+    ex = native.Executable(ctx, g.build())
+    kept, feeds = [ctx.upload(held[0]), ctx.upload(held[1])], [ctx.upload(f) for f in fed]
+    outs = [ctx.buffer(4 * n * k) for _ in range(8)]
+    try:
+        for run, out in enumerate(outs):
+            ex.enqueue(kept + [feeds[run % 2]], [out])
+        ex.finish()
+        assert ex.launch_count() == 3       # pieces, product, sums of the slices
+        for run, out in enumerate(outs):
+            assert np.array_equal(out.download(np.float32, (n, k)), want[run % 2]), run
+    finally:
+        ex.close()
+        for b in outs + feeds + kept:
+            b.close()
