@@ -159,7 +159,8 @@ struct Executable {
     void *constants = nullptr;              // 8 bytes per constant slot
     std::vector<Planes> planes;
     std::map<PlaneKey, int> plane_index;
-    std::map<int, MxTiles> mx_tiles;        // by the program value of the scales
+    // by the program value of the scales and the blocks of a row that are used: codes of other widths may share the scales
+    std::map<std::pair<int, int64_t>, MxTiles> mx_tiles;
     float *gemm_workspace = nullptr;        // partial products of GEMMs whose contraction is split into slices
     int64_t gemm_workspace_floats = 0;
     int *unit_counters = nullptr;           // one per plan step, zeroed at the start of every run (dynamic tile assignment)
@@ -496,7 +497,7 @@ int32_t prepare_executable(Executable *x) {
         } else if (st.kind == StepKind::MX_LINEAR && st.m > 0 && kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) {
             for (int operand = 0; operand < 2; operand++) {
                 const int64_t bytes = kern::mx_tile_bytes(operand ? st.n : st.m, st.k);
-                MxTiles &tiles = x->mx_tiles[operand ? st.scale_b : st.scale_a];
+                MxTiles &tiles = x->mx_tiles[std::make_pair(operand ? st.scale_b : st.scale_a, mx_blocks(st.k))];
                 if (tiles.ptr) continue;
                 void *p; if (!alloc((uint64_t)bytes, &p)) return ALLOCATION_FAILED;
                 if (cudaMemsetAsync(p, 0, (uint64_t)bytes, ctx->stream) != cudaSuccess) return EXECUTION_FAILED;
@@ -783,7 +784,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 break;
             case StepKind::MX_QUANTIZE: {
                 const View &a = plan.views[st.a];
-                auto tiles = x->mx_tiles.find(st.out2);
+                auto tiles = x->mx_tiles.find(std::make_pair(st.out2, mx_blocks(st.n)));
                 LAUNCH(kern::mx_quantize(s, (int)st.scalar_bits, a.dtype, ptr(st.a), index4(a.shape, &a.strides, nullptr, nullptr, &a.shape),
                                          (uint8_t *)ptr(st.out), (uint8_t *)ptr(st.out2), tiles != x->mx_tiles.end() ? tiles->second.ptr : nullptr));
                 if (tiles != x->mx_tiles.end()) tiles->second.last_run = x->run_counter;
@@ -799,7 +800,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 const bool after_x = st.overlaps_quantize && !time_steps && !x->comm;
                 for (int operand = 0; operand < 2; operand++) {
                     const int value = operand ? st.scale_b : st.scale_a;
-                    auto it = x->mx_tiles.find(value);
+                    auto it = x->mx_tiles.find(std::make_pair(value, mx_blocks(st.k)));
                     if (it == x->mx_tiles.end() || !kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) continue;
                     if (it->second.last_run != x->run_counter) {
                         // W's may be tiled beside the launch that makes x; x's own scales are that launch's output

@@ -456,3 +456,28 @@ def test_sums_of_slices_are_complete_before_they_are_added(ctx, kind, rows, k, n
         ex.close()
         for b in outs + feeds + kept:
             b.close()
+
+
+@pytest.mark.parametrize("order", [(32, 128), (128, 32), (160, 256)])
+def test_products_that_share_scales_take_as_many_as_they_have_blocks(ctx, order):
+    """One tensor of scales serves codes of other widths, as long as they fill the same row of scales: each product reads
+    the blocks it has, whatever the one before it read."""
+    m, n = 3000, 1000                   # enough tiles for scales in tiles
+    rng = np.random.default_rng(order[0])
+    wide = max(order)
+    w_codes, w_scales = random_held(rng, "mx4", (n, wide))
+    w_scales[::7, wide // 32 - 1] = 255         # NaN for the wide product, nothing to the narrow one
+    xs = {k: random_held(rng, "mx4", (m, k)) for k in order}
+    g = GraphBuilder()
+    scales = g.feed(program.U8, w_scales.shape)
+    feeds, want = [w_scales], []
+    for k in order:
+        x = g.mx_feed("mx4", (m, k))
+        codes = g.feed(program.U8, (n, k // 2))
+        g.publish(g.mx_linear(x, program.MxValue("mx4", (n, k), codes, scales)))
+        feeds += [*xs[k], w_codes[:, :k // 2]]
+        padded = w_scales.copy()
+        padded[:, k // 32:] = 0
+        want.append(linear(ctx, "f32", (*xs[k], (m, k)), (np.ascontiguousarray(w_codes[:, :k // 2]), padded, (n, k)), None, None))
+    for got, expected in zip(run_image(ctx, g, feeds), want):
+        assert np.array_equal(got, expected.astype(np.float32), equal_nan=True)
