@@ -12,6 +12,10 @@ nearest, ties to even.  Kinds of cases:
   activation  dZ = G * act'(Z8): the gradient of an activation from the 8-bit checkpoint of its input
 
 `own` false: elementary torch operations.  `own` true: the calls a user makes of this framework.
+
+The framework launches on a stream of its own that torch's stream does not wait for, and `run` only enqueues, like a
+program that keeps several passes in flight.  Whoever reads its results waits first: for the device, for `context()`, or
+with the `finish` of the state's plan, which also raises what the kernels reported.
 """
 import math
 
@@ -211,6 +215,7 @@ class Plan:
         fed = [Memory(tensor.nbytes) for tensor in inputs]
         for memory, tensor in zip(fed, inputs):
             memory.tensor(tensor.shape, tensor.dtype).copy_(tensor)
+        torch.cuda.synchronize()        # the framework's stream does not wait for torch's
         made = [Memory(math.prod(shape) * dtype.itemsize) for shape, dtype in outputs]
         self.results = [memory.tensor(*out) for memory, out in zip(made, outputs)]
         self.fed, self.inputs, self.outputs = fed, [m.buffer for m in fed], [m.buffer for m in made]
@@ -220,9 +225,16 @@ class Plan:
         self.executable.enqueue(self.inputs, self.outputs)
         return self.results
 
+    def finish(self):
+        """Waits for the enqueued passes; raises when a kernel reported an error."""
+        self.executable.finish()
+
     def __del__(self):
         if hasattr(self, "executable"):
-            self.executable.close()
+            try:
+                self.finish()
+            finally:
+                self.executable.close()
 
 
 def prepare(case, seed):
