@@ -208,7 +208,7 @@ cudaError_t argmax_rows_low(cudaStream_t s, int kind, const void *x, int64_t *ou
 // words.  `format` 4 or 8 bits.
 // ix: the iteration space of x, last axis in shape[3], strides in sa; codes and scales dense.  tiles (optional):
 // the scales once more in the order the two-SM product reads, mx_tile_bytes(rows, k) bytes that were zero at first.
-cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles = nullptr);
+cudaError_t mx_quantize(cudaStream_t s, int format, bool keep_nonzero, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles = nullptr);
 cudaError_t mx_restore(cudaStream_t s, int format, DType dtype, const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *out);
 // out = g * act'(z), z held in 8 bits; g and out dense [rows, cols] of one type.
 cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const uint8_t *codes, const uint8_t *scales, const void *g,

@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(MX_THREADS) mx_tile_scales_kernel(const uint8_
 // x -> codes, scales.  Bound by HBM: the wide tensor once, an eighth to a half of it written.  A thread takes 32 aligned
 // bytes (8 FLOAT32 or 16 16-bit elements) where rows allow, 8 elements through shared memory elsewhere.  Positions in 32
 // bits where they fit: with 64-bit ones and 8 elements the 16-bit types were bound by the instructions around them.
-template <int FORMAT, int KIND, bool VEC, typename I>
+// KEEP_NONZERO is a kernel of its own for the same reason: as a flag it cost the 16-bit types 2 %.
+template <int FORMAT, int KIND, bool VEC, bool KEEP_NONZERO, typename I>
 __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename MxElement<KIND>::type *__restrict__ x, Index4 ix, MxRows<I> r, int64_t row_step, int even,
                                                                  uint8_t *__restrict__ codes, uint8_t *__restrict__ scales, uint8_t *__restrict__ tiles, uint32_t atoms) {
     constexpr int E = VEC && KIND != 0 ? 16 : 8, LANES = MX_BLOCK / E;      // lanes per block
@@ -300,6 +301,11 @@ __global__ void __launch_bounds__(MX_THREADS) mx_quantize_kernel(const typename 
         if (byte == 255u) {
 #pragma unroll
             for (int i = 0; i < E; i++) v[i] = 0.0f;
+        }
+        if constexpr (KEEP_NONZERO) {
+            const float least = (FORMAT == 4 ? 0.5f : 0.001953125f) * mx_scale_value(byte);     // the smallest element, 2^-136 or more: exact; no block of NaN is below it
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = v[i] != 0.0f && fabsf(v[i]) < least ? copysignf(least, v[i]) : v[i];
         }
         // the inverse scale 2^(127 - byte) is a normal number for every other byte that occurs; a product with it is
         // exact, or below half the smallest element
@@ -1454,7 +1460,7 @@ static cudaError_t mx_launch_dependent(void (*kernel)(Args...), dim3 grid, int t
 
 #define MX_KINDS(dtype, CALL) ((dtype) == DType::F32 ? CALL(0) : (dtype) == DType::BF16 ? CALL(1) : (dtype) == DType::F16 ? CALL(2) : cudaErrorInvalidValue)
 
-template <int FORMAT, int KIND>
+template <int FORMAT, int KIND, bool KEEP>
 static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles) {
     using T = typename MxElement<KIND>::type;
     const int64_t rows = ix.shape[0] * ix.shape[1] * ix.shape[2], cols = ix.shape[3];
@@ -1477,18 +1483,18 @@ static cudaError_t launch_mx_quantize(cudaStream_t s, const void *x, const Index
     const uint32_t atoms = (uint32_t)mx_tile_atoms(cols);
     const auto launch = [&](auto kernel, auto shape) { kernel<<<grid, MX_THREADS, 0, s>>>((const T *)x, ix, shape, row_step, even ? 1 : 0, codes, scales, tiles, atoms); };
     if (mx_narrow_rows(r, c)) {
-        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT, E));
-        else launch(mx_quantize_kernel<FORMAT, KIND, false, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, KEEP, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT, E));
+        else launch(mx_quantize_kernel<FORMAT, KIND, false, KEEP, uint32_t>, mx_rows<uint32_t>(r, c, FORMAT));
     } else {
-        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, int64_t>, mx_rows<int64_t>(r, c, FORMAT, E));
-        else launch(mx_quantize_kernel<FORMAT, KIND, false, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
+        if (vec) launch(mx_quantize_kernel<FORMAT, KIND, true, KEEP, int64_t>, mx_rows<int64_t>(r, c, FORMAT, E));
+        else launch(mx_quantize_kernel<FORMAT, KIND, false, KEEP, int64_t>, mx_rows<int64_t>(r, c, FORMAT));
     }
     return cudaGetLastError();
 }
 
-cudaError_t mx_quantize(cudaStream_t s, int format, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles) {
-#define CALL4(KIND) launch_mx_quantize<4, KIND>(s, x, ix, codes, scales, tiles)
-#define CALL8(KIND) launch_mx_quantize<8, KIND>(s, x, ix, codes, scales, tiles)
+cudaError_t mx_quantize(cudaStream_t s, int format, bool keep_nonzero, DType dtype, const void *x, const Index4 &ix, uint8_t *codes, uint8_t *scales, uint8_t *tiles) {
+#define CALL4(KIND) (keep_nonzero ? launch_mx_quantize<4, KIND, true>(s, x, ix, codes, scales, tiles) : launch_mx_quantize<4, KIND, false>(s, x, ix, codes, scales, tiles))
+#define CALL8(KIND) (keep_nonzero ? launch_mx_quantize<8, KIND, true>(s, x, ix, codes, scales, tiles) : launch_mx_quantize<8, KIND, false>(s, x, ix, codes, scales, tiles))
     return format == 4 ? MX_KINDS(dtype, CALL4) : format == 8 ? MX_KINDS(dtype, CALL8) : cudaErrorInvalidValue;
 #undef CALL4
 #undef CALL8

@@ -1095,7 +1095,7 @@ Status lower_program(const Program &source, const LoweringOptions &options, Plan
                 for (int v : n.outputs) assign_output(v);
                 st.kind = StepKind::MX_QUANTIZE; st.a = in0; st.out = out0; st.out2 = n.outputs[1];
                 st.n = g.values[in0].shape.back(); st.m = g.values[in0].elements() / st.n;
-                st.scalar_bits = n.attrs[0];
+                st.scalar_bits = n.attrs[0]; st.keep_nonzero = n.attr_i(1) == 1;
                 finish_step(st);
                 break;
             case Op::MX_RESTORE:
@@ -1183,6 +1183,7 @@ std::string describe_plan(const Program &g, const Plan &plan) {
         if (st.kind == StepKind::MX_LINEAR || st.kind == StepKind::MX_WEIGHT_GRADIENT) os << " k=" << st.k << (st.bias >= 0 ? " bias" : "");
         if (st.kind >= StepKind::MX_LINEAR && st.act) os << " act=" << op_name((Op)st.act);
         if (st.kind != StepKind::GEMM && st.kind != StepKind::CROSS_ENTROPY && st.m) os << " m=" << st.m << " n=" << st.n;
+        if (st.keep_nonzero) os << " keep_nonzero";
         if (st.overlaps_quantize) os << " overlaps_quantize";
         os << " nodes=[";
         for (size_t i = 0; i < st.nodes.size(); i++) os << (i ? "," : "") << op_name(g.nodes[st.nodes[i]].op);

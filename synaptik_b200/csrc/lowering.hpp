@@ -55,6 +55,7 @@ struct Step {
     int out = -1, out2 = -1, out3 = -1;   // output value ids
     int bias = -1, mask = -1;       // GEMM epilogue operands
     int scale_a = -1, scale_b = -1; // scale bytes of block-scaled operands a and b
+    bool keep_nonzero = false;      // MX_QUANTIZE: no element that is not zero becomes zero
     bool overlaps_quantize = false; // MX_LINEAR: may start, and read its weight, while the MX_QUANTIZE step before it makes a
     bool relu = false;
     int act = 0;                    // GEMM epilogue activation other than ReLU: the wire code of TANH, SIGMOID, SILU, GELU_TANH or GELU

@@ -287,8 +287,9 @@ Status check_node(const Program &g, int index, std::string &message) {
             return OK;
         }
         case Op::MX_QUANTIZE: {
-            if (!need(1, 2) || n.attrs.size() != 1) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
+            if (!need(1, 2) || n.attrs.size() < 1 || n.attrs.size() > 2) FAIL(GRAPH_COMPILATION_FAILED, name << ": arity");
             if (n.attrs[0] != 4 && n.attrs[0] != 8) FAIL(UNSUPPORTED_OPERATION, name << ": formats of 4 or 8 bits");
+            if (n.attrs.size() == 2 && n.attrs[1] > 1) FAIL(UNSUPPORTED_OPERATION, name << ": keep nonzero is 0 or 1");
             if (!dtype_floating(in(0).dtype) || out(0).dtype != DType::U8 || out(1).dtype != DType::U8) FAIL(UNSUPPORTED_OPERATION, name << ": needs a floating input and U8 results");
             if (in(0).shape.empty() || in(0).shape.size() > 4) FAIL(UNSUPPORTED_SHAPE, name << ": rank outside 1..4");
             if (Status s = check_mx_pair(out(0), out(1), in(0).shape, n.attr_i(0), name, message)) return s;

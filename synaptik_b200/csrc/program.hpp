@@ -68,8 +68,10 @@ enum class Op : uint32_t {
 //   scales  [.., mx_scale_bytes(K)]          K / 32 rounded up to a multiple of four; bytes past the last block zero
 // MX_QUANTIZE chooses the least scale, from 2^-127 up, under which the block's largest magnitude does not exceed
 // the element type's (6 or 448): nothing saturates.  Elements round to nearest even.  A block that holds an
-// infinity or a NaN gets scale 255 and stands for NaN throughout.
-//   MX_QUANTIZE             x (FLOAT32 / BFLOAT16 / FLOAT16) -> codes, scales          attributes: format (4 or 8)
+// infinity or a NaN gets scale 255 and stands for NaN throughout.  With `keep nonzero` an element that is not zero does
+// not become zero: below the type's smallest magnitude (0.5 or 2^-9 under the scale) it takes that magnitude, so the
+// signs of a checkpoint are those of the tensor, which a ReLU gate reads.
+//   MX_QUANTIZE             x (FLOAT32 / BFLOAT16 / FLOAT16) -> codes, scales          attributes: format (4 or 8), optionally keep nonzero (0 or 1)
 //   MX_RESTORE              codes, scales -> values                                    attributes: format, K
 //   MX_LINEAR               codes, scales of x [.., M, K] and of W [N, K] (format 4), optional bias [N]
 //                           -> act(x W^T + bias)                                       attributes: activation (0 or its wire code)

@@ -785,7 +785,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
             case StepKind::MX_QUANTIZE: {
                 const View &a = plan.views[st.a];
                 auto tiles = x->mx_tiles.find(std::make_pair(st.out2, mx_blocks(st.n)));
-                LAUNCH(kern::mx_quantize(s, (int)st.scalar_bits, a.dtype, ptr(st.a), index4(a.shape, &a.strides, nullptr, nullptr, &a.shape),
+                LAUNCH(kern::mx_quantize(s, (int)st.scalar_bits, st.keep_nonzero, a.dtype, ptr(st.a), index4(a.shape, &a.strides, nullptr, nullptr, &a.shape),
                                          (uint8_t *)ptr(st.out), (uint8_t *)ptr(st.out2), tiles != x->mx_tiles.end() ? tiles->second.ptr : nullptr));
                 if (tiles != x->mx_tiles.end()) tiles->second.last_run = x->run_counter;
                 break;

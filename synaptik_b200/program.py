@@ -331,12 +331,14 @@ class GraphBuilder:
         shape = tuple(int(d) for d in shape)
         return MxValue(fmt, shape, self.feed(U8, shape[:-1] + (mx_code_bytes(fmt, shape[-1]),)), self.feed(U8, shape[:-1] + (mx_scale_bytes(shape[-1]),)))
 
-    def mx_quantize(self, x: Value, fmt: str) -> MxValue:
+    def mx_quantize(self, x: Value, fmt: str, keep_nonzero: bool = False) -> MxValue:
         """MX_QUANTIZE: x in 4 or 8 bits per element.  Each block of 32 takes the least power-of-two scale under
-        which nothing saturates and rounds to nearest even; a block with an infinity or a NaN stands for NaN."""
+        which nothing saturates and rounds to nearest even; a block with an infinity or a NaN stands for NaN.
+        ``keep_nonzero``: what is not zero does not become zero but at least the smallest element of its sign."""
         codes = self._value(U8, tuple(x.shape[:-1]) + (mx_code_bytes(fmt, x.shape[-1]),))
         scales = self._value(U8, tuple(x.shape[:-1]) + (mx_scale_bytes(x.shape[-1]),))
-        self.nodes.append(_Node(OPS["MX_QUANTIZE"], [x.index], [codes.index, scales.index], [MX_FORMATS[fmt]]))
+        self.nodes.append(_Node(OPS["MX_QUANTIZE"], [x.index], [codes.index, scales.index],
+                                [MX_FORMATS[fmt]] + ([1] if keep_nonzero else [])))
         return MxValue(fmt, tuple(x.shape), codes, scales)
 
     def mx_restore(self, x: MxValue, dtype: int = F32) -> Value:
@@ -361,8 +363,9 @@ class GraphBuilder:
         return self._node("MX_WEIGHT_GRADIENT", [checkpoint.codes, checkpoint.scales, upstream], F32, (upstream.shape[-1], checkpoint.shape[-1]), [checkpoint.shape[-1]])
 
     def mx_activation_gradient(self, kind: str, checkpoint: MxValue, upstream: Value) -> Value:
-        """MX_ACTIVATION_GRADIENT: upstream * act'(z) from the 8-bit checkpoint of the pre-activation z (for "relu"
-        the activation's own checkpoint serves as well: it is positive exactly where the held z is)."""
+        """MX_ACTIVATION_GRADIENT: upstream * act'(z) from the 8-bit checkpoint of the pre-activation z.  For "relu" the
+        checkpoint of relu(z) serves as well, and taken with keep_nonzero it is positive exactly where z is; without, a z
+        below about 2^-18 of its block's largest value may be held as 0, which closes its gate."""
         if checkpoint.format != "mx8" or checkpoint.shape != tuple(upstream.shape):
             raise ValueError("MX_ACTIVATION_GRADIENT needs an 8-bit checkpoint of the upstream gradient's shape")
         return self._node("MX_ACTIVATION_GRADIENT", [checkpoint.codes, checkpoint.scales, upstream], upstream.dtype, upstream.shape, [OPS[kind.upper()]])
@@ -637,7 +640,8 @@ def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_
 
     ``checkpoints="mx8"`` (no counterpart in the reference): the backward pass reads the layers' inputs, and the
     pre-activations of activations other than ReLU, from 8-bit checkpoints taken in the forward pass, so nothing keeps
-    the FLOAT32 tensors; the forward pass and the objective are the same."""
+    the FLOAT32 tensors; the forward pass and the objective are the same.  A ReLU's gate is exact: its output is held with
+    ``keep_nonzero``."""
     if checkpoints not in (None, "mx8"):
         raise ValueError("checkpoints must be None or 'mx8'")
     g = GraphBuilder()
@@ -663,7 +667,8 @@ def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_
     a = x
     for l, (w, b) in enumerate(params):
         if checkpoints:
-            held_inputs.append(g.mx_quantize(a, checkpoints))
+            # what a ReLU passed on is also its gate, so what is open stays positive
+            held_inputs.append(g.mx_quantize(a, checkpoints, keep_nonzero=activation == "relu" and l > 0))
         wt, z = g.linear(a, w, b)
         wts.append(wt)
         zs.append(z)
@@ -687,7 +692,7 @@ def mlp_training_graph(dims: Sequence[int], batch: int, loss: str = "ce", label_
         else:
             dx, dw, db = g.linear_backward(acts[l], wts[l], dz, need_dx=l > 0, bias=bias)
         grads[2 * l], grads[2 * l + 1] = dw, db
-        if l > 0 and checkpoints:       # a ReLU's own output is positive exactly where its input is
+        if l > 0 and checkpoints:       # a ReLU's output is positive exactly where its input is, and so is what is held of it
             dz = g.mx_activation_gradient(activation, held_inputs[l] if activation == "relu" else held_zs[l - 1], dx)
         elif l > 0:
             dz = g.activation_backward(activation, zs[l - 1], acts[l], dx)

@@ -481,3 +481,49 @@ def test_products_that_share_scales_take_as_many_as_they_have_blocks(ctx, order)
         want.append(linear(ctx, "f32", (*xs[k], (m, k)), (np.ascontiguousarray(w_codes[:, :k // 2]), padded, (n, k)), None, None))
     for got, expected in zip(run_image(ctx, g, feeds), want):
         assert np.array_equal(got, expected.astype(np.float32), equal_nan=True)
+
+
+def keep_nonzero(x, codes, fmt):
+    """Codes in which what is not zero takes at least the smallest element of its sign; blocks of NaN stay as they are."""
+    b = ref.blocked(x)
+    tiny = ((b != 0) & np.isfinite(b).all(-1, keepdims=True)).reshape(x.shape[:-1] + (-1,))
+    negative = np.signbit(b).reshape(tiny.shape)
+    if fmt == "mx8":
+        return np.where(tiny & (codes & 127 == 0), np.where(negative, 129, 1), codes).astype(np.uint8)
+    each = np.stack((codes & 15, codes >> 4), -1).reshape(tiny.shape)
+    each = np.where(tiny & (each & 7 == 0), np.where(negative, 9, 1), each).astype(np.uint8)
+    return each[..., 0::2] | (each[..., 1::2] << 4)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("fmt", ["mx4", "mx8"])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 33), (64, 784), (33, 785), (300, 256)])
+def test_quantize_keeps_what_is_not_zero(ctx, kind, fmt, shape):
+    rng = np.random.default_rng(shape[-1])
+    x = mixed(rng, *shape) * np.exp2(rng.integers(-40, 1, shape))       # most of a block far below its largest
+    x[..., ::5] = 0
+    x[..., 1::7] *= -1
+    fed, exact = ref.stored(kind, x)
+    g = GraphBuilder()
+    held = g.mx_quantize(g.feed(ref.STORAGE[kind], shape), fmt, keep_nonzero=True)
+    g.publish(held.codes)
+    g.publish(held.scales)
+    codes, scales = run_image(ctx, g, [fed])
+    want_codes, want_scales = ref.quantize(exact, fmt)
+    assert np.array_equal(scales, want_scales)
+    assert np.array_equal(codes, keep_nonzero(exact, want_codes, fmt))
+    back = ref.values(codes, scales, fmt, shape[-1])        # blocks with an infinity (large FLOAT16 values) are NaN
+    assert np.array_equal(np.sign(back[~np.isnan(back)]), np.sign(exact[~np.isnan(back)]))
+
+
+def test_quantize_keeps_special_blocks(ctx):
+    """Zeros of both signs, blocks of NaN, numbers that vanish under their block's scale in FLOAT32."""
+    x = special_blocks().reshape(-1, 32)
+    x = np.concatenate([x, [np.concatenate([[f], np.full(31, -2.0 ** -149)]) for f in (3e38, 1.0, 2.0 ** -149)]]).astype(np.float32)
+    g = GraphBuilder()
+    held = g.mx_quantize(g.feed(F32, x.shape), "mx8", keep_nonzero=True)
+    g.publish(held.codes)
+    g.publish(held.scales)
+    codes, scales = run_image(ctx, g, [x])
+    want_codes, want_scales = ref.quantize(x, "mx8")
+    assert np.array_equal(scales, want_scales) and np.array_equal(codes, keep_nonzero(x.astype(np.float64), want_codes, "mx8"))

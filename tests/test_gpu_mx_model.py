@@ -236,3 +236,27 @@ def test_two_threads_with_a_context_each(ctx):
     first = results[0][0]
     for got in results[0] + results[1]:
         assert all(np.array_equal(a, b) for a, b in zip(first, got))
+
+
+def test_small_activations_beside_large_ones_keep_their_gradient(ctx):
+    """One unit at 1000 and others at 1e-6 to 1e-3 in a block: each open unit's gradient is what FLOAT32 checkpoints give it
+    (the inputs are exact in 8 bits), each closed unit's is zero."""
+    hidden = 64
+    target = np.zeros((4, 1), dtype=np.float32)
+    x = np.ones((4, 2), dtype=np.float32)
+    w0 = np.zeros((hidden, 2), dtype=np.float32)
+    w0[:, 0] = np.where(np.arange(hidden) % 3 == 0, -1, 1) * np.geomspace(1e-6, 1e-3, hidden)
+    w0[0, 0] = w0[33, 0] = 1000
+    w1 = np.linspace(0.5, 1.5, hidden, dtype=np.float32)[None]
+    grads = []
+    for kind in (None, "mx8"):
+        model = nn.Model([2, hidden, 1], ctx, checkpoints=kind)
+        model.load_parameters([w0, np.zeros(hidden, np.float32), w1, np.zeros(1, np.float32)])
+        model.configure_training("mse", nn.Sgd(0.01))
+        grads.append(model.gradients(x, target)[1])
+        model.close()
+    opened = w0[:, 0] > 0
+    assert (grads[1][0][opened] != 0).all() and (grads[1][0][~opened] == 0).all()
+    # four equal rows: each result is a sum of at most 12 exact products, one rounding each
+    assert np.allclose(grads[1][0], grads[0][0], rtol=16 * 2.0 ** -23, atol=0)
+    assert np.allclose(grads[1][1], grads[0][1], rtol=16 * 2.0 ** -23, atol=0)

@@ -199,3 +199,18 @@ def test_a_product_does_not_overlap_what_is_not_its_quantisation():
     g.publish(g.mx_linear(q, w))
     g.publish(g.mx_linear(w, q))            # behind a product, not behind its quantisation
     assert "overlaps_quantize" not in native.describe(g.build())
+
+
+def test_gates_of_relu_checkpoints_stay_open():
+    """What a ReLU passed on is its gate in the backward pass: it is held so that nothing positive becomes zero."""
+    steps = lambda activation: [line for line in native.describe(program.mlp_training_graph([784, 256, 256, 10], 64, activation=activation, checkpoints="mx8").image).splitlines()       # noqa: E731
+                                if line.startswith("mx_quantize")]
+    assert ["keep_nonzero" in line for line in steps("relu")] == [False, True, True]       # the model's input is no gate
+    assert not any("keep_nonzero" in line for line in steps("gelu"))
+
+
+@pytest.mark.parametrize("attrs,want", [([8], 0), ([8, 0], 0), ([8, 1], 0), ([4, 1], 0), ([8, 2], 13), ([8, 1, 0], 9), ([], 9)])
+def test_attributes_of_quantise(attrs, want):
+    g = GraphBuilder()
+    raw(g, "MX_QUANTIZE", [g.feed(F32, (4, 32))], [(U8, (4, 16 if attrs[:1] == [4] else 32)), (U8, (4, 4))], attrs)
+    assert status(g) == want
