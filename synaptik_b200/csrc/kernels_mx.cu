@@ -482,6 +482,11 @@ __device__ __noinline__ float4 mx_activate4(int act, float4 z) {
 // order [lane = row mod 32][column = row / 32], four contraction blocks per 32-bit word.
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_BK = 256;                      // contraction steps per k-block
+// k-blocks per partial sum in tensor memory, by the type of the result: 64 MMAs for FLOAT32, 256 for 16 bits.  Tensor
+// memory adds with truncation: two-SM sums of positive terms fell short by 0.1 units of 2^-23 per MMA and more as they grow (6 units
+// after 64 MMAs, 2600 after 16384).  Longer contractions add their partial sums in FP32 registers (8 units), each
+// at the price of a stop of the MMAs: 8192 x 16384 x 4096 in FLOAT32 takes 6 % longer than with one sum (237 against 224 us).
+template <int KIND> constexpr int mx_chunk() { return KIND == 0 ? 16 : 64; }
 
 // Instruction descriptor of kind::mxf4: E2M1 x E2M1 (format 1), UE8M0 scales (bit 23), K-major, M rows, N columns;
 // sf: which two of the four scale bytes per word the 64 contraction steps use (0 or 2).
@@ -583,22 +588,22 @@ template <int BN, int KIND>
 __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, MxLinear prm, int slices) {
     using Cfg = MxFewConfig<BN>;
     using T = typename MxElement<KIND>::type;
-    constexpr int S = Cfg::kStages;
+    constexpr int S = Cfg::kStages, CHUNK = mx_chunk<KIND>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * (Cfg::kStageBytes + Cfg::kScaleBytes));
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 2);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bar_base = smem_u32(bars), smem_base = smem_u32(smem), scale_base = smem_base + S * Cfg::kStageBytes;
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (S + s); };
     auto scale_bar = [&](int s) { return bar_base + 8u * (2 * S + s); };
-    const uint32_t done_bar = bar_base + 8u * (3 * S);
+    const uint32_t done_bar = bar_base + 8u * (3 * S), drained_bar = bar_base + 8u * (3 * S + 1);     // of a partial sum
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); mbar_init(scale_bar(s), 2); }
-        mbar_init(done_bar, 1);
+        mbar_init(done_bar, 1); mbar_init(drained_bar, 4);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -649,6 +654,11 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
             const uint32_t id0 = mx_idesc(128, BN, 0), id2 = mx_idesc(128, BN, 2);
             bool ok = true;
             for (int kb = kb0; kb < kb1; kb++) {
+                const int in_chunk = (kb - kb0) % CHUNK, chunk = (kb - kb0) / CHUNK;
+                if (in_chunk == 0 && chunk > 0) {
+                    umma_commit(done_bar);
+                    if (!mbar_wait(drained_bar, (uint32_t)(chunk - 1) & 1u, abort_flag)) { ok = false; break; }
+                }
                 if (!mbar_wait(full_bar(stage), phase, abort_flag) || !mbar_wait(scale_bar(stage), phase, abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes, ps = scale_base + stage * Cfg::kScaleBytes;
@@ -658,7 +668,7 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
 #pragma unroll
                 for (int k4 = 0; k4 < 4; k4++)
                     mx_mma<0>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 4,
-                              (kb != kb0 || k4 != 0) ? 1u : 0u);
+                              (in_chunk != 0 || k4 != 0) ? 1u : 0u);
                 umma_commit(empty_bar(stage));
                 if (++stage == S) { stage = 0; phase ^= 1u; }
             }
@@ -693,18 +703,28 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
     bool ok = true;
     float *partial = reinterpret_cast<float *>(smem);       // [BN][128]
     if (warp >= 4) {
-        ok = kb1 == kb0 || mbar_wait(done_bar, 0u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        tc_fence_after();
         const int row = (warp & 3) * 32 + lane;             // of W's tile
+        const uint32_t taddr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        float sum[BN];
 #pragma unroll
-        for (int c = 0; c < BN / 16; c++) {
-            float t[16];
-            if (ok && kb1 > kb0) tmem_load16(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(c * 16), t);
-            else for (int i = 0; i < 16; i++) t[i] = 0.0f;
+        for (int i = 0; i < BN; i++) sum[i] = -0.0f;        // what adds up to the first partial sum as it is
+        for (int kb = kb0; kb < kb1; kb += CHUNK) {
+            ok = __all_sync(0xffffffffu, mbar_wait(done_bar, (uint32_t)((kb - kb0) / CHUNK) & 1u, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < 16; i++) partial[(c * 16 + i) * 128 + row] = t[i];
+            for (int c = 0; c < BN / 16; c++) {
+                float t[16];
+                tmem_load16(taddr + (uint32_t)(c * 16), t);
+#pragma unroll
+                for (int i = 0; i < 16; i++) sum[c * 16 + i] = __fadd_rn(sum[c * 16 + i], t[i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(drained_bar);
         }
+#pragma unroll
+        for (int i = 0; i < BN; i++) partial[i * 128 + row] = sum[i];
     }
     tc_fence_before();
     if (slices > 1) cluster_sync_all(); else __syncthreads();
@@ -850,7 +870,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
         const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ws, MxLinear prm) {
     using Cfg = MxPairConfig;
     using T = typename MxElement<KIND>::type;
-    constexpr int S = Cfg::kStages, R = Cfg::kScaleSlots, BN = Cfg::BN;
+    constexpr int S = Cfg::kStages, R = Cfg::kScaleSlots, BN = Cfg::BN, CHUNK = mx_chunk<KIND>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S * Cfg::kStageBytes + R * Cfg::kScaleBytes + Cfg::kStagingBytes);
@@ -942,23 +962,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                 const uint32_t id0 = mx_idesc(256, BN, 0), id2 = mx_idesc(256, BN, 2);
                 int stage = 0; uint32_t phase = 0, done = 0;
                 bool ok = true;
-                for (int tile = pair; tile < total_tiles && ok; tile += pairs, done++) {
-                    if (!mbar_wait_cluster(acc_empty_bar, (done & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    for (int kb = 0; kb < kb_count; kb++) {
-                        if (!mbar_wait(scale_bar(stage), phase, abort_flag) || !mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                for (int tile = pair; tile < total_tiles && ok; tile += pairs) {
+                    for (int kb0 = 0; kb0 < kb_count && ok; kb0 += CHUNK, done++) {
+                        if (!mbar_wait_cluster(acc_empty_bar, (done & 1u) ^ 1u, abort_flag)) { ok = false; break; }
                         tc_fence_after();
-                        const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes;
-                        const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
+                        const int kb1 = kb0 + CHUNK < kb_count ? kb0 + CHUNK : kb_count;
+                        for (int kb = kb0; kb < kb1; kb++) {
+                            if (!mbar_wait(scale_bar(stage), phase, abort_flag) || !mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                            tc_fence_after();
+                            const uint32_t pa = smem_base + stage * Cfg::kStageBytes, pb = pa + Cfg::kABytes;
+                            const uint32_t ts = tmem_base + BN + (uint32_t)(stage * Cfg::kScaleCols);
 #pragma unroll
-                        for (int k4 = 0; k4 < 4; k4++)
-                            mx_mma<1>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 8,
-                                      (kb != 0 || k4 != 0) ? 1u : 0u);
-                        umma_commit_pair(empty_bar(stage));
-                        umma_commit_pair(map_to_rank(empty_bar(stage), 1));
-                        if (++stage == S) { stage = 0; phase ^= 1u; }
+                            for (int k4 = 0; k4 < 4; k4++)
+                                mx_mma<1>(tmem_base, mx_operand_desc(pa + k4 * 32), mx_operand_desc(pb + k4 * 32), (k4 & 1) ? id2 : id0, ts + (k4 >> 1) * 4, ts + 8 + (k4 >> 1) * 8,
+                                          (kb != kb0 || k4 != 0) ? 1u : 0u);
+                            umma_commit_pair(empty_bar(stage));
+                            umma_commit_pair(map_to_rank(empty_bar(stage), 1));
+                            if (++stage == S) { stage = 0; phase ^= 1u; }
+                        }
+                        if (ok) { umma_commit_pair(acc_full_bar); umma_commit_pair(map_to_rank(acc_full_bar, 1)); }
                     }
-                    if (ok) { umma_commit_pair(acc_full_bar); umma_commit_pair(map_to_rank(acc_full_bar, 1)); }
                 }
             }
         }
@@ -999,7 +1022,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MX_PAIR_REGS_EPILOGUE));
         const int quarter = warp & 3, half = (warp - 8) >> 2;
         uint32_t done = 0;
-        for (int tile = pair; tile < total_tiles; tile += pairs, done++) {
+        bool ok = true;
+        for (int tile = pair; tile < total_tiles && ok; tile += pairs) {
             int mi, ni;
             tile_origin(tile, prm.tiles_m, prm.tiles_n, prm.group_n, mi, ni);
             const int row0 = mi * 256 + (int)rank * 128 + quarter * 32, col0 = ni * BN + half * 128;
@@ -1012,18 +1036,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
                 if (c + 2 < prm.n) bias_lane.z = mx_load<KIND>(b + c + 2);
                 if (c + 3 < prm.n) bias_lane.w = mx_load<KIND>(b + c + 3);
             }
-            if (!mx_warp_wait(acc_full_bar, done & 1u, abort_flag, lane)) break;
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+            ok = mx_warp_wait(acc_full_bar, done & 1u, abort_flag, lane);
+            if (!ok) break;
             tc_fence_after();
             float sum[128];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 float t[32];
-                tmem_load32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128 + c * 32), t);
+                tmem_load32(taddr + (uint32_t)(c * 32), t);
 #pragma unroll
                 for (int i = 0; i < 32; i++) sum[c * 32 + i] = t[i];
             }
             tc_fence_before();
             mx_arrive_rank(acc_empty_bar, 0);
+            done++;
+            for (int kb = CHUNK; kb < kb_count; kb += CHUNK, done++) {
+                ok = mx_warp_wait(acc_full_bar, done & 1u, abort_flag, lane);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    float t[16];
+                    tmem_load16(taddr + (uint32_t)(c * 16), t);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) sum[c * 16 + i] = __fadd_rn(sum[c * 16 + i], t[i]);
+                }
+                tc_fence_before();
+                mx_arrive_rank(acc_empty_bar, 0);
+            }
+            if (!ok) break;
             mx_emit<KIND, GENERAL>(prm, &map_out, staging_base + (uint32_t)((warp - 8) * 4096), row0, col0, sum, bias_lane, lane);
         }
         staged_drain(lane);

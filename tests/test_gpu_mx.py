@@ -527,3 +527,35 @@ def test_quantize_keeps_special_blocks(ctx):
     codes, scales = run_image(ctx, g, [x])
     want_codes, want_scales = ref.quantize(x, "mx8")
     assert np.array_equal(scales, want_scales) and np.array_equal(codes, keep_nonzero(x.astype(np.float64), want_codes, "mx8"))
+
+
+@pytest.mark.parametrize("k", [4096, 4128, 8192, 1 << 20])
+def test_linear_long_contractions_of_one_sign(ctx, k):
+    """Terms that are all positive: tensor memory truncates, so the error of a sum kept there grows with the contraction.
+    At most 64 steps of the tensor cores, each losing up to one unit of 2^-23 of the running sum, lie between two additions
+    in FP32 registers, and those (one per 4096 terms, and one per slice) lose half a unit each."""
+    rng = np.random.default_rng(k)
+    m, n = 3, 8
+    held = []
+    for rows in (m, n):
+        codes, scales = random_held(rng, "mx4", (rows, k))
+        # scales from 2^-10 to 1 in every row: with equal ones the sums would be whole numbers of small units, and exact
+        held.append((codes & 0x77, (scales != 0) * rng.integers(117, 128, scales.shape).astype(np.uint8), (rows, k)))
+    xv, wv = (ref.values(*h[:2], "mx4", k) for h in held)
+    want = xv @ wv.T
+    got = linear(ctx, "f32", *held, None, None)
+    bound = (64 + (k / 4096 + 8) / 2) * 2.0 ** -23
+    assert (np.abs(got - want) <= bound * want).all(), float((np.abs(got - want) / want).max() * 2 ** 23)
+
+
+@pytest.mark.parametrize("form", [0, 1])
+def test_both_forms_of_the_product_at_every_size(form):
+    """The products above again, in a process that takes one-SM tiles (0) or two-SM tiles (1) whatever the size: single rows on two-SM
+    tiles, rows of results that are not whole 16 bytes, every activation, more tiles than SMs on one-SM tiles."""
+    import os
+    import subprocess
+    import sys
+    env = dict(os.environ, SYNAPTIK_CUDA_MX_PAIR=str(form))
+    ran = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
+                          "(linear or product or same_bits or share_scales) and not every_size"], env=env, capture_output=True, text=True, timeout=600)
+    assert ran.returncode == 0, ran.stdout[-3000:]
