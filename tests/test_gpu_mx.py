@@ -559,3 +559,10 @@ def test_both_forms_of_the_product_at_every_size(form):
     ran = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", "-k",
                           "(linear or product or same_bits or share_scales) and not every_size"], env=env, capture_output=True, text=True, timeout=600)
     assert ran.returncode == 0, ran.stdout[-3000:]
+
+
+@pytest.mark.parametrize("act", ACTIVATIONS)
+@pytest.mark.parametrize("kind", KINDS)
+def test_linear_activations_on_many_rows(ctx, kind, act):
+    """More tiles than SMs, and rows of 16-bit results that are not whole 16 bytes."""
+    check_linear(ctx, kind, (2100,), 64, 1100, act)
