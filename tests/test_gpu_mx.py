@@ -566,3 +566,30 @@ def test_both_forms_of_the_product_at_every_size(form):
 def test_linear_activations_on_many_rows(ctx, kind, act):
     """More tiles than SMs, and rows of 16-bit results that are not whole 16 bytes."""
     check_linear(ctx, kind, (2100,), 64, 1100, act)
+
+
+@pytest.mark.parametrize("act", ACTIVATIONS[1:])
+def test_activation_gradient_of_every_held_value(ctx, act):
+    """All codes under all scales.  In units of 2^-24: an exponential of -x is off by 4 + 2.35 x of itself, and by x per unit of
+    its argument's rounding (none for x = |z| or 2 |z|, 1 for z^2 / 2, 4 for the tanh form's u); the divisions, polynomials and
+    the other roundings by 24 of the sum of the slope's terms.  Below 2^-125 results leave the normal numbers."""
+    codes = np.tile(np.arange(256, dtype=np.uint8).reshape(8, 32), (255, 1))
+    codes[(codes & 127) == 127] = 0
+    scales = np.zeros((8 * 255, 4), dtype=np.uint8)
+    scales[:, 0] = np.repeat(np.arange(255), 8)
+    z = ref.values(codes, scales, "mx8", 32)
+    g = GraphBuilder()
+    held, u = g.mx_feed("mx8", z.shape), g.feed(F32, z.shape)
+    g.publish(g.mx_activation_gradient(act, held, u))
+    got, = run_image(ctx, g, [codes, scales, np.ones(z.shape, dtype=np.float32)])
+    want = ref.slope(act, z)
+    a = np.minimum(np.abs(z), 120)
+    zc = np.clip(z, -120, 120)
+    u = np.abs(2 * ref.C * (zc + 0.044715 * zc ** 3))
+    near = lambda x: np.exp(-x) / (1 + np.exp(-x)) ** 2         # noqa: E731
+    x, roundings, terms = {"tanh": (2 * a, 0, want), "sigmoid": (a, 0, want), "silu": (a, 0, ref.sigmoid(zc) + a * near(a)),
+                           "gelu_tanh": (u, 4, ref.sigmoid(np.copysign(u, zc)) + a * near(u) * 2 * ref.C * (1 + 3 * 0.044715 * a * a)),
+                           "gelu": (a * a / 2, 1, ref.slope("gelu", zc) + 2 * a * np.exp(-a * a / 2) / np.sqrt(2 * np.pi))}[act]
+    bound = 2.0 ** -24 * (4 + (2.35 + roundings) * x + 24) * np.abs(terms) + 2.0 ** -125
+    assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) / bound).max())
+    assert np.abs(got - want).max() <= 6 * 2.0 ** -24
