@@ -146,7 +146,10 @@ SYNAPTIK_CUDA_API int32_t synaptik_cuda_host_free(void *pointer);
  * `program` is one little-endian "SCU1" image (layout in synaptik_b200/csrc/program.hpp) that
  * lists a whole backend partition in topological order: value descriptors (dtype, shape,
  * element strides, role), nodes (operation wire code, attributes, input and output value
- * references), the ordered feed values and the ordered publication values.  Creation validates
+ * references), the ordered feed values and the ordered publication values.  Data type code 7 (U8) and
+ * operations 37 to 41 (block-scaled 4-bit and 8-bit tensors, described there) extend what the image may
+ * hold without changing a symbol: a library of this ABI version that lacks them refuses such an image with
+ * UNSUPPORTED_OPERATION, also in synaptik_cuda_program_describe, which needs no GPU.  Creation validates
  * the image, lowers it to fused kernel launches and reserves every intermediate; it performs no
  * device work on the hot path.  run binds `input_count` buffers to the feeds and `output_count`
  * buffers to the publications in image order (the role BoundInvocation.executeBound plays,

@@ -217,7 +217,7 @@ cudaError_t mx_activation_gradient(cudaStream_t s, int act, DType dtype, const u
 // says so the product runs on two-SM tiles and needs the scales of both operands in tiles (else x_tiles = w_tiles = null).
 // after_x: the launch before this one in the stream was the mx_quantize that makes x, or an mx_tile_scales behind it; this
 // one may then start early.  mx_tile_scales does not wait for it before it reads: the scales must be older than that launch.
-bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count);
+bool mx_linear_tiled(int64_t m, int64_t n, int sm_count);
 int64_t mx_tile_bytes(int64_t rows, int64_t k);
 cudaError_t mx_tile_scales(cudaStream_t s, const uint8_t *scales, int64_t rows, int64_t k, uint8_t *tiles, bool after_x);
 cudaError_t mx_linear(cudaStream_t s, DType dtype, int act, int64_t m, int64_t n, int64_t k, const uint8_t *x, const uint8_t *x_scales,

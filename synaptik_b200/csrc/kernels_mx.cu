@@ -1123,7 +1123,6 @@ template <int PIECES> struct MxGradConfig {
 
 struct MxGrad {
     int n, k;
-    int64_t rows;
     int staged;                         // rows of `out` can be written by TMA
     int tiles_n, whole_tiles, units;    // units: the whole tiles, then `slices` per tile that is left
     int slices, stages, stages_per_slice;       // of MX_ROWS rows
@@ -1693,7 +1692,7 @@ static int forced_mx_pair() {
 // Two-SM tiles where the one-SM tiles of 128 x 128 would take more than one wave: measured with the quantisation of x, K =
 // 4096: 512 x 4096 (128 tiles) 34.6 us on one-SM tiles and 32.8 on two-SM ones, 4096 x 128 (32) 31.9 and 41.4, 1024 x 4096
 // (256) 60.6 and 34.2, 1 x 4096 15.4 and 29.7.
-bool mx_linear_tiled(int64_t m, int64_t n, int64_t k, int sm_count) {
+bool mx_linear_tiled(int64_t m, int64_t n, int sm_count) {
     if (sm_count < 2) return false;
     if (forced_mx_pair() >= 0) return forced_mx_pair() == 1;
     return m > 128 && ((m + 127) / 128) * ((n + 127) / 128) > sm_count;
@@ -1894,7 +1893,7 @@ cudaError_t mx_weight_gradient(cudaStream_t s, DType dtype, int64_t rows, int64_
     CUtensorMap map_g, map_x;
     if (!make_piece_map(&map_g, p.direct ? g : g_planes, p.pieces, rows, n, p.direct ? n : p.g_pitch) || !make_piece_map(&map_x, x_plane, 0, rows, x_pitch, x_pitch)) return cudaErrorInvalidValue;
     MxGrad prm = {};
-    prm.n = (int)n; prm.k = (int)k; prm.rows = rows;
+    prm.n = (int)n; prm.k = (int)k;
     prm.tiles_n = p.tiles_n; prm.whole_tiles = p.whole_tiles; prm.units = (int)units;
     prm.slices = p.slices; prm.stages = p.stages; prm.stages_per_slice = p.stages_per_slice;
     prm.out = out; prm.partial = (float *)((uint8_t *)workspace + p.g_bytes + p.x_bytes); prm.error_word = error_word;

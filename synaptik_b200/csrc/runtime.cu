@@ -494,7 +494,7 @@ int32_t prepare_executable(Executable *x) {
             se.tc = kern::tc_gemm_prepare(se.tc_p, se.tc_q, se.tc_m, se.tc_n, st.k, ctx->sm_count, mode, &status);
             if (se.tc) workspace_floats = std::max(workspace_floats, kern::tc_gemm_workspace_floats(se.tc));
             if (!se.tc) return status;
-        } else if (st.kind == StepKind::MX_LINEAR && st.m > 0 && kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) {
+        } else if (st.kind == StepKind::MX_LINEAR && st.m > 0 && kern::mx_linear_tiled(st.m, st.n, ctx->sm_count)) {
             for (int operand = 0; operand < 2; operand++) {
                 const int64_t bytes = kern::mx_tile_bytes(operand ? st.n : st.m, st.k);
                 MxTiles &tiles = x->mx_tiles[std::make_pair(operand ? st.scale_b : st.scale_a, mx_blocks(st.k))];
@@ -801,7 +801,7 @@ int32_t enqueue_executable(Executable *x, const Binding &bind) {
                 for (int operand = 0; operand < 2; operand++) {
                     const int value = operand ? st.scale_b : st.scale_a;
                     auto it = x->mx_tiles.find(std::make_pair(value, mx_blocks(st.k)));
-                    if (it == x->mx_tiles.end() || !kern::mx_linear_tiled(st.m, st.n, st.k, ctx->sm_count)) continue;
+                    if (it == x->mx_tiles.end() || !kern::mx_linear_tiled(st.m, st.n, ctx->sm_count)) continue;
                     if (it->second.last_run != x->run_counter) {
                         // W's may be tiled beside the launch that makes x; x's own scales are that launch's output
                         LAUNCH(kern::mx_tile_scales(s, (const uint8_t *)ptr(value), operand ? st.n : st.m, st.k, it->second.ptr, after_x && operand == 1));
