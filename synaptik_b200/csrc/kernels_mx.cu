@@ -37,8 +37,9 @@ template <int KIND> __device__ __forceinline__ typename MxElement<KIND>::type mx
 // Element-wise passes, bound by HBM.  A thread owns a group of 8 consecutive elements (16 where the quantiser reads
 // 16-bit types), so 2 or 4 lanes own a block of 32: 16 or 32 bytes of the wide tensor per thread and access, the
 // block's largest magnitude by one or two shuffles.  A row has `per_row` groups, counted over the padded scales (a
-// multiple of 8 or 16), so a block never straddles two warps.  65536 x 4096 FLOAT32, 8 bits: quantisation 225 us (6.0 TB/s),
-// restoration 240 us (5.6 TB/s), activation gradients 382 us (6.3 TB/s).
+// multiple of 8 or 16), so a block never straddles two warps.  65536 x 4096 FLOAT32, 8 bits: quantisation 220 us (6.1 TB/s),
+// restoration 240 us (5.6 TB/s), activation gradients 381 (ReLU) to 408 us (SiLU; 5.9 to 6.4 TB/s).  16-bit types are bound by their instructions:
+// BFLOAT16 to 4 bits 146 us (4.7 TB/s), ReLU gradient 312 us (4.3 TB/s).
 // ------------------------------------------------------------------------------------------------
 // I: int64_t, or uint32_t where the groups of the whole tensor, and a step beyond them, can be counted with it.
 template <typename I> struct MxRows {
@@ -770,8 +771,8 @@ __global__ void __launch_bounds__(256, 1) mx_linear_few_kernel(const __grid_cons
 // (128 + 256) x 128 bytes of codes into shared memory and the tensor core read them out again within 512 clocks of
 // MMA, more than shared memory delivers; the pair moves a third less.  Accumulators take 256 columns of tensor memory
 // and the scales of the stages in flight most of the rest, so there is one accumulator: the epilogue warps first copy
-// it to registers, hand it back, and finish the tile under the next one's main loop.  37888 x 4096 x 4096: 287 us, 4.4
-// PFLOP/s; without any load the MMAs alone take 232 us.
+// it to registers, hand it back, and finish the tile under the next one's main loop.  37888 x 4096 x 4096: 297 us
+// in a burst (4.3 PFLOP/s), 338 us in a row under the power cap (1.64 GHz); an earlier build's MMAs alone, without any load, took 232.
 // Scales: TMA fetches their tiles into a ring of their own, further ahead than the codes, and four warps move them on
 // to tensor memory through registers as soon as a stage's columns are free, so they lie there before the codes land.
 // tcgen05.cp from shared memory shares the tensor pipe with the MMAs: its six copies per k-block cost 60 of 334 us on
@@ -1094,8 +1095,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // (tcgen05 kind::f16, BFLOAT16 operands, FP32 accumulators), two-SM tiles of 256 n x 256 k (784 columns as
 // four tiles of 224 start off 128-byte lines and took 12 % longer than four of 256).
 //   An E4M3 element under a power-of-two scale is a BFLOAT16 number as it stands (below 2^-133 it rounds), so the
-// checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly: 8 + 8 + 8 significand bits for
-// FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
+// checkpoint costs one operand.  g is cut into BFLOAT16 pieces that add up to it exactly (apart from what lies below 2^-133):
+// 8 + 8 + 8 significand bits for FLOAT32 (three products), 8 + 3 for FLOAT16 (two), one for BFLOAT16.  Every product is then exact; a FLOAT32 gradient
 // takes three products at the BFLOAT16 rate where a split into TF32 numbers would take three at half of it.
 //   mx_pieces_kernel writes the pieces and the checkpoint's values to scratch (10 bytes to move per element of a FLOAT32 g, 3
 // per element of x; BFLOAT16 gradients whose rows TMA can address stay where they are), once each.  Converting inside the
@@ -1106,8 +1107,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_PAIR_THREADS, 1) 
 // of kChunk stages, which the epilogue warps add into FP32 registers: two accumulators in turn.
 //   Tiles that do not fill a wave of block pairs are cut into slices of the rows; their sums go to scratch and are
 // added in ascending order by a last launch.
-//   8192 x 4096 x 4096: FLOAT32 620 us (1.33 PFLOP/s of BFLOAT16 products, the sustained rate under the power cap is 1.39),
-// BFLOAT16 257 us (1.07: the operand loads of one product per stage do not keep up).
+//   8192 x 4096 x 4096, whole calls in a row: FLOAT32 645 to 671 us (1.25 PFLOP/s of BFLOAT16 products with the conversion; the sustained rate
+// under the power cap is 1.39), BFLOAT16 254 us (1.08: the operand loads of one product per stage do not keep up).
+//   Sums of 65536 positive terms fall short by 17 units of 2^-23 (20 at most), of 1024 in BFLOAT16 or 512 in FLOAT16, one partial
+// sum without a break, by 31 at most; half as many MMAs per partial sum cost 5 % (416 -> 437 us on 65536 x 784 x 4096, one call at a time).
 // ------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 64;             // rows per stage
 constexpr int MX_GRAD_THREADS = 384;    // warp 0 TMA, warp 1 MMA, warps 4-11 epilogue
