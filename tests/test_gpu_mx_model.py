@@ -260,3 +260,56 @@ def test_small_activations_beside_large_ones_keep_their_gradient(ctx):
     # four equal rows: each result is a sum of at most 12 exact products, one rounding each
     assert np.allclose(grads[1][0], grads[0][0], rtol=16 * 2.0 ** -23, atol=0)
     assert np.allclose(grads[1][1], grads[0][1], rtol=16 * 2.0 ** -23, atol=0)
+
+
+@pytest.mark.parametrize("dims,batch,activation", [([256, 512, 512, 512, 16], 2048, "relu"), ([100, 300, 260, 10], 700, "gelu"), ([64, 384, 384, 384, 384, 8], 1024, "tanh")])
+def test_shared_memory_does_not_change_a_bit(ctx, dims, batch, activation):
+    """Intermediates of a program with 8-bit checkpoints share memory.  Published ones have memory of their own, and who writes
+    the operand planes of a product changes which of them live when: the gradients are the same bits."""
+    rng = np.random.default_rng(batch)
+    x, target = rng.standard_normal((batch, dims[0])).astype(np.float32), rng.integers(0, dims[-1], batch).astype(np.int32)
+    params = [(rng.standard_normal(s) / np.sqrt(s[-1])).astype(np.float32) for l in range(len(dims) - 1) for s in ((dims[l + 1], dims[l]), (dims[l + 1],))]
+    results = []
+    try:
+        for publish in (False, True):
+            for fused in (1, 0, 2, 3):
+                for timed in (0, 1):
+                    ctx.set_option("fused_planes", fused)
+                    ctx.set_option("time_steps", timed)
+                    graph = program.mlp_training_graph(dims, batch, "ce", activation=activation, publish_activations=publish, checkpoints="mx8")
+                    exe = native.Executable(ctx, graph.image)
+                    feeds = [ctx.upload(a) for a in [x, target, np.ones(1, np.float32)] + params]
+                    outs = [ctx.buffer(max(int(np.prod(graph.shapes[name])) * 4, 4)) for name in graph.publications]
+                    for _ in range(2):
+                        exe.enqueue(feeds, outs)
+                    exe.finish()
+                    got = {name: b.download(np.float32, graph.shapes[name]) for name, b in zip(graph.publications, outs)}
+                    results.append({name: v for name, v in got.items() if name in graph.publications[:1 + len(params)]})
+                    exe.close()
+                    for b in feeds + outs:
+                        b.close()
+    finally:
+        ctx.set_option("fused_planes", 1)
+        ctx.set_option("time_steps", 0)
+    assert len(results[0]) == 1 + len(params)
+    for other in results[1:]:
+        assert other.keys() == results[0].keys()
+        assert all(np.array_equal(other[name], results[0][name]) for name in other)
+
+
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("activation", ["relu", "tanh", "sigmoid", "silu", "gelu_tanh", "gelu"])
+def test_checkpointed_training_of_every_activation(ctx, activation, bias):
+    """Against FLOAT32 checkpoints: each held value is off by at most 2^-4 of itself, each slope likewise."""
+    dims, batch = [33, 96, 65, 7], 130
+    rng = np.random.default_rng(6)
+    x, target = rng.standard_normal((batch, dims[0])).astype(np.float32), rng.standard_normal((batch, dims[-1])).astype(np.float32)
+    grads = []
+    for kind in (None, "mx8"):
+        model = nn.Model(dims, ctx, seed=5, bias=bias, activation=activation, checkpoints=kind)
+        model.configure_training("mse", nn.Sgd(0.01))
+        grads.append(model.gradients(x, target))
+        model.close()
+    assert grads[0][0] == grads[1][0]
+    for a, b in zip(grads[1][1], grads[0][1]):
+        assert np.linalg.norm(a - b) <= 0.25 * np.linalg.norm(b)
