@@ -593,3 +593,49 @@ def test_activation_gradient_of_every_held_value(ctx, act):
     bound = 2.0 ** -24 * (4 + (2.35 + roundings) * x + 24) * np.abs(terms) + 2.0 ** -125
     assert (np.abs(got - want) <= bound).all(), float((np.abs(got - want) / bound).max())
     assert np.abs(got - want).max() <= 6 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("x_byte,w_byte", [(0, 227), (254, 0), (227, 0), (1, 200), (254, 20), (127, 127)])
+def test_linear_scales_at_the_ends_of_their_range(ctx, x_byte, w_byte):
+    """The least and the largest power of two as a scale, against one that brings the result back into range."""
+    rng = np.random.default_rng(x_byte)
+    m, n, k = 150, 140, 160
+    held = []
+    for rows, byte in ((m, x_byte), (n, w_byte)):
+        codes, scales = random_held(rng, "mx4", (rows, k))
+        held.append((codes, np.where(np.arange(scales.shape[1]) < k // 32, byte, 0).astype(np.uint8) + np.zeros_like(scales), (rows, k)))
+    got = linear(ctx, "f32", *held, None, None)
+    xv, wv = (ref.values(*h[:2], "mx4", k) for h in held)
+    want, s = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    assert (np.abs(got - want) <= (k / 32 + 4) * 2.0 ** -23 * s + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("fmt", ["mx4", "mx8"])
+def test_quantize_broadcast_views(ctx, kind, fmt):
+    """EXPAND along rows, along columns and of a scalar: strides of zero."""
+    rng = np.random.default_rng(3)
+    for source, shape in [((1, 96), (50, 96)), ((50, 1), (50, 96)), ((1, 1), (7, 70)), ((3, 1, 40), (3, 9, 40)), ((3, 9, 1), (3, 9, 33)), ((), (5, 64))]:
+        fed, exact = ref.stored(kind, mixed(rng, *source) if source else np.float32(2.7).reshape(()))
+        g = GraphBuilder()
+        held = g.mx_quantize(g.expand(g.feed(ref.STORAGE[kind], source), shape), fmt)
+        g.publish(held.codes)
+        g.publish(held.scales)
+        codes, scales = run_image(ctx, g, [fed])
+        want_codes, want_scales = ref.quantize(np.broadcast_to(exact, shape), fmt)
+        assert np.array_equal(scales, want_scales) and np.array_equal(codes, want_codes), (source, shape)
+
+
+@pytest.mark.parametrize("exponent", [-100, -112, -118, -126, -140])
+def test_weight_gradient_of_tiny_gradients(ctx, exponent):
+    """What lies below 2^-133 in an element of a FLOAT32 gradient is lost, and nothing else."""
+    rng = np.random.default_rng(-exponent)
+    rows, k, n = 300, 300, 264
+    held = ref.quantize((rng.standard_normal((rows, k)) * 2.0 ** 30).astype(np.float32), "mx8")
+    up = np.ldexp(rng.standard_normal((rows, n)), exponent).astype(np.float32)
+    x = ref.values(*held, "mx8", k)
+    up64 = up.astype(np.float64)
+    want, s = up64.T @ x, np.abs(up64).T @ np.abs(x)
+    got = weight_gradient(ctx, "f32", held, (rows, k), up, n)
+    bound = (rows / 16 * 4 + 4) * 2.0 ** -23 * s + 2.0 ** -133 * np.abs(x).sum(0) + 2.0 ** -149
+    assert (np.abs(got - want) <= bound).all()
