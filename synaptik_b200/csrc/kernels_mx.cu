@@ -577,7 +577,7 @@ struct MxLinear {
 // One block multiplies 128 rows of W by BN rows of x over a slice of the contraction; the up to eight blocks of a
 // cluster share a tile and add their partial sums, in ascending order, through each other's shared memory.  With
 // W as the M operand a tile wastes no MMA rows on absent rows of x, and the result leaves with 32 consecutive
-// columns per warp without a transposition.  Bound by latency: one row of 4096 against 4096 x 4096 takes 12.9 us per call
+// columns per warp without a transposition.  Bound by latency: one row of 4096 against 4096 x 4096 takes 12.7 to 15.3 us per call
 // with its quantisation, 11 of them on the host.  Two warps fetch the scales word by word, with 4-byte asynchronous
 // copies, into the order of tensor memory; the issuing thread sends them there with tcgen05.cp in front of the MMAs.
 template <int BN> struct MxFewConfig {
